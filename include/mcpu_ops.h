@@ -33,7 +33,8 @@ typedef enum mcpuDtype {
   MCPU_BOOL = 6,
   MCPU_FLOAT64 = 7,
   MCPU_INT8 = 8,
-  MCPU_INT16 = 9
+  MCPU_INT16 = 9,
+  MCPU_FLOAT8_E4M3 = 10 /* held in key / value caches only */
 } mcpuDtype;
 
 typedef enum mcpuScoring {
@@ -423,6 +424,122 @@ OPENREG_EXPORT orError_t mcpu_vllm_bad_words(void* logits, int dtype, int64_t nu
                                              int64_t max_seq_len, const int32_t* prompt_len,
                                              const int32_t* total_len, const int32_t* input_ids,
                                              const int32_t* expanded_local_pos, orStream_t stream);
+
+/*
+ * The attention path of a serving step: rotary positions, a paged key / value
+ * cache that is quantised as it is written, its read-back, and attention over
+ * it for single tokens, chains and trees of drafted tokens.  No counterpart
+ * in the reference, whose mcpu device leaves attention to vLLM's CPU backend;
+ * the Python signatures follow vLLM's (rotary_embedding, reshape_and_cache,
+ * gather_cache).
+ *
+ * mcpuKvCache: key and value are [num_blocks, block_size, kv_heads,
+ *   head_size] with strides (in elements) for block, slot in the block and
+ *   head, head_size contiguous; base and strides multiples of 16 bytes,
+ *   head_size a multiple of 16, at most 512.  dtype is the tensors' own type
+ *   (bf16 / fp16), MCPU_FLOAT8_E4M3 or MCPU_INT8.  8-bit caches hold
+ *   q = rn(x / s) with an fp32 scale s found at block*stride[0] +
+ *   slot*stride[1] + head*stride[2]: MCPU_KV_SCALE_GIVEN scales (positive,
+ *   strides of 0 where one is shared: per head or per cache) are read,
+ *   MCPU_KV_SCALE_TOKEN ones (one per token and head) are written with the
+ *   row: s = rn(max|x| / 448) (e4m3) or rn(max|x| / 127) (int8).  A row of
+ *   zeros has s = 0.  With token scales, a row that holds an infinity or a
+ *   NaN reads back as NaN throughout; with given scales values beyond the
+ *   range saturate, NaN stays NaN in e4m3 and becomes 0 in int8.
+ *
+ * mcpu_rotary_embedding: for each token t, with row = cos_sin_cache[
+ *   positions[t]] (fp32, rotary_dim/2 cosines then rotary_dim/2 sines), every
+ *   head's pairs (a, b) -- (x[i], x[i + rotary_dim/2]) when is_neox, else
+ *   (x[2i], x[2i+1]) -- become (a cos - b sin, b cos + a sin), rounded once,
+ *   in place; dimensions from rotary_dim on are not touched.  Heads lie at
+ *   token and head strides (elements), dimensions contiguous; query and key
+ *   do not overlap; num_kv_heads may be 0.  fp32, bf16 or fp16.  A position
+ *   outside [0, max_position) leaves the token and sets mcpu_device_error.
+ *
+ * mcpu_rotary_reshape_and_cache: query rotated in place; the rotated key
+ *   (rounded once to its type; the key tensor itself is left as it is) and
+ *   the value written to the cache at slot_mapping[t] = block*block_size +
+ *   slot.  Cache contents are those of mcpu_rotary_embedding on the key
+ *   followed by the write alone.  rotary_dim a multiple of 16, at most
+ *   head_size; rotary_dim = 0 (and num_heads = 0, positions and cos_sin_cache
+ *   NULL) writes the key as it is.  A negative slot writes nothing (padded
+ *   token); one beyond the cache, or a position out of range, writes nothing
+ *   and sets mcpu_device_error.  No two tokens of a call share a slot.
+ *
+ * mcpu_gather_cache: row t of key_out / value_out [num_tokens, kv_heads,
+ *   head_size] (contiguous, `dtype`) = token seq_starts[b] + t -
+ *   cu_seq_lens[b] of sequence b, cu_seq_lens[b] <= t < cu_seq_lens[b+1]
+ *   (int32 [batch + 1], from 0, not falling; seq_starts int32 [batch] or
+ *   NULL for 0), found through block_table (int32 [batch, table_width] rows
+ *   table_stride apart) and dequantised: rn(q * s).  Rows from
+ *   cu_seq_lens[batch] on are left as they are.  A page outside the table or
+ *   the cache leaves the row and sets mcpu_device_error.
+ */
+enum { MCPU_KV_SCALE_NONE = 0, MCPU_KV_SCALE_GIVEN = 1, MCPU_KV_SCALE_TOKEN = 2 };
+
+typedef struct mcpuKvCache {
+  void* key;
+  void* value;
+  float* k_scale;
+  float* v_scale;
+  int64_t num_blocks;
+  int64_t key_stride[3];
+  int64_t value_stride[3];
+  int64_t k_scale_stride[3];
+  int64_t v_scale_stride[3];
+  int32_t block_size, kv_heads, head_size, dtype, scale_mode, reserved;
+} mcpuKvCache;
+
+OPENREG_EXPORT orError_t mcpu_rotary_embedding(const int64_t* positions, int64_t num_tokens, void* query,
+                                               int num_heads, int64_t query_token_stride,
+                                               int64_t query_head_stride, void* key, int num_kv_heads,
+                                               int64_t key_token_stride, int64_t key_head_stride, int rotary_dim,
+                                               const float* cos_sin_cache, int64_t max_position, int is_neox,
+                                               int dtype, orStream_t stream);
+OPENREG_EXPORT orError_t mcpu_rotary_reshape_and_cache(
+    const int64_t* positions, int64_t num_tokens, void* query, int num_heads, int64_t query_token_stride,
+    int64_t query_head_stride, const void* key, int64_t key_token_stride, int64_t key_head_stride,
+    const void* value, int64_t value_token_stride, int64_t value_head_stride, int rotary_dim,
+    const float* cos_sin_cache, int64_t max_position, int is_neox, int dtype, const int64_t* slot_mapping,
+    const mcpuKvCache* cache, orStream_t stream);
+OPENREG_EXPORT orError_t mcpu_gather_cache(const mcpuKvCache* cache, const int32_t* block_table,
+                                           int64_t table_stride, int64_t table_width, int64_t batch,
+                                           const int32_t* cu_seq_lens, const int32_t* seq_starts, void* key_out,
+                                           void* value_out, int64_t num_tokens, int dtype, orStream_t stream);
+
+/*
+ * tree_attention: attention over the paged cache for the new tokens of a
+ * decoding step.  query [num_tokens, num_heads, head_size] (bf16 / fp16, the
+ * cache's other type; head_size 64 or 128, contiguous) holds the requests'
+ * new tokens one request after the other: request b has tokens
+ * cu_query_lens[b] .. cu_query_lens[b+1] (int32 [batch + 1]), at most
+ * max_query_len (<= MCPU_TREE_MAX_QUERIES) of them, and seq_lens[b] keys in
+ * the cache (int32), its n new tokens the last n of them.  Query i sees every
+ * key of the context and, of the new ones, key d where bit d % 64 of
+ * tree_mask[token][d / 64] is set (int64 rows mask_stride apart, mask_words
+ * words); tree_mask NULL: d <= i.  Query head h reads key / value head
+ * h / (num_heads / kv_heads).
+ *   out = softmax(scale * q . k) v over the keys seen, rounded once;
+ *   lse (fp32 [num_tokens, num_heads], or NULL) = log sum exp of the scores.
+ * A query that sees no key gives zeros and -inf; what unseen keys, values and
+ * slots behind seq_lens hold (NaN included) does not matter.  Tokens outside
+ * every request are left as they are.  A request that does not fit (lengths
+ * negative or falling, seq_lens[b] < n or beyond the block table, more tokens
+ * than the mask has bits) gives zeros, one with a page outside the cache
+ * reads block 0 instead; both set mcpu_device_error.
+ * workspace: mcpu_tree_attention_workspace_bytes bytes, 16-byte aligned, of
+ * any content; calls that may run at the same time have one each.
+ */
+#define MCPU_TREE_MAX_QUERIES 256
+
+OPENREG_EXPORT orError_t mcpu_tree_attention(
+    const void* query, int64_t query_token_stride, int64_t query_head_stride, int64_t num_tokens, int num_heads,
+    void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, int dtype, const mcpuKvCache* cache,
+    const int32_t* block_table, int64_t table_stride, int64_t table_width, int64_t batch, const int32_t* seq_lens,
+    const int32_t* cu_query_lens, int64_t max_query_len, const int64_t* tree_mask, int64_t mask_stride,
+    int64_t mask_words, float scale, void* workspace, uint64_t workspace_bytes, orStream_t stream);
+OPENREG_EXPORT orError_t mcpu_tree_attention_workspace_bytes(int64_t max_query_len, int num_heads, int num_kv_heads,
+                                                             int head_size, uint64_t* bytes);
 
 /* *flag = 1 if a kernel on the current device (tensor-core GEMM, TMA-fed
  * router or bulk-copy-fed rms_norm) gave up on a bounded wait, or a gather /

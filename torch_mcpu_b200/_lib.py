@@ -108,6 +108,17 @@ SIGNATURES = {
                                     c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "mcpu_vllm_bincount": (c_int, [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
                                    c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p]),
+    "mcpu_rotary_embedding": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int, c_int64,
+                                      c_int64, c_int, c_void_p, c_int64, c_int, c_int, c_void_p]),
+    "mcpu_rotary_reshape_and_cache": (c_int, [c_void_p, c_int64, c_void_p, c_int, c_int64, c_int64, c_void_p, c_int64,
+                                              c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_int64, c_int,
+                                              c_int, c_void_p, c_void_p, c_void_p]),
+    "mcpu_gather_cache": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p,
+                                  c_void_p, c_int64, c_int, c_void_p]),
+    "mcpu_tree_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int64, c_int64, c_void_p,
+                                    c_int, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                    c_void_p, c_int64, c_int64, c_float, c_void_p, ctypes.c_uint64, c_void_p]),
+    "mcpu_tree_attention_workspace_bytes": (c_int, [c_int64, c_int, c_int, c_int, ctypes.POINTER(ctypes.c_uint64)]),
     "mcpu_device_error": (c_int, [ctypes.POINTER(c_int), c_int]),
     "mcpu_mem_get_info": (c_int, [c_int, ctypes.POINTER(ctypes.c_size_t), ctypes.POINTER(ctypes.c_size_t)]),
     "mcpu_mem_pool_reserved": (c_int, [c_int, ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)]),

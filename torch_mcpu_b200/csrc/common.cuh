@@ -48,6 +48,8 @@ orError_t launch(const int32_t* topk_ids, long long numel, int E, int bs, int32_
                  cudaStream_t st);
 }  // namespace moe
 orError_t sampler_read_error(int* flag, bool reset);
+orError_t kv_read_error(int* flag, bool reset);
+orError_t attn_read_error(int* flag, bool reset);
 
 inline cudaStream_t as_cuda(orStream_t s) {
   return reinterpret_cast<cudaStream_t>(s);

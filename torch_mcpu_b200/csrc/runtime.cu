@@ -146,7 +146,13 @@ orError_t mcpu_device_error(int* flag, int reset) {
   int sp = 0;
   e = sampler_read_error(&sp, reset != 0);
   if (e != orSuccess) return e;
-  *flag = a | b | c | d | m | sp;
+  int kv = 0;
+  e = kv_read_error(&kv, reset != 0);
+  if (e != orSuccess) return e;
+  int at = 0;
+  e = attn_read_error(&at, reset != 0);
+  if (e != orSuccess) return e;
+  *flag = a | b | c | d | m | sp | kv | at;
   return orSuccess;
 }
 

@@ -1,0 +1,1038 @@
+// Attention over the paged key / value cache for the tokens of a decoding
+// step: one token per request, a chain, or a tree of drafted tokens whose
+// keys and values are already in the cache behind the request's context.
+//
+// Mathematics.  Request b has length L (its n new tokens included) and
+// context C = L - n.  Its query i sees key j where j < C, or where bit j - C
+// of the query's mask words is set (without a mask: j - C <= i).  Per query
+// head: s_j = scale * q.k_j, o = sum p_j v_j / sum p_j, p_j = 2^(s_j log2 e -
+// m), computed in one pass over the keys with the running maximum m and sum
+// kept in fp32; a query that sees nothing (or only scores of -inf) gives
+// zeros and lse = -inf.
+//
+// Bound by HBM while few rows share a key: the rows of one key / value head
+// are the request's queries times the query heads that share it.
+//
+// Work split.  The unit is one tile of TN keys against one tile of MT rows of
+// a (request, key / value head).  Units are numbered request by request, and
+// each of a fixed grid of blocks takes an equal contiguous run of them, found
+// from the lengths on the device: any mix of lengths fills the GPU evenly, and
+// a captured graph stays balanced when the lengths change.  A row tile whose
+// keys lie in several blocks leaves partial sums in a workspace (at most two
+// per block), which a second kernel, launched ahead and waiting on the first
+// (programmatic dependent launch), joins in key order: results do not depend
+// on timing.
+//
+// 8-bit caches are multiplied as fp16, which holds e4m3 and int8 values
+// exactly: the scales of the keys go onto the scores, those of the values onto
+// the probabilities.
+#include <math.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "kv_cache.cuh"
+
+namespace mcpu {
+namespace attn {
+
+__device__ int g_attn_error = 0;
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr unsigned kFull = 0xFFFFFFFFu;
+
+enum Kind { kSame = 0, kE4M3 = 1, kInt8 = 2 };
+
+struct Params {
+  const void* q;
+  long long q_tok, q_head;
+  void* out;
+  long long o_tok, o_head;
+  float* lse;  // [tokens, heads] or NULL
+  mcpuKvCache c;
+  const int* table;
+  long long table_stride;
+  int table_width, block_log2;  // block_log2 < 0: not a power of two
+  const int* seq_lens;
+  const int* cu;
+  const long long* mask;  // [tokens, words] or NULL
+  long long mask_stride;
+  int mask_words;
+  int batch, tokens, kv_heads, group;
+  float scale_log2;
+  int min_share;
+  float* part_o;   // [grid][2][MT][D]
+  float* part_ml;  // [grid][2][MT][2]
+};
+
+// ---------------------------------------------------------------- schedule
+struct Request {
+  int first, n, len;  // first token, new tokens, length; len = 0: nothing to do
+};
+
+__device__ __forceinline__ Request request(const Params& p, int b) {
+  Request r;
+  r.first = p.cu[b];
+  const int end = p.cu[b + 1];
+  r.n = end - r.first;
+  r.len = p.seq_lens[b];
+  const bool fits = r.first >= 0 && r.n >= 0 && end <= p.tokens;
+  const long long room = static_cast<long long>(p.table_width) * p.c.block_size;
+  const bool words = p.mask == nullptr || r.n <= 64 * p.mask_words;
+  if (!fits || r.len < r.n || r.len > room || !words) {
+    atomicOr(&g_attn_error, 1);
+    if (!fits) r.first = 0, r.n = 0;
+    r.len = 0;
+  }
+  if (r.n == 0) r.len = 0;
+  return r;
+}
+
+template <int MT, int TN>
+struct Sched {
+  static __device__ __forceinline__ int tiles(const Request& r) { return (r.len + TN - 1) / TN; }
+  static __device__ __forceinline__ int row_tiles(const Params& p, const Request& r) {
+    return (r.n * p.group + MT - 1) / MT;
+  }
+  static __device__ __forceinline__ int units(const Params& p, const Request& r) {
+    return r.len == 0 ? 0 : p.kv_heads * row_tiles(p, r) * tiles(r);
+  }
+
+  // Block-wide: total units, then the request that holds `unit` (a function of
+  // the total) and the units before it.
+  template <int NT, typename F>
+  static __device__ __forceinline__ void locate(const Params& p, F&& unit_of, int* red, int& total, int& unit, int& b,
+                                                int& before) {
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int mine = 0;
+    for (int i = tid; i < p.batch; i += NT) mine += units(p, request(p, i));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kFull, mine, o);
+    if (lane == 0) red[warp] = mine;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NT / 32; ++w) total += red[w];
+    unit = unit_of(total);
+    int* found = red + NT / 32;
+    if (tid == 0) found[0] = p.batch, found[1] = total;
+    __syncthreads();
+    int base = 0;
+    for (int i0 = 0; i0 < p.batch; i0 += NT) {
+      const int i = i0 + tid;
+      const int u = i < p.batch ? units(p, request(p, i)) : 0;
+      int incl = u;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(kFull, incl, o);
+        if (lane >= o) incl += v;
+      }
+      if (lane == 31) red[warp] = incl;
+      __syncthreads();
+      int off = base;
+#pragma unroll
+      for (int w = 0; w < NT / 32; ++w) {
+        off += w < warp ? red[w] : 0;
+        base += red[w];
+      }
+      const int from = off + incl - u;
+      if (unit >= from && unit < from + u) found[0] = i, found[1] = from;
+      __syncthreads();
+      if (base > unit) break;
+    }
+    b = found[0];
+    before = found[1];
+  }
+};
+
+__device__ __forceinline__ int share_of(const Params& p, int total, int grid) {
+  return max((total + grid - 1) / grid, p.min_share);
+}
+
+// Position in the list of units: request, item (key / value head, row tile)
+// and key tile.
+template <int MT, int TN>
+struct Walk {
+  int b, item, tile, items, tiles;
+  Request r;
+  __device__ __forceinline__ void open(const Params& p) {
+    r = request(p, b);
+    tiles = Sched<MT, TN>::tiles(r);
+    items = r.len == 0 ? 0 : p.kv_heads * Sched<MT, TN>::row_tiles(p, r);
+  }
+  __device__ __forceinline__ void seek(const Params& p, int b_, int offset) {
+    b = b_;
+    open(p);
+    item = offset / tiles;
+    tile = offset - item * tiles;
+  }
+  __device__ __forceinline__ void next(const Params& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++item < items) return;
+    item = 0;
+    do {
+      ++b;
+      if (b >= p.batch) return;
+      open(p);
+    } while (items == 0);
+  }
+};
+
+// ---------------------------------------------------------------- instructions
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr));
+}
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (BF16)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2^-22 relative, 0 for -inf
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (BF16) {
+    return pack_bf16x2(lo, hi);
+  } else {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// Two 8-bit values (bytes SEL of w) as a pair of fp16.
+template <int KIND, int B0, int B1>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {  // int8: w already biased by 128
+  uint32_t h2;
+  if constexpr (KIND == kE4M3) {
+    const uint32_t two = (B0 == 0 && B1 == 1) ? w : (B0 == 2 && B1 == 3) ? w >> 16 : __byte_perm(w, 0, B0 | B1 << 4);
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(two)));
+  } else {
+    // 0x6400 + u is 1024 + u in fp16; u = value + 128
+    const uint32_t u = __byte_perm(w, 0x64646464u, B0 | 4 << 4 | B1 << 8 | 4 << 12);
+    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
+    h2 = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  return h2;
+}
+
+// Values that are not finite, in drafted tokens that some rows do not see: a
+// product with a probability of 0 would make them NaN in those rows too.  A
+// fragment is split into its finite values (others 0) and two indicators, of
+// values that add +inf (or NaN) and of values that add -inf (or NaN); products
+// with the rows' view of the keys tell which outputs they reach.
+template <bool BF16>
+__device__ __forceinline__ void split_finite(uint32_t b, uint32_t& clean, uint32_t& plus, uint32_t& minus) {
+  constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x3F803F80u : 0x3C003C00u;
+  constexpr uint32_t kFrac = BF16 ? 0x007F007Fu : 0x03FF03FFu;
+  const uint32_t wild = __vcmpeq2(b & kExp, kExp);
+  const uint32_t nan = wild & ~__vcmpeq2(b & kFrac, 0u);
+  const uint32_t neg = __vcmpeq2(b & 0x80008000u, 0x80008000u);
+  clean = b & ~wild;
+  plus = wild & (~neg | nan) & kOne;
+  minus = wild & (neg | nan) & kOne;
+}
+template <bool BF16>
+__device__ __forceinline__ void mma_seen(float (&acc)[4], const uint32_t (&p)[4], const uint32_t (&seen)[4], uint32_t b0,
+                                         uint32_t b1) {
+  uint32_t c0, c1, p0, p1, m0, m1;
+  split_finite<BF16>(b0, c0, p0, m0);
+  split_finite<BF16>(b1, c1, p1, m1);
+  mma<BF16>(acc, p, c0, c1);
+  float up[4] = {0.f, 0.f, 0.f, 0.f}, down[4] = {0.f, 0.f, 0.f, 0.f};
+  mma<BF16>(up, seen, p0, p1);
+  mma<BF16>(down, seen, m0, m1);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    if (up[x] > 0.0f) acc[x] += INFINITY;
+    if (down[x] > 0.0f) acc[x] -= INFINITY;
+  }
+}
+
+// ---------------------------------------------------------------- main kernel
+template <typename T, int KIND_, int D_, int MT_, int TN_, int STAGES_>
+struct Cfg {
+  static constexpr int KIND = KIND_, D = D_, MT = MT_, TN = TN_, STAGES = STAGES_;
+  static constexpr bool kSmall = KIND != kSame;
+  static constexpr bool kBf16 = !kSmall && std::is_same<T, __nv_bfloat16>::value;  // type of the products
+  static constexpr int kRow = D * (kSmall ? 1 : 2);                                // bytes of a key row
+  static constexpr int kChunks = kRow / 16;
+  static constexpr int kTile = TN * kRow;
+  static constexpr int kScales = kSmall ? 2 * TN * 4 : 0;
+  static constexpr int kStage = 2 * kTile + kScales;
+  static constexpr int WM = MT / 16, WK = kWarps / WM;  // warps over rows and over keys
+  static constexpr int KW = TN / WK;                    // keys of a tile per warp
+  static constexpr int kScratch = WK > 1 ? kWarps * 16 * 32 * 4 : 0;  // joining the warps' sums, 32 dimensions a turn
+  static constexpr int kSmem = STAGES * kStage + kScratch + kWarps * 16 * 8 + 64;
+  static_assert(KW % 16 == 0, "a warp takes whole steps of 16 keys");
+};
+
+// Byte offset of 16-byte chunk c of a row: rows shifted against one another so
+// that the 8 rows a matrix load touches lie in different banks.
+template <typename C>
+__device__ __forceinline__ uint32_t place(int row, int c) {
+  if constexpr (C::kChunks >= 8)
+    return row * C::kRow + ((c ^ (row & 7)) << 4);
+  else
+    return row * C::kRow + ((c ^ ((row >> 1) & 3)) << 4);
+}
+
+template <typename C>
+__device__ __forceinline__ void load_tile(const Params& p, const Walk<C::MT, C::TN>& w, uint32_t stage) {
+  constexpr int kRowsPerTurn = kThreads / C::kChunks;
+  const int tid = threadIdx.x;
+  const int c = tid % C::kChunks;
+  const int key0 = w.tile * C::TN;
+  const int h = w.item / Sched<C::MT, C::TN>::row_tiles(p, w.r);
+  const int* table = p.table + w.b * p.table_stride;
+  constexpr int kSize = C::kSmall ? 1 : 2;
+  const uint8_t* kb = static_cast<const uint8_t*>(p.c.key) + (h * p.c.key_stride[2]) * kSize + c * 16;
+  const uint8_t* vb = static_cast<const uint8_t*>(p.c.value) + (h * p.c.value_stride[2]) * kSize + c * 16;
+#pragma unroll
+  for (int i = 0; i < C::TN / kRowsPerTurn; ++i) {
+    const int row = tid / C::kChunks + i * kRowsPerTurn;
+    const int key = key0 + row;
+    const bool valid = key < w.r.len;
+    long long ko = 0, vo = 0;
+    if (valid) {
+      const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
+      const int slot = key - page * p.c.block_size;
+      const long long id = kv::checked_block(table[page], p.c.num_blocks, &g_attn_error);
+      ko = (id * p.c.key_stride[0] + slot * p.c.key_stride[1]) * kSize;
+      vo = (id * p.c.value_stride[0] + slot * p.c.value_stride[1]) * kSize;
+    }
+    cp_async16(stage + place<C>(row, c), kb + ko, valid);
+    cp_async16(stage + C::kTile + place<C>(row, c), vb + vo, valid);
+  }
+  if constexpr (C::kSmall) {
+#pragma unroll
+    for (int i = tid; i < C::TN; i += kThreads) {
+      const int key = key0 + i;
+      const bool valid = key < w.r.len;
+      long long ko = 0, vo = 0;
+      if (valid) {
+        const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
+        const int slot = key - page * p.c.block_size;
+        const long long id = kv::checked_block(table[page], p.c.num_blocks, &g_attn_error);
+        ko = id * p.c.k_scale_stride[0] + slot * p.c.k_scale_stride[1] + h * p.c.k_scale_stride[2];
+        vo = id * p.c.v_scale_stride[0] + slot * p.c.v_scale_stride[1] + h * p.c.v_scale_stride[2];
+      }
+      cp_async4(stage + 2 * C::kTile + 4 * i, p.c.k_scale + ko, valid);
+      cp_async4(stage + 2 * C::kTile + 4 * (C::TN + i), p.c.v_scale + vo, valid);
+    }
+  }
+}
+
+// Whether any of a warp's KW value rows holds an infinity or a NaN.
+template <typename C>
+__device__ __forceinline__ bool any_wild(const uint8_t* values, int row0) {
+  bool wild = false;
+  const uint4* v = reinterpret_cast<const uint4*>(values + row0 * C::kRow);  // rows are whole, their order is no matter
+#pragma unroll 4
+  for (int i = threadIdx.x & 31; i < C::KW * C::kChunks; i += 32) {
+    const uint4 u = v[i];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      if constexpr (C::KIND == kE4M3)
+        wild = wild || ((((w[x] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0);
+      else if constexpr (C::kBf16)
+        wild = wild || __vcmpeq2(w[x] & 0x7F807F80u, 0x7F807F80u) != 0;
+      else
+        wild = wild || __vcmpeq2(w[x] & 0x7C007C00u, 0x7C007C00u) != 0;
+    }
+  }
+  return __any_sync(kFull, wild);
+}
+
+// Whether query i (token t of request r) sees key j < r.len.
+__device__ __forceinline__ bool sees(const Params& p, const Request& r, int t, int i, int key) {
+  const int d = key - (r.len - r.n);
+  if (key >= r.len) return false;
+  if (d < 0) return true;
+  if (p.mask == nullptr) return d <= i;
+  return (p.mask[t * p.mask_stride + (d >> 6)] >> (d & 63)) & 1;
+}
+
+template <typename T, typename C>
+__global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ Params p) {
+  constexpr int D = C::D, MT = C::MT, TN = C::TN, KW = C::KW, KIND = C::KIND;
+  constexpr int kNT = KW / 8;   // 8-key tiles of the scores
+  constexpr int kDT = D / 8;    // 8-dimension tiles of the output
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t stages = smem_u32(smem);
+  float* scratch = reinterpret_cast<float*>(smem + C::STAGES * C::kStage);
+  float2* warp_ml = reinterpret_cast<float2*>(smem + C::STAGES * C::kStage + C::kScratch);
+  __shared__ int red[kWarps + 2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, j4 = lane & 3;
+  const int wm = warp / C::WK, wk = warp % C::WK;
+
+  // the joining kernel may start; it waits for this one to end before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // requests without work (no keys, or refused) still have outputs
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    const Request r = request(p, b);
+    if (r.len != 0 || r.n == 0) continue;
+    const int heads = p.kv_heads * p.group;
+    for (int i = tid; i < r.n * heads; i += kThreads) {
+      const int t = r.first + i / heads, h = i % heads;
+      T* o = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
+      for (int d = 0; d < D; ++d) o[d] = T(0.0f);
+      if (p.lse) p.lse[static_cast<long long>(t) * heads + h] = -INFINITY;
+    }
+  }
+
+  int total, unit, b0, before;
+  int share = 0;
+  Sched<MT, TN>::template locate<kThreads>(
+      p, [&](int tot) { share = share_of(p, tot, gridDim.x); return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll)); }, red,
+      total, unit, b0, before);
+  if (unit >= total) return;
+  const int end = min(unit + share, total);
+
+  Walk<MT, TN> cur, ahead;
+  cur.seek(p, b0, unit - before);
+  ahead = cur;
+  int loaded = unit;
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) {
+    if (loaded < end) {
+      load_tile<C>(p, ahead, stages + s * C::kStage);
+      ahead.next(p);
+      ++loaded;
+    }
+    cp_commit();
+  }
+
+  uint32_t qf[D / 16][4];
+  float qscale[2];
+  float acc[kDT][4];
+  float m[2], l[2], vref = 0.0f;
+  bool fresh = true;
+  int first_tile = 0;
+  int tok[2], qi[2], head[2];
+  bool row_ok[2];
+  int stage = 0;
+
+  for (int u = unit; u < end; ++u) {
+    cp_wait<C::STAGES - 2>();
+    __syncthreads();
+    if (loaded < end) {
+      int s = stage + C::STAGES - 1;
+      if (s >= C::STAGES) s -= C::STAGES;
+      load_tile<C>(p, ahead, stages + s * C::kStage);
+      ahead.next(p);
+      ++loaded;
+    }
+    cp_commit();
+
+    if (fresh) {
+      fresh = false;
+      first_tile = cur.tile;
+      const int rts = Sched<MT, TN>::row_tiles(p, cur.r);
+      const int h = cur.item / rts, rt = cur.item - h * rts;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = rt * MT + wm * 16 + g + 8 * e;
+        row_ok[e] = row < cur.r.n * p.group;
+        qi[e] = row / p.group;
+        head[e] = h * p.group + row - qi[e] * p.group;
+        tok[e] = cur.r.first + qi[e];
+        m[e] = -INFINITY;
+        l[e] = 0.0f;
+        qscale[e] = p.scale_log2;
+        const T* q = static_cast<const T*>(p.q) + tok[e] * p.q_tok + head[e] * p.q_head;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          uint32_t lo = 0, hi = 0;
+          if (row_ok[e]) {
+            if constexpr (C::kSmall) {  // dimensions 4j..4j+3, the order the 8-bit keys come in
+              const uint32_t* src = reinterpret_cast<const uint32_t*>(q + kk * 16 + 4 * j4);
+              lo = src[0], hi = src[1];
+            } else {
+              lo = *reinterpret_cast<const uint32_t*>(q + kk * 16 + 2 * j4);
+              hi = *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8 + 2 * j4);
+            }
+          }
+          qf[kk][e] = lo;
+          qf[kk][2 + e] = hi;
+        }
+        if constexpr (C::kSmall && std::is_same<T, __nv_bfloat16>::value) {
+          // bf16 queries as fp16: scaled by a power of two to a maximum in [1, 2), which is exact for all values
+          // that count beside the row's largest
+          float top = 0.0f;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t v = qf[kk][2 * x + e];
+              top = fmaxf(top, fmaxf(fabsf(__uint_as_float(v << 16)), fabsf(__uint_as_float(v & 0xFFFF0000u))));
+            }
+          top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+          const uint32_t ex = min(max(__float_as_uint(top) & 0x7F800000u, 0x0A000000u), 0x75000000u);
+          const float down = __uint_as_float(0x7F000000u - ex);
+          qscale[e] *= __uint_as_float(ex);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t v = qf[kk][2 * x + e];
+              qf[kk][2 * x + e] =
+                  pack2<false>(__uint_as_float(v << 16) * down, __uint_as_float(v & 0xFFFF0000u) * down);
+            }
+        }
+      }
+      vref = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[i][x] = 0.0f;
+    }
+
+    // ---- scores of this warp's 16 rows and KW keys
+    const uint32_t ks = stages + stage * C::kStage, vs = ks + C::kTile;
+    const float* scale_k = reinterpret_cast<const float*>(smem + stage * C::kStage + 2 * C::kTile);
+    const float* scale_v = scale_k + TN;
+    float s[kNT][4];
+#pragma unroll
+    for (int i = 0; i < kNT; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[i][x] = 0.0f;
+    const int mi = lane >> 3, mr = lane & 7;
+    if constexpr (!C::kSmall) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int n = 0; n < kNT; n += 2) {
+          uint32_t b[4];
+          ldsm4(b, ks + place<C>(wk * KW + n * 8 + (mi >> 1) * 8 + mr, kk * 2 + (mi & 1)));
+          mma<C::kBf16>(s[n], qf[kk], b[0], b[1]);
+          mma<C::kBf16>(s[n + 1], qf[kk], b[2], b[3]);
+        }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk += 2)
+#pragma unroll
+        for (int n = 0; n < kNT; n += 2) {
+          uint32_t b[4];
+          ldsm4(b, ks + place<C>(wk * KW + n * 8 + (mi >> 1) * 8 + mr, kk + (mi & 1)));
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const uint32_t w = KIND == kInt8 ? b[x] ^ 0x80808080u : b[x];
+            mma<false>(s[n + (x >> 1)], qf[kk + (x & 1)], widen<KIND, 0, 1>(w), widen<KIND, 2, 3>(w));
+          }
+        }
+    }
+
+    // ---- scale, mask, running maximum
+    const int key0 = cur.tile * TN + wk * KW;
+    const bool tail = (cur.tile + 1) * TN > cur.r.len - cur.r.n;
+    float top[2] = {-INFINITY, -INFINITY};
+    float vmax = 0.0f;
+    uint32_t seen = 0;  // bit 4 n + x: tail tiles only
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      float2 sk = make_float2(1.0f, 1.0f);
+      if constexpr (C::kSmall) {
+        sk = *reinterpret_cast<const float2*>(scale_k + wk * KW + n * 8 + 2 * j4);
+        const float2 sv = *reinterpret_cast<const float2*>(scale_v + wk * KW + n * 8 + 2 * j4);
+        vmax = fmaxf(vmax, fmaxf(sv.x < 1e30f ? sv.x : 0.0f, sv.y < 1e30f ? sv.y : 0.0f));
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[n][x] *= qscale[x >> 1] * ((x & 1) ? sk.y : sk.x);
+        if (tail) {
+          if (sees(p, cur.r, row_ok[x >> 1] ? tok[x >> 1] : cur.r.first, qi[x >> 1], key0 + n * 8 + 2 * j4 + (x & 1)))
+            seen |= 1u << (4 * n + x);
+          else
+            s[n][x] = -INFINITY;
+        }
+        top[x >> 1] = fmaxf(top[x >> 1], s[n][x]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      top[e] = fmaxf(top[e], __shfl_xor_sync(kFull, top[e], 1));
+      top[e] = fmaxf(top[e], __shfl_xor_sync(kFull, top[e], 2));
+    }
+    float shrink = 1.0f;  // of the sums, when the reference scale of the values moves
+    if constexpr (C::kSmall) {
+      vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, 1));
+      vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, 2));
+      if (vmax > 64.0f * vref) {
+        const float to = __uint_as_float(max(__float_as_uint(vmax) & 0x7F800000u, 0x0A000000u));
+        shrink = vref / to;
+        vref = to;
+      }
+    }
+    if (__any_sync(kFull, top[0] > m[0] || top[1] > m[1]) || shrink != 1.0f) {
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float now = fmaxf(m[e], top[e]);
+        alpha[e] = now == -INFINITY ? 1.0f : exp2_fast(m[e] - now);
+        l[e] *= alpha[e];
+        alpha[e] *= shrink;
+        m[e] = now;
+      }
+#pragma unroll
+      for (int i = 0; i < kDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[i][x] *= alpha[x >> 1];
+    }
+    const float inv_vref = C::kSmall ? __uint_as_float(0x7F000000u - __float_as_uint(vref)) : 1.0f;
+    const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+    uint32_t pf[kNT / 2][4];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      float pr[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        pr[x] = exp2_fast(s[n][x] - sub[x >> 1]);
+        l[x >> 1] += pr[x];
+      }
+      if constexpr (C::kSmall) {
+        const float2 sv = *reinterpret_cast<const float2*>(scale_v + wk * KW + n * 8 + 2 * j4);
+        const float f[2] = {sv.x * inv_vref, sv.y * inv_vref};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) pr[x] = pr[x] == 0.0f && tail ? 0.0f : pr[x] * f[x & 1];
+      }
+      pf[n >> 1][(n & 1) * 2] = pack2<C::kBf16>(pr[0], pr[1]);
+      pf[n >> 1][(n & 1) * 2 + 1] = pack2<C::kBf16>(pr[2], pr[3]);
+    }
+
+    // ---- probabilities times values
+    if (KIND != kInt8 && tail && cur.r.n > 1 && any_wild<C>(smem + stage * C::kStage + C::kTile, wk * KW)) {
+#pragma unroll
+      for (int kk = 0; kk < kNT / 2; ++kk) {
+        const int row = wk * KW + kk * 16 + (mi & 1) * 8 + mr;
+        uint32_t view[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const uint32_t two = seen >> (8 * kk + 4 * (x >> 1) + 2 * (x & 1));
+          view[x] = ((two & 1u) | (two & 2u) << 15) * (C::kBf16 ? 0x3F80u : 0x3C00u);
+        }
+        if constexpr (!C::kSmall) {
+#pragma unroll
+          for (int n = 0; n < kDT; n += 2) {
+            uint32_t b[4];
+            ldsm4t(b, vs + place<C>(row, n + (mi >> 1)));
+            mma_seen<C::kBf16>(acc[n], pf[kk], view, b[0], b[1]);
+            mma_seen<C::kBf16>(acc[n + 1], pf[kk], view, b[2], b[3]);
+          }
+        } else {
+#pragma unroll
+          for (int n = 0; n < D / 16; n += 2) {
+            uint32_t b[4];
+            ldsm4t(b, vs + place<C>(row, n + (mi >> 1)));
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              mma_seen<false>(acc[2 * (n + x)], pf[kk], view, widen<KIND, 0, 2>(b[2 * x]), widen<KIND, 0, 2>(b[2 * x + 1]));
+              mma_seen<false>(acc[2 * (n + x) + 1], pf[kk], view, widen<KIND, 1, 3>(b[2 * x]), widen<KIND, 1, 3>(b[2 * x + 1]));
+            }
+          }
+        }
+      }
+    } else
+#pragma unroll
+    for (int kk = 0; kk < kNT / 2; ++kk) {
+      const int row = wk * KW + kk * 16 + (mi & 1) * 8 + mr;
+      if constexpr (!C::kSmall) {
+#pragma unroll
+        for (int n = 0; n < kDT; n += 2) {
+          uint32_t b[4];
+          ldsm4t(b, vs + place<C>(row, n + (mi >> 1)));
+          mma<C::kBf16>(acc[n], pf[kk], b[0], b[1]);
+          mma<C::kBf16>(acc[n + 1], pf[kk], b[2], b[3]);
+        }
+      } else {
+        // 16 dimensions of a chunk: even ones in one output tile, odd ones in the next
+#pragma unroll
+        for (int n = 0; n < D / 16; n += 2) {
+          uint32_t b[4];
+          ldsm4t(b, vs + place<C>(row, n + (mi >> 1)));
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (KIND == kInt8) b[x] ^= 0x80808080u;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            mma<false>(acc[2 * (n + x)], pf[kk], widen<KIND, 0, 2>(b[2 * x]), widen<KIND, 0, 2>(b[2 * x + 1]));
+            mma<false>(acc[2 * (n + x) + 1], pf[kk], widen<KIND, 1, 3>(b[2 * x]), widen<KIND, 1, 3>(b[2 * x + 1]));
+          }
+        }
+      }
+    }
+
+    // ---- end of the item, or of this block's run: join the warps, write
+    const bool last_tile = cur.tile + 1 == cur.tiles;
+    if (last_tile || u + 1 == end) {
+      fresh = true;
+      const bool whole = first_tile == 0 && last_tile;
+      const int slot = first_tile == 0 ? 1 : 0;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        l[e] += __shfl_xor_sync(kFull, l[e], 1);
+        l[e] += __shfl_xor_sync(kFull, l[e], 2);
+      }
+      float f[2] = {1.0f, 1.0f};
+      if constexpr (C::WK > 1) {
+        if (j4 == 0) {
+          warp_ml[warp * 16 + g] = make_float2(m[0], l[0]);
+          warp_ml[warp * 16 + g + 8] = make_float2(m[1], l[1]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+          for (int w = 0; w < C::WK; ++w) mm = fmaxf(mm, warp_ml[(wm * C::WK + w) * 16 + g + 8 * e].x);
+#pragma unroll
+          for (int w = 0; w < C::WK; ++w) {
+            const float2 o = warp_ml[(wm * C::WK + w) * 16 + g + 8 * e];
+            ll += o.x == -INFINITY ? o.y : exp2_fast(o.x - mm) * o.y;
+          }
+          f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
+          m[e] = mm;
+          l[e] = ll;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if (C::kSmall) f[e] *= vref;
+        if (whole) f[e] = l[e] == 0.0f ? 0.0f : f[e] / l[e];
+      }
+      const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * MT;
+      if (wk == 0 && j4 == 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = wm * 16 + g + 8 * e;
+          if (!whole) {
+            p.part_ml[(part + row) * 2] = m[e];
+            p.part_ml[(part + row) * 2 + 1] = l[e];
+          } else if (row_ok[e] && p.lse) {
+            p.lse[static_cast<long long>(tok[e]) * p.kv_heads * p.group + head[e]] =
+                l[e] == 0.0f ? -INFINITY : (m[e] + log2f(l[e])) * 0.69314718055994531f;
+          }
+        }
+      }
+      if constexpr (C::WK == 1) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = wm * 16 + g + 8 * e;
+          T* o = static_cast<T*>(p.out) + tok[e] * p.o_tok + head[e] * p.o_head;
+          float* po = p.part_o + (part + row) * D;
+#pragma unroll
+          for (int i = 0; i < kDT; i += 2) {
+            const float a = acc[i][2 * e] * f[e], b = acc[i][2 * e + 1] * f[e];
+            const float c = acc[i + 1][2 * e] * f[e], d = acc[i + 1][2 * e + 1] * f[e];
+            // 16-bit caches: dimensions 8i + 2j, +1 of each tile; 8-bit ones: 16 dimensions over two tiles
+            if constexpr (C::kSmall) {
+              if (!whole)
+                *reinterpret_cast<float4*>(po + i * 8 + 4 * j4) = make_float4(a, c, b, d);
+              else if (row_ok[e])
+                *reinterpret_cast<uint2*>(o + i * 8 + 4 * j4) =
+                    make_uint2(pack2<std::is_same<T, __nv_bfloat16>::value>(a, c),
+                               pack2<std::is_same<T, __nv_bfloat16>::value>(b, d));
+            } else {
+              if (!whole) {
+                *reinterpret_cast<float2*>(po + i * 8 + 2 * j4) = make_float2(a, b);
+                *reinterpret_cast<float2*>(po + i * 8 + 8 + 2 * j4) = make_float2(c, d);
+              } else if (row_ok[e]) {
+                *reinterpret_cast<uint32_t*>(o + i * 8 + 2 * j4) = pack2<C::kBf16>(a, b);
+                *reinterpret_cast<uint32_t*>(o + i * 8 + 8 + 2 * j4) = pack2<C::kBf16>(c, d);
+              }
+            }
+          }
+        }
+      } else {
+        const int rts = Sched<MT, TN>::row_tiles(p, cur.r);
+        const int h = cur.item / rts, rt = cur.item - h * rts;
+#pragma unroll
+        for (int d0 = 0; d0 < D; d0 += 32) {
+          __syncthreads();
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float* to = scratch + (warp * 16 + g + 8 * e) * 32 + i * 8;
+              const float(&x)[4] = acc[d0 / 8 + i];
+              const float(&y)[4] = acc[d0 / 8 + i + 1];
+              if constexpr (C::kSmall) {
+                *reinterpret_cast<float4*>(to + 4 * j4) =
+                    make_float4(x[2 * e] * f[e], y[2 * e] * f[e], x[2 * e + 1] * f[e], y[2 * e + 1] * f[e]);
+              } else {
+                *reinterpret_cast<float2*>(to + 2 * j4) = make_float2(x[2 * e] * f[e], x[2 * e + 1] * f[e]);
+                *reinterpret_cast<float2*>(to + 8 + 2 * j4) = make_float2(y[2 * e] * f[e], y[2 * e + 1] * f[e]);
+              }
+            }
+          }
+          __syncthreads();
+          for (int i = tid; i < MT * 8; i += kThreads) {  // 4 dimensions of a row each
+            const int row = i >> 3, d = (i & 7) * 4;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < C::WK; ++w) {
+              const float4 v =
+                  *reinterpret_cast<const float4*>(scratch + (((row >> 4) * C::WK + w) * 16 + (row & 15)) * 32 + d);
+              sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+            }
+            const int r = rt * MT + row;
+            if (!whole) {
+              *reinterpret_cast<float4*>(p.part_o + (part + row) * D + d0 + d) = sum;
+            } else if (r < cur.r.n * p.group) {
+              const int i2 = r / p.group;
+              T* o = static_cast<T*>(p.out) + (cur.r.first + i2) * p.o_tok + (h * p.group + r - i2 * p.group) * p.o_head;
+              constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
+              *reinterpret_cast<uint2*>(o + d0 + d) = make_uint2(pack2<kOutBf16>(sum.x, sum.y), pack2<kOutBf16>(sum.z, sum.w));
+            }
+          }
+        }
+      }
+    }
+    cur.next(p);
+    if (++stage == C::STAGES) stage = 0;
+  }
+}
+
+// ---------------------------------------------------------------- joining kernel
+// Block c joins the one row tile that begins in the main kernel's block c and
+// goes on behind it: its parts lie in slot 1 of c and slot 0 of the next blocks.
+template <typename T, typename C>
+__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
+  constexpr int D = C::D, MT = C::MT, TN = C::TN;
+  __shared__ int red[kWarps + 2];
+  const int grid = gridDim.x, c = blockIdx.x;
+  int total, unit, b, before, share = 0;
+  Sched<MT, TN>::template locate<kThreads>(
+      p, [&](int tot) { share = share_of(p, tot, grid); return static_cast<int>(min((c + 1ll) * share - 1, 2147483647ll)); },
+      red, total, unit, b, before);
+  // every block waits, also those with nothing to join: what follows on the
+  // stream must not overtake the main kernel
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (unit >= total - 1) return;
+  const Request r = request(p, b);
+  const int tiles = Sched<MT, TN>::tiles(r);
+  const int item = (unit - before) / tiles;
+  const int from = before + item * tiles, to = from + tiles - 1;
+  if (from / share != c || to / share == c) return;
+  const int parts = to / share - c + 1;
+  const int rts = Sched<MT, TN>::row_tiles(p, r);
+  const int h = item / rts, rt = item - h * rts;
+  constexpr int kLanes = D / 4;                // threads per row, 4 dimensions each
+  constexpr int kRows = kThreads / kLanes;
+  const int d = (threadIdx.x % kLanes) * 4;
+  for (int row = blockIdx.y * kRows + threadIdx.x / kLanes; row < MT; row += gridDim.y * kRows) {
+    const int rr = rt * MT + row;
+    if (rr >= r.n * p.group) break;
+    float m = -INFINITY, l = 0.0f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k = 0; k < parts; ++k) {
+      const long long at = ((static_cast<long long>(c) + k) * 2 + (k == 0 ? 1 : 0)) * MT + row;
+      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
+      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + d);
+      const float now = fmaxf(m, ml.x);
+      const float a = now == -INFINITY ? 1.0f : exp2_fast(m - now);
+      const float w = now == -INFINITY ? 1.0f : exp2_fast(ml.x - now);
+      l = l * a + ml.y * w;
+      o.x = o.x * a + v.x * w, o.y = o.y * a + v.y * w, o.z = o.z * a + v.z * w, o.w = o.w * a + v.w * w;
+      m = now;
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    const int i = rr / p.group, head = h * p.group + rr - i * p.group;
+    const long long t = r.first + i;
+    T* out = static_cast<T*>(p.out) + t * p.o_tok + head * p.o_head + d;
+    constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
+    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<kOutBf16>(o.x * f, o.y * f), pack2<kOutBf16>(o.z * f, o.w * f));
+    if (p.lse && d == 0)
+      p.lse[t * p.kv_heads * p.group + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+  }
+}
+
+// ---------------------------------------------------------------- host side
+struct Device {
+  int sms;
+};
+
+orError_t device(Device* d) {
+  int dev = 0;
+  MCPU_CUDA_TRY(cudaGetDevice(&dev), "tree_attention");
+  MCPU_CUDA_TRY(cudaDeviceGetAttribute(&d->sms, cudaDevAttrMultiProcessorCount, dev), "tree_attention");
+  return orSuccess;
+}
+
+constexpr int kMaxResident = 4;  // blocks per SM the workspace is sized for
+
+int row_tile(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
+
+unsigned long long workspace_bytes(int sms, long long rows, int D) {
+  const unsigned long long parts = 2ull * kMaxResident * sms * row_tile(rows);
+  return parts * (D + 2) * 4;
+}
+
+template <typename T, typename C>
+orError_t launch(Params& p, void* ws, cudaStream_t st, int sms) {
+  const void* fn = reinterpret_cast<const void*>(&attend_kernel<T, C>);
+  MCPU_CUDA_TRY(ensure_dynamic_smem(fn, C::kSmem), "tree_attention");
+  int resident = 0;
+  MCPU_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, attend_kernel<T, C>, kThreads, C::kSmem),
+                "tree_attention");
+  resident = std::max(1, std::min(resident, kMaxResident));
+  const int grid = resident * sms;
+  const unsigned long long parts = 2ull * grid * C::MT;
+  p.part_o = static_cast<float*>(ws);
+  p.part_ml = p.part_o + parts * C::D;
+  p.min_share = 1;
+  attend_kernel<T, C><<<grid, kThreads, C::kSmem, st>>>(p);
+  MCPU_CUDA_TRY(cudaGetLastError(), "tree_attention launch");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, C::MT / 16);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return from_cuda(cudaLaunchKernelEx(&cfg, join_kernel<T, C>, p), "tree_attention join launch");
+}
+
+template <typename T, int KIND, int D>
+orError_t dispatch_rows(Params& p, long long rows, void* ws, cudaStream_t st, int sms) {
+  constexpr int TN16 = KIND == kSame ? 64 : 128;
+  switch (row_tile(rows)) {
+    case 16: return launch<T, Cfg<T, KIND, D, 16, TN16, 3>>(p, ws, st, sms);
+    case 32: return launch<T, Cfg<T, KIND, D, 32, 64, 3>>(p, ws, st, sms);
+    default: return launch<T, Cfg<T, KIND, D, 64, 64, 3>>(p, ws, st, sms);
+  }
+}
+
+template <typename T, int D>
+orError_t dispatch_kind(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, int sms) {
+  if (p.c.dtype == dtype) return dispatch_rows<T, kSame, D>(p, rows, ws, st, sms);
+  if (p.c.dtype == MCPU_INT8) return dispatch_rows<T, kInt8, D>(p, rows, ws, st, sms);
+  return dispatch_rows<T, kE4M3, D>(p, rows, ws, st, sms);
+}
+
+}  // namespace attn
+
+orError_t attn_read_error(int* flag, bool reset) {
+  int z = 0;
+  MCPU_CUDA_TRY(cudaMemcpyFromSymbol(flag, attn::g_attn_error, sizeof(int)), "mcpu_device_error");
+  if (reset) MCPU_CUDA_TRY(cudaMemcpyToSymbol(attn::g_attn_error, &z, sizeof(int)), "mcpu_device_error");
+  return orSuccess;
+}
+
+}  // namespace mcpu
+
+using namespace mcpu;
+
+extern "C" orError_t mcpu_tree_attention_workspace_bytes(int64_t max_query_len, int num_heads, int num_kv_heads,
+                                                         int head_size, uint64_t* bytes) {
+  const char* op = "tree_attention";
+  MCPU_ARG_CHECK(bytes != nullptr, "%s: bytes is NULL", op);
+  MCPU_ARG_CHECK(num_kv_heads > 0 && num_heads > 0 && num_heads % num_kv_heads == 0,
+                 "%s: num_heads (%d) must be a multiple of num_kv_heads (%d)", op, num_heads, num_kv_heads);
+  MCPU_ARG_CHECK(head_size == 64 || head_size == 128, "%s: head_size %d is not 64 or 128", op, head_size);
+  MCPU_ARG_CHECK(max_query_len > 0 && max_query_len <= MCPU_TREE_MAX_QUERIES, "%s: max_query_len must be in 1..%d", op,
+                 MCPU_TREE_MAX_QUERIES);
+  attn::Device d{};
+  if (attn::device(&d) != orSuccess) d.sms = 148;
+  *bytes = attn::workspace_bytes(d.sms, max_query_len * (num_heads / num_kv_heads), head_size);
+  return orSuccess;
+}
+
+extern "C" orError_t mcpu_tree_attention(
+    const void* query, int64_t query_token_stride, int64_t query_head_stride, int64_t num_tokens, int num_heads,
+    void* out, int64_t out_token_stride, int64_t out_head_stride, float* lse, int dtype, const mcpuKvCache* cache,
+    const int32_t* block_table, int64_t table_stride, int64_t table_width, int64_t batch, const int32_t* seq_lens,
+    const int32_t* cu_query_lens, int64_t max_query_len, const int64_t* tree_mask, int64_t mask_stride,
+    int64_t mask_words, float scale, void* workspace, uint64_t workspace_bytes, orStream_t stream) {
+  const char* op = "tree_attention";
+  orError_t e = kv::check_cache(cache, dtype, op);
+  if (e != orSuccess) return e;
+  const int D = cache->head_size, kv = cache->kv_heads;
+  uint64_t need = 0;
+  MCPU_ARG_CHECK(num_tokens >= 0 && num_tokens < (1LL << 31) && batch >= 0 && batch < (1LL << 30) && table_width >= 0 &&
+                     table_width < (1LL << 31) && table_stride >= table_width,
+                 "%s: bad sizes", op);
+  if (num_tokens == 0 || batch == 0) return orSuccess;
+  e = mcpu_tree_attention_workspace_bytes(max_query_len, num_heads, kv, D, &need);
+  if (e != orSuccess) return e;
+  MCPU_ARG_CHECK(cache->num_blocks > 0, "%s: the cache has no blocks", op);
+  MCPU_ARG_CHECK(query && out && block_table && seq_lens && cu_query_lens && workspace, "%s: NULL pointer", op);
+  MCPU_ARG_CHECK(workspace_bytes >= need, "%s: workspace holds %llu bytes, %llu needed", op,
+                 static_cast<unsigned long long>(workspace_bytes), static_cast<unsigned long long>(need));
+  MCPU_ARG_CHECK(((reinterpret_cast<uintptr_t>(query) | reinterpret_cast<uintptr_t>(out) |
+                   reinterpret_cast<uintptr_t>(workspace)) & 15) == 0 &&
+                     (query_token_stride | query_head_stride | out_token_stride | out_head_stride) % 8 == 0,
+                 "%s: query, out and workspace must be 16-byte aligned, with strides of whole 16 bytes", op);
+  MCPU_ARG_CHECK(tree_mask == nullptr || (mask_words > 0 && mask_words <= (1 << 20) && mask_stride >= mask_words &&
+                                          64 * mask_words >= max_query_len),
+                 "%s: tree_mask has %lld words of 64 tokens, max_query_len is %lld", op,
+                 static_cast<long long>(mask_words), static_cast<long long>(max_query_len));
+  // unit numbers are 32-bit: the longest requests the table can hold, with tiles of 64 keys and 16 rows
+  const double room = static_cast<double>(table_width) * cache->block_size;
+  const double rows = static_cast<double>(max_query_len) * (num_heads / kv);
+  MCPU_ARG_CHECK(room < 2147483000.0 && batch * kv * (rows / 16 + 1) * (room / 64 + 1) < 2147483000.0,
+                 "%s: batch, heads and block_table are too large for one call", op);
+  attn::Device d{};
+  e = attn::device(&d);
+  if (e != orSuccess) return e;
+  attn::Params p{};
+  p.q = query, p.q_tok = query_token_stride, p.q_head = query_head_stride;
+  p.out = out, p.o_tok = out_token_stride, p.o_head = out_head_stride;
+  p.lse = lse;
+  p.c = *cache;
+  p.table = block_table, p.table_stride = table_stride, p.table_width = static_cast<int>(table_width);
+  p.block_log2 = -1;
+  for (int i = 0; i < 31; ++i)
+    if (cache->block_size == (1 << i)) p.block_log2 = i;
+  p.seq_lens = seq_lens, p.cu = cu_query_lens;
+  p.mask = reinterpret_cast<const long long*>(tree_mask), p.mask_stride = mask_stride;
+  p.mask_words = static_cast<int>(std::min<int64_t>(mask_words, 1 << 20));
+  p.batch = static_cast<int>(batch), p.tokens = static_cast<int>(num_tokens);
+  p.kv_heads = kv, p.group = num_heads / kv;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  const long long rows_max = max_query_len * p.group;
+  cudaStream_t st = as_cuda(stream);
+  if (dtype == MCPU_FLOAT16)
+    return D == 64 ? attn::dispatch_kind<__half, 64>(p, dtype, rows_max, workspace, st, d.sms)
+                   : attn::dispatch_kind<__half, 128>(p, dtype, rows_max, workspace, st, d.sms);
+  return D == 64 ? attn::dispatch_kind<__nv_bfloat16, 64>(p, dtype, rows_max, workspace, st, d.sms)
+                 : attn::dispatch_kind<__nv_bfloat16, 128>(p, dtype, rows_max, workspace, st, d.sms);
+}

@@ -313,3 +313,13 @@ def sigmoid(x: torch.Tensor) -> torch.Tensor:
 def silu(x: torch.Tensor) -> torch.Tensor:
     """x / (1 + exp(-x)) with exp correctly rounded (unary_out.cpp:50-51)."""
     return _elementwise("silu", x)
+
+
+from .attention import (  # noqa: E402,F401
+    gather_cache,
+    reshape_and_cache,
+    rotary_cos_sin_cache,
+    rotary_embedding,
+    rotary_reshape_and_cache,
+    tree_attention,
+)
