@@ -26,174 +26,20 @@
 // 8-bit caches are multiplied as fp16, which holds e4m3 and int8 values
 // exactly: the scales of the keys go onto the scores, those of the values onto
 // the probabilities.
-#include <math.h>
-
 #include <algorithm>
 #include <type_traits>
 
-#include "kv_cache.cuh"
+#include "tree_attention.cuh"
 
 namespace mcpu {
 namespace attn {
 
-__device__ int g_attn_error = 0;
-
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr unsigned kFull = 0xFFFFFFFFu;
-
-enum Kind { kSame = 0, kE4M3 = 1, kInt8 = 2 };
-
-struct Params {
-  const void* q;
-  long long q_tok, q_head;
-  void* out;
-  long long o_tok, o_head;
-  float* lse;  // [tokens, heads] or NULL
-  mcpuKvCache c;
-  const int* table;
-  long long table_stride;
-  int table_width, block_log2;  // block_log2 < 0: not a power of two
-  const int* seq_lens;
-  const int* cu;
-  const long long* mask;  // [tokens, words] or NULL
-  long long mask_stride;
-  int mask_words;
-  int batch, tokens, kv_heads, group;
-  float scale_log2;
-  int min_share;
-  float* part_o;   // [grid][2][MT][D]
-  float* part_ml;  // [grid][2][MT][2]
-};
-
-// ---------------------------------------------------------------- schedule
-struct Request {
-  int first, n, len;  // first token, new tokens, length; len = 0: nothing to do
-};
-
-__device__ __forceinline__ Request request(const Params& p, int b) {
-  Request r;
-  r.first = p.cu[b];
-  const int end = p.cu[b + 1];
-  r.n = end - r.first;
-  r.len = p.seq_lens[b];
-  const bool fits = r.first >= 0 && r.n >= 0 && end <= p.tokens;
-  const long long room = static_cast<long long>(p.table_width) * p.c.block_size;
-  const bool words = p.mask == nullptr || r.n <= 64 * p.mask_words;
-  if (!fits || r.len < r.n || r.len > room || !words) {
-    atomicOr(&g_attn_error, 1);
-    if (!fits) r.first = 0, r.n = 0;
-    r.len = 0;
-  }
-  if (r.n == 0) r.len = 0;
-  return r;
-}
-
-template <int MT, int TN>
-struct Sched {
-  static __device__ __forceinline__ int tiles(const Request& r) { return (r.len + TN - 1) / TN; }
-  static __device__ __forceinline__ int row_tiles(const Params& p, const Request& r) {
-    return (r.n * p.group + MT - 1) / MT;
-  }
-  static __device__ __forceinline__ int units(const Params& p, const Request& r) {
-    return r.len == 0 ? 0 : p.kv_heads * row_tiles(p, r) * tiles(r);
-  }
-
-  // Block-wide: total units, then the request that holds `unit` (a function of
-  // the total) and the units before it.
-  template <int NT, typename F>
-  static __device__ __forceinline__ void locate(const Params& p, F&& unit_of, int* red, int& total, int& unit, int& b,
-                                                int& before) {
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    int mine = 0;
-    for (int i = tid; i < p.batch; i += NT) mine += units(p, request(p, i));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kFull, mine, o);
-    if (lane == 0) red[warp] = mine;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (int w = 0; w < NT / 32; ++w) total += red[w];
-    unit = unit_of(total);
-    int* found = red + NT / 32;
-    if (tid == 0) found[0] = p.batch, found[1] = total;
-    __syncthreads();
-    int base = 0;
-    for (int i0 = 0; i0 < p.batch; i0 += NT) {
-      const int i = i0 + tid;
-      const int u = i < p.batch ? units(p, request(p, i)) : 0;
-      int incl = u;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(kFull, incl, o);
-        if (lane >= o) incl += v;
-      }
-      if (lane == 31) red[warp] = incl;
-      __syncthreads();
-      int off = base;
-#pragma unroll
-      for (int w = 0; w < NT / 32; ++w) {
-        off += w < warp ? red[w] : 0;
-        base += red[w];
-      }
-      const int from = off + incl - u;
-      if (unit >= from && unit < from + u) found[0] = i, found[1] = from;
-      __syncthreads();
-      if (base > unit) break;
-    }
-    b = found[0];
-    before = found[1];
-  }
-};
-
-__device__ __forceinline__ int share_of(const Params& p, int total, int grid) {
-  return max((total + grid - 1) / grid, p.min_share);
-}
-
-// Position in the list of units: request, item (key / value head, row tile)
-// and key tile.
-template <int MT, int TN>
-struct Walk {
-  int b, item, tile, items, tiles;
-  Request r;
-  __device__ __forceinline__ void open(const Params& p) {
-    r = request(p, b);
-    tiles = Sched<MT, TN>::tiles(r);
-    items = r.len == 0 ? 0 : p.kv_heads * Sched<MT, TN>::row_tiles(p, r);
-  }
-  __device__ __forceinline__ void seek(const Params& p, int b_, int offset) {
-    b = b_;
-    open(p);
-    item = offset / tiles;
-    tile = offset - item * tiles;
-  }
-  __device__ __forceinline__ void next(const Params& p) {
-    if (++tile < tiles) return;
-    tile = 0;
-    if (++item < items) return;
-    item = 0;
-    do {
-      ++b;
-      if (b >= p.batch) return;
-      open(p);
-    } while (items == 0);
-  }
-};
 
 // ---------------------------------------------------------------- instructions
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(valid ? 4 : 0) : "memory");
-}
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -218,52 +64,11 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2^-22 relative, 0 for -inf
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-template <bool BF16>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-  if constexpr (BF16) {
-    return pack_bf16x2(lo, hi);
-  } else {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
-// Two 8-bit values (bytes SEL of w) as a pair of fp16.
-template <int KIND, int B0, int B1>
-__device__ __forceinline__ uint32_t widen(uint32_t w) {  // int8: w already biased by 128
-  uint32_t h2;
-  if constexpr (KIND == kE4M3) {
-    const uint32_t two = (B0 == 0 && B1 == 1) ? w : (B0 == 2 && B1 == 3) ? w >> 16 : __byte_perm(w, 0, B0 | B1 << 4);
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(two)));
-  } else {
-    // 0x6400 + u is 1024 + u in fp16; u = value + 128
-    const uint32_t u = __byte_perm(w, 0x64646464u, B0 | 4 << 4 | B1 << 8 | 4 << 12);
-    const __half2 v = __hsub2(*reinterpret_cast<const __half2*>(&u), __half2half2(__ushort_as_half(0x6480)));
-    h2 = *reinterpret_cast<const uint32_t*>(&v);
-  }
-  return h2;
-}
-
 // Values that are not finite, in drafted tokens that some rows do not see: a
 // product with a probability of 0 would make them NaN in those rows too.  A
 // fragment is split into its finite values (others 0) and two indicators, of
 // values that add +inf (or NaN) and of values that add -inf (or NaN); products
 // with the rows' view of the keys tell which outputs they reach.
-template <bool BF16>
-__device__ __forceinline__ void split_finite(uint32_t b, uint32_t& clean, uint32_t& plus, uint32_t& minus) {
-  constexpr uint32_t kExp = BF16 ? 0x7F807F80u : 0x7C007C00u, kOne = BF16 ? 0x3F803F80u : 0x3C003C00u;
-  constexpr uint32_t kFrac = BF16 ? 0x007F007Fu : 0x03FF03FFu;
-  const uint32_t wild = __vcmpeq2(b & kExp, kExp);
-  const uint32_t nan = wild & ~__vcmpeq2(b & kFrac, 0u);
-  const uint32_t neg = __vcmpeq2(b & 0x80008000u, 0x80008000u);
-  clean = b & ~wild;
-  plus = wild & (~neg | nan) & kOne;
-  minus = wild & (neg | nan) & kOne;
-}
 template <bool BF16>
 __device__ __forceinline__ void mma_seen(float (&acc)[4], const uint32_t (&p)[4], const uint32_t (&seen)[4], uint32_t b0,
                                          uint32_t b1) {
@@ -310,12 +115,12 @@ __device__ __forceinline__ uint32_t place(int row, int c) {
 }
 
 template <typename C>
-__device__ __forceinline__ void load_tile(const Params& p, const Walk<C::MT, C::TN>& w, uint32_t stage) {
+__device__ __forceinline__ void load_tile(const Params& p, const Walk& w, uint32_t stage) {
   constexpr int kRowsPerTurn = kThreads / C::kChunks;
   const int tid = threadIdx.x;
   const int c = tid % C::kChunks;
   const int key0 = w.tile * C::TN;
-  const int h = w.item / Sched<C::MT, C::TN>::row_tiles(p, w.r);
+  const int h = w.item / row_tiles(p, w.r);
   const int* table = p.table + w.b * p.table_stride;
   constexpr int kSize = C::kSmall ? 1 : 2;
   const uint8_t* kb = static_cast<const uint8_t*>(p.c.key) + (h * p.c.key_stride[2]) * kSize + c * 16;
@@ -403,28 +208,17 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
   // the joining kernel may start; it waits for this one to end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // requests without work (no keys, or refused) still have outputs
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    const Request r = request(p, b);
-    if (r.len != 0 || r.n == 0) continue;
-    const int heads = p.kv_heads * p.group;
-    for (int i = tid; i < r.n * heads; i += kThreads) {
-      const int t = r.first + i / heads, h = i % heads;
-      T* o = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
-      for (int d = 0; d < D; ++d) o[d] = T(0.0f);
-      if (p.lse) p.lse[static_cast<long long>(t) * heads + h] = -INFINITY;
-    }
-  }
+  clear_idle_requests<T, kThreads>(p, D);
 
   int total, unit, b0, before;
   int share = 0;
-  Sched<MT, TN>::template locate<kThreads>(
+  locate<kThreads>(
       p, [&](int tot) { share = share_of(p, tot, gridDim.x); return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll)); }, red,
       total, unit, b0, before);
   if (unit >= total) return;
   const int end = min(unit + share, total);
 
-  Walk<MT, TN> cur, ahead;
+  Walk cur, ahead;
   cur.seek(p, b0, unit - before);
   ahead = cur;
   int loaded = unit;
@@ -463,7 +257,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
     if (fresh) {
       fresh = false;
       first_tile = cur.tile;
-      const int rts = Sched<MT, TN>::row_tiles(p, cur.r);
+      const int rts = row_tiles(p, cur.r);
       const int h = cur.item / rts, rt = cur.item - h * rts;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -780,7 +574,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
           }
         }
       } else {
-        const int rts = Sched<MT, TN>::row_tiles(p, cur.r);
+        const int rts = row_tiles(p, cur.r);
         const int h = cur.item / rts, rt = cur.item - h * rts;
 #pragma unroll
         for (int d0 = 0; d0 < D; d0 += 32) {
@@ -832,42 +626,45 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 // ---------------------------------------------------------------- joining kernel
 // Block c joins the one row tile that begins in the main kernel's block c and
 // goes on behind it: its parts lie in slot 1 of c and slot 0 of the next blocks.
-template <typename T, typename C>
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
-  constexpr int D = C::D, MT = C::MT, TN = C::TN;
   __shared__ int red[kWarps + 2];
-  const int grid = gridDim.x, c = blockIdx.x;
+  const int grid = gridDim.x, c = blockIdx.x, rows = 1 << p.rows_log2;
   int total, unit, b, before, share = 0;
-  Sched<MT, TN>::template locate<kThreads>(
-      p, [&](int tot) { share = share_of(p, tot, grid); return static_cast<int>(min((c + 1ll) * share - 1, 2147483647ll)); },
+  locate<kThreads>(
+      p,
+      [&](int tot) {
+        share = share_of(p, tot, grid);
+        return static_cast<int>(min((c + 1ll) * share - 1, 2147483647ll));
+      },
       red, total, unit, b, before);
   // every block waits, also those with nothing to join: what follows on the
   // stream must not overtake the main kernel
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (unit >= total - 1) return;
   const Request r = request(p, b);
-  const int tiles = Sched<MT, TN>::tiles(r);
+  const int tiles = key_tiles(p, r);
   const int item = (unit - before) / tiles;
   const int from = before + item * tiles, to = from + tiles - 1;
   if (from / share != c || to / share == c) return;
   const int parts = to / share - c + 1;
-  const int rts = Sched<MT, TN>::row_tiles(p, r);
+  const int rts = row_tiles(p, r);
   const int h = item / rts, rt = item - h * rts;
-  constexpr int kLanes = D / 4;                // threads per row, 4 dimensions each
+  constexpr int kLanes = D / 4;  // threads per row, 4 dimensions each
   constexpr int kRows = kThreads / kLanes;
   const int d = (threadIdx.x % kLanes) * 4;
-  for (int row = blockIdx.y * kRows + threadIdx.x / kLanes; row < MT; row += gridDim.y * kRows) {
-    const int rr = rt * MT + row;
+  for (int row = blockIdx.y * kRows + threadIdx.x / kLanes; row < rows; row += gridDim.y * kRows) {
+    const int rr = rt * rows + row;
     if (rr >= r.n * p.group) break;
     float m = -INFINITY, l = 0.0f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 0; k < parts; ++k) {
-      const long long at = ((static_cast<long long>(c) + k) * 2 + (k == 0 ? 1 : 0)) * MT + row;
+      const long long at = ((static_cast<long long>(c) + k) * 2 + (k == 0 ? 1 : 0)) * rows + row;
       const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
       const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + d);
       const float now = fmaxf(m, ml.x);
-      const float a = now == -INFINITY ? 1.0f : exp2_fast(m - now);
-      const float w = now == -INFINITY ? 1.0f : exp2_fast(ml.x - now);
+      const float a = m == -INFINITY ? 1.0f : exp2_fast(m - now);  // nothing yet: sums of 0 (or NaN)
+      const float w = ml.x == -INFINITY ? 1.0f : exp2_fast(ml.x - now);
       l = l * a + ml.y * w;
       o.x = o.x * a + v.x * w, o.y = o.y * a + v.y * w, o.z = o.z * a + v.z * w, o.w = o.w * a + v.w * w;
       m = now;
@@ -896,31 +693,45 @@ orError_t device(Device* d) {
 }
 
 constexpr int kMaxResident = 4;  // blocks per SM the workspace is sized for
+constexpr int kFewRows = 16;     // rows per key / value head that take the kernel above
 
-int row_tile(long long rows) { return rows <= 16 ? 16 : rows <= 32 ? 32 : 64; }
-
-unsigned long long workspace_bytes(int sms, long long rows, int D) {
-  const unsigned long long parts = 2ull * kMaxResident * sms * row_tile(rows);
-  return parts * (D + 2) * 4;
+// Rows of partial sums a call may leave: two parts for every block.
+unsigned long long part_rows(int sms, long long rows) {
+  if (rows <= kFewRows) return 2ull * kMaxResident * sms * 16;
+  return 2ull * sms * (rows <= 128 ? 128 : 256);
 }
 
 template <typename T, typename C>
-orError_t launch(Params& p, void* ws, cudaStream_t st, int sms) {
+orError_t launch(Params& p, cudaStream_t st, int sms, int* grid) {
   const void* fn = reinterpret_cast<const void*>(&attend_kernel<T, C>);
   MCPU_CUDA_TRY(ensure_dynamic_smem(fn, C::kSmem), "tree_attention");
   int resident = 0;
   MCPU_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, attend_kernel<T, C>, kThreads, C::kSmem),
                 "tree_attention");
-  resident = std::max(1, std::min(resident, kMaxResident));
-  const int grid = resident * sms;
-  const unsigned long long parts = 2ull * grid * C::MT;
-  p.part_o = static_cast<float*>(ws);
-  p.part_ml = p.part_o + parts * C::D;
+  *grid = std::max(1, std::min(resident, kMaxResident)) * sms;
+  p.rows_log2 = C::MT == 16 ? 4 : C::MT == 32 ? 5 : 6;
+  p.keys_log2 = C::TN == 64 ? 6 : 7;
   p.min_share = 1;
-  attend_kernel<T, C><<<grid, kThreads, C::kSmem, st>>>(p);
-  MCPU_CUDA_TRY(cudaGetLastError(), "tree_attention launch");
+  attend_kernel<T, C><<<*grid, kThreads, C::kSmem, st>>>(p);
+  return from_cuda(cudaGetLastError(), "tree_attention launch");
+}
+
+template <typename T, int D>
+orError_t launch_few(Params& p, int dtype, cudaStream_t st, int sms, int* grid) {
+  if (p.c.dtype == dtype) return launch<T, Cfg<T, kSame, D, 16, 64, 3>>(p, st, sms, grid);
+  if (p.c.dtype == MCPU_INT8) return launch<T, Cfg<T, kInt8, D, 16, 128, 3>>(p, st, sms, grid);
+  return launch<T, Cfg<T, kE4M3, D, 16, 128, 3>>(p, st, sms, grid);
+}
+
+template <typename T, int D>
+orError_t run(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, int sms) {
+  p.part_o = static_cast<float*>(ws);
+  p.part_ml = p.part_o + part_rows(sms, rows) * D;
+  int grid = 0;
+  const orError_t e = rows <= kFewRows ? launch_few<T, D>(p, dtype, st, sms, &grid) : launch_tc(p, D, rows, st, sms, &grid);
+  if (e != orSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, C::MT / 16);
+  cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / 32));
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -928,32 +739,19 @@ orError_t launch(Params& p, void* ws, cudaStream_t st, int sms) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return from_cuda(cudaLaunchKernelEx(&cfg, join_kernel<T, C>, p), "tree_attention join launch");
-}
-
-template <typename T, int KIND, int D>
-orError_t dispatch_rows(Params& p, long long rows, void* ws, cudaStream_t st, int sms) {
-  constexpr int TN16 = KIND == kSame ? 64 : 128;
-  switch (row_tile(rows)) {
-    case 16: return launch<T, Cfg<T, KIND, D, 16, TN16, 3>>(p, ws, st, sms);
-    case 32: return launch<T, Cfg<T, KIND, D, 32, 64, 3>>(p, ws, st, sms);
-    default: return launch<T, Cfg<T, KIND, D, 64, 64, 3>>(p, ws, st, sms);
-  }
-}
-
-template <typename T, int D>
-orError_t dispatch_kind(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, int sms) {
-  if (p.c.dtype == dtype) return dispatch_rows<T, kSame, D>(p, rows, ws, st, sms);
-  if (p.c.dtype == MCPU_INT8) return dispatch_rows<T, kInt8, D>(p, rows, ws, st, sms);
-  return dispatch_rows<T, kE4M3, D>(p, rows, ws, st, sms);
+  return from_cuda(cudaLaunchKernelEx(&cfg, join_kernel<T, D>, p), "tree_attention join launch");
 }
 
 }  // namespace attn
 
 orError_t attn_read_error(int* flag, bool reset) {
   int z = 0;
+  int tc = 0;
+  const orError_t e = attn::tc_read_error(&tc, reset);
+  if (e != orSuccess) return e;
   MCPU_CUDA_TRY(cudaMemcpyFromSymbol(flag, attn::g_attn_error, sizeof(int)), "mcpu_device_error");
   if (reset) MCPU_CUDA_TRY(cudaMemcpyToSymbol(attn::g_attn_error, &z, sizeof(int)), "mcpu_device_error");
+  *flag |= tc;
   return orSuccess;
 }
 
@@ -972,7 +770,7 @@ extern "C" orError_t mcpu_tree_attention_workspace_bytes(int64_t max_query_len, 
                  MCPU_TREE_MAX_QUERIES);
   attn::Device d{};
   if (attn::device(&d) != orSuccess) d.sms = 148;
-  *bytes = attn::workspace_bytes(d.sms, max_query_len * (num_heads / num_kv_heads), head_size);
+  *bytes = attn::part_rows(d.sms, max_query_len * (num_heads / num_kv_heads)) * (head_size + 2) * 4;
   return orSuccess;
 }
 
@@ -1030,9 +828,10 @@ extern "C" orError_t mcpu_tree_attention(
   p.scale_log2 = scale * 1.4426950408889634f;
   const long long rows_max = max_query_len * p.group;
   cudaStream_t st = as_cuda(stream);
+  p.bf16 = dtype == MCPU_BFLOAT16;
   if (dtype == MCPU_FLOAT16)
-    return D == 64 ? attn::dispatch_kind<__half, 64>(p, dtype, rows_max, workspace, st, d.sms)
-                   : attn::dispatch_kind<__half, 128>(p, dtype, rows_max, workspace, st, d.sms);
-  return D == 64 ? attn::dispatch_kind<__nv_bfloat16, 64>(p, dtype, rows_max, workspace, st, d.sms)
-                 : attn::dispatch_kind<__nv_bfloat16, 128>(p, dtype, rows_max, workspace, st, d.sms);
+    return D == 64 ? attn::run<__half, 64>(p, dtype, rows_max, workspace, st, d.sms)
+                   : attn::run<__half, 128>(p, dtype, rows_max, workspace, st, d.sms);
+  return D == 64 ? attn::run<__nv_bfloat16, 64>(p, dtype, rows_max, workspace, st, d.sms)
+                 : attn::run<__nv_bfloat16, 128>(p, dtype, rows_max, workspace, st, d.sms);
 }
