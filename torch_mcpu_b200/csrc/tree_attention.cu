@@ -36,6 +36,7 @@ namespace attn {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kJoinThreads = 128;  // 16 rows a block
 
 // ---------------------------------------------------------------- instructions
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -208,7 +209,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
   // the joining kernel may start; it waits for this one to end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  clear_idle_requests<T, kThreads>(p, D);
+  clear_idle_requests<kThreads>(p, D);
 
   int total, unit, b0, before;
   int share = 0;
@@ -627,11 +628,11 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 // Block c joins the one row tile that begins in the main kernel's block c and
 // goes on behind it: its parts lie in slot 1 of c and slot 0 of the next blocks.
 template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ Params p) {
-  __shared__ int red[kWarps + 2];
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p) {
+  __shared__ int red[kJoinThreads / 32 + 2];
   const int grid = gridDim.x, c = blockIdx.x, rows = 1 << p.rows_log2;
   int total, unit, b, before, share = 0;
-  locate<kThreads>(
+  locate<kJoinThreads>(
       p,
       [&](int tot) {
         share = share_of(p, tot, grid);
@@ -650,33 +651,49 @@ __global__ void __launch_bounds__(kThreads) join_kernel(const __grid_constant__ 
   const int parts = to / share - c + 1;
   const int rts = row_tiles(p, r);
   const int h = item / rts, rt = item - h * rts;
-  constexpr int kLanes = D / 4;  // threads per row, 4 dimensions each
-  constexpr int kRows = kThreads / kLanes;
+  // D / 4 lanes hold a row, 4 dimensions each; a warp takes kAtOnce rows together so that their parts' loads overlap
+  constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes, kAtOnce = 4 / kPerWarp;
   const int d = (threadIdx.x % kLanes) * 4;
-  for (int row = blockIdx.y * kRows + threadIdx.x / kLanes; row < rows; row += gridDim.y * kRows) {
-    const int rr = rt * rows + row;
-    if (rr >= r.n * p.group) break;
-    float m = -INFINITY, l = 0.0f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k = 0; k < parts; ++k) {
-      const long long at = ((static_cast<long long>(c) + k) * 2 + (k == 0 ? 1 : 0)) * rows + row;
-      const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + at * 2);
-      const float4 v = *reinterpret_cast<const float4*>(p.part_o + at * D + d);
-      const float now = fmaxf(m, ml.x);
-      const float a = m == -INFINITY ? 1.0f : exp2_fast(m - now);  // nothing yet: sums of 0 (or NaN)
-      const float w = ml.x == -INFINITY ? 1.0f : exp2_fast(ml.x - now);
-      l = l * a + ml.y * w;
-      o.x = o.x * a + v.x * w, o.y = o.y * a + v.y * w, o.z = o.z * a + v.z * w, o.w = o.w * a + v.w * w;
-      m = now;
+  const int row0 = (blockIdx.y * (kJoinThreads / 32) + threadIdx.x / 32) * 4 + (threadIdx.x % 32) / kLanes;
+  float m[kAtOnce], l[kAtOnce];
+  float4 o[kAtOnce];
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) m[i] = -INFINITY, l[i] = 0.0f, o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (rt * rows + row0 - (threadIdx.x % 32) / kLanes >= r.n * p.group) return;
+  for (int k = 0; k < parts; ++k) {
+    float2 ml[kAtOnce];
+    float4 v[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const long long at = ((static_cast<long long>(c) + k) * 2 + (k == 0 ? 1 : 0)) * rows + row0 + i * kPerWarp;
+      const bool in = rt * rows + row0 + i * kPerWarp < r.n * p.group;
+      ml[i] = in ? *reinterpret_cast<const float2*>(p.part_ml + at * 2) : make_float2(-INFINITY, 0.0f);
+      v[i] = in ? *reinterpret_cast<const float4*>(p.part_o + at * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    const float f = l == 0.0f ? 0.0f : 1.0f / l;
-    const int i = rr / p.group, head = h * p.group + rr - i * p.group;
-    const long long t = r.first + i;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float now = fmaxf(m[i], ml[i].x);
+      const float a = m[i] == -INFINITY ? 1.0f : exp2_fast(m[i] - now);  // nothing yet: sums of 0 (or NaN)
+      const float w = ml[i].x == -INFINITY ? 1.0f : exp2_fast(ml[i].x - now);
+      l[i] = l[i] * a + ml[i].y * w;
+      o[i].x = o[i].x * a + v[i].x * w, o[i].y = o[i].y * a + v[i].y * w;
+      o[i].z = o[i].z * a + v[i].z * w, o[i].w = o[i].w * a + v[i].w * w;
+      m[i] = now;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kAtOnce; ++i) {
+    const int rr = rt * rows + row0 + i * kPerWarp;
+    if (rr >= r.n * p.group) break;
+    const float f = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+    const int q = rr / p.group, head = h * p.group + rr - q * p.group;
+    const long long t = r.first + q;
     T* out = static_cast<T*>(p.out) + t * p.o_tok + head * p.o_head + d;
     constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
-    *reinterpret_cast<uint2*>(out) = make_uint2(pack2<kOutBf16>(o.x * f, o.y * f), pack2<kOutBf16>(o.z * f, o.w * f));
+    *reinterpret_cast<uint2*>(out) =
+        make_uint2(pack2<kOutBf16>(o[i].x * f, o[i].y * f), pack2<kOutBf16>(o[i].z * f, o[i].w * f));
     if (p.lse && d == 0)
-      p.lse[t * p.kv_heads * p.group + head] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.69314718055994531f;
+      p.lse[t * p.kv_heads * p.group + head] = l[i] == 0.0f ? -INFINITY : (m[i] + log2f(l[i])) * 0.69314718055994531f;
   }
 }
 
@@ -731,8 +748,8 @@ orError_t run(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, i
   const orError_t e = rows <= kFewRows ? launch_few<T, D>(p, dtype, st, sms, &grid) : launch_tc(p, D, rows, st, sms, &grid);
   if (e != orSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / 32));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / (kJoinThreads / 8)));
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -803,6 +820,12 @@ extern "C" orError_t mcpu_tree_attention(
                                           64 * mask_words >= max_query_len),
                  "%s: tree_mask has %lld words of 64 tokens, max_query_len is %lld", op,
                  static_cast<long long>(mask_words), static_cast<long long>(max_query_len));
+  for (int i = 0; i < 2; ++i) {  // places in 16-byte units are 32-bit
+    const int64_t* st = i == 0 ? cache->key_stride : cache->value_stride;
+    const double span = (static_cast<double>(cache->num_blocks - 1) * st[0] + static_cast<double>(cache->block_size - 1) * st[1]) *
+                        (cache->dtype == dtype ? 2 : 1);
+    MCPU_ARG_CHECK(span < 64.0 * 1073741824.0, "%s: a cache tensor spans at most 64 GB", op);
+  }
   // unit numbers are 32-bit: the longest requests the table can hold, with tiles of 64 keys and 16 rows
   const double room = static_cast<double>(table_width) * cache->block_size;
   const double rows = static_cast<double>(max_query_len) * (num_heads / kv);

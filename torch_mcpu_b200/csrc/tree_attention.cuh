@@ -78,8 +78,9 @@ template <int NT, typename F>
 __device__ __forceinline__ void locate(const Params& p, F&& unit_of, int* red, int& total, int& unit, int& b,
                                        int& before) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int mine = 0;
-  for (int i = tid; i < p.batch; i += NT) mine += units(p, request(p, i));
+  const int own = tid < p.batch ? units(p, request(p, tid)) : 0;
+  int mine = own;
+  for (int i = tid + NT; i < p.batch; i += NT) mine += units(p, request(p, i));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(kFull, mine, o);
   if (lane == 0) red[warp] = mine;
@@ -94,7 +95,7 @@ __device__ __forceinline__ void locate(const Params& p, F&& unit_of, int* red, i
   int base = 0;
   for (int i0 = 0; i0 < p.batch; i0 += NT) {
     const int i = i0 + tid;
-    const int u = i < p.batch ? units(p, request(p, i)) : 0;
+    const int u = i0 == 0 ? own : i < p.batch ? units(p, request(p, i)) : 0;
     int incl = u;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -153,18 +154,19 @@ struct Walk {
   __device__ __forceinline__ void next(const Params& p) { skip(p, 1); }
 };
 
-// Requests without work (no keys, or refused) still have outputs.
-template <typename T, int NT>
+// Requests without work (no keys, or refused) still have outputs: a warp each.
+template <int NT>
 __device__ __forceinline__ void clear_idle_requests(const Params& p, int D) {
-  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+  const int lane = threadIdx.x & 31;
+  for (int b = blockIdx.x * (NT / 32) + (threadIdx.x >> 5); b < p.batch; b += gridDim.x * (NT / 32)) {
     const Request r = request(p, b);
     if (r.len != 0 || r.n == 0) continue;
     const int heads = p.kv_heads * p.group;
-    for (int i = threadIdx.x; i < r.n * heads; i += NT) {
+    for (int i = 0; i < r.n * heads; ++i) {
       const int t = r.first + i / heads, h = i % heads;
-      T* o = static_cast<T*>(p.out) + t * p.o_tok + h * p.o_head;
-      for (int d = 0; d < D; ++d) o[d] = T(0.0f);
-      if (p.lse) p.lse[static_cast<long long>(t) * heads + h] = -INFINITY;
+      uint16_t* o = static_cast<uint16_t*>(p.out) + t * p.o_tok + h * p.o_head;  // zero in either type
+      for (int d = lane; d < D; d += 32) o[d] = 0;
+      if (p.lse && lane == 0) p.lse[static_cast<long long>(t) * heads + h] = -INFINITY;
     }
   }
 }

@@ -10,15 +10,17 @@
 // with more, two row tiles against every key tile, which also halves the
 // traffic of keys and values.
 //
-// One block per SM, 13 warps:
-//   warps 0-3, 4-7  softmax of stream 0 and 1: a thread owns a row (its
-//                   tensor-memory lane), reads the scores, keeps the running
-//                   maximum and sum, writes the probabilities over the scores
-//                   as 16-bit values, the left operand of the second product
-//   warps 8-11      loaders: pages to shared memory by 16-byte asynchronous
-//                   copies into the 128-byte-swizzled layout; 8-bit caches go
-//                   through a raw ring and are widened to fp16
-//   warp 12         one thread issues the products
+// One block per SM, groups of four warps:
+//   2 groups  softmax of stream 0 and 1: a thread owns a row (its
+//             tensor-memory lane), reads the scores, keeps the running maximum
+//             and sum, writes the probabilities over the scores as 16-bit
+//             values, the left operand of the second product
+//   1 or 2    loaders.  16-bit caches: pages to shared memory by 16-byte
+//             asynchronous copies into the 128-byte-swizzled layout.  8-bit
+//             ones (2 groups): rows of a raw ring widened to fp16
+//   1         its first warp issues the products; with 8-bit caches two more
+//             fetch the rows of keys and of values, and the
+//             last looks at the scales
 // Tensor memory: scores of the two streams (2 x 128 columns), outputs (2 x D).
 //
 // The output is scaled down only when a row's maximum grew by more than 2^8
@@ -36,12 +38,14 @@ namespace tc {
 
 using namespace sm100;
 
-constexpr int kSoftWarps = 8, kLoadWarps = 4;
-constexpr int kWarpsTc = kSoftWarps + kLoadWarps + 1;
-constexpr int kThreadsTc = 32 * kWarpsTc;
+constexpr int kSoftWarps = 8;
 constexpr int kTile = 128;        // rows and keys of a tile
 constexpr int kTmemCols = 512;
 constexpr int kScaleRing = 8;     // key tiles whose scales are kept
+#ifndef POLY
+#define POLY 0
+#endif
+constexpr int kPolyOf4 = POLY;
 constexpr float kGrow = 8.0f;     // log2 of the growth of a maximum that is tolerated
 
 template <int KIND_, bool BF16_, int D_, bool TOKEN_>
@@ -50,6 +54,14 @@ struct Cfg {
   static constexpr bool BF16 = BF16_;    // type of the products; 8-bit caches: fp16
   static constexpr bool TOKEN = TOKEN_;  // a scale for every token and head
   static constexpr bool kSmall = KIND != kSame;
+  static constexpr int kLoadWarps = kSmall ? 8 : 4;
+  static constexpr int kRowsPerWarp = kTile / kLoadWarps;
+  static constexpr int kWarps = kSoftWarps + kLoadWarps + 4;
+  static constexpr int kThreads = 32 * kWarps;
+  // registers: what the block is launched with (a multiple of 8 that fits), then each group's own share of it
+  static constexpr int kRegs = kSmall ? 96 : 128, kSoftRegs = kSmall ? 144 : 200, kLoadRegs = kSmall ? 56 : 64,
+                       kIssueRegs = kSmall ? 80 : 48;
+  static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + 4 * kIssueRegs <= kWarps * kRegs, "more than launched with");
   static constexpr int kSlots = kSmall ? 3 : 4;  // key or value tiles in shared memory
   static constexpr int kSlot = kTile * D * 2;
   static constexpr int kBlock = kTile * 128;     // 64 dimensions of a tile
@@ -60,36 +72,57 @@ struct Cfg {
   static constexpr int kOffRowWild = kOffWild + kSlots * kWild;
   static constexpr int kOffScale = kOffRowWild + (KIND == kInt8 ? 0 : 2 * kTile * 32);
   static constexpr int kOffMl = kOffScale + (TOKEN ? kScaleRing * (2 * kTile * 4 + 16) : 0);
-  static constexpr int kOffBars = kOffMl + 2 * kTile * 8;
-  static constexpr int kOffQ = (kOffBars + 512 + 1023) / 1024 * 1024;
+  static constexpr int kOffBars = kOffMl + 2 * kTile * 16;
+  static constexpr int kOffQ = (kOffBars + 768 + 1023) / 1024 * 1024;
   static constexpr int raw_depth(int nq) { return !kSmall ? 0 : nq == 1 ? 4 : 2; }
-  static constexpr int smem(int nq) { return kOffQ + nq * kSlot + raw_depth(nq) * kRaw + 1024; }
+  static constexpr int q_bytes(int nq) { return nq * kSlot < 32768 ? 32768 : nq * kSlot; }  // 4 KB a warp for the outputs
+  static constexpr int smem(int nq) { return kOffQ + q_bytes(nq) + raw_depth(nq) * kRaw + 1024; }
 };
 
 struct Bars {
-  uint64_t kv_full[4], kv_empty[4], q_full, s_full[2], p_full[2], o_done[2], both, drain;
+  uint64_t kv_full[4], kv_empty[4], raw_full[4], raw_empty[4], sc_full[kScaleRing], sc_top[kScaleRing], q_full, s_full[2], p_full[2], o_done[2], both, drain;
   uint32_t tmem;
   int abort;
-  int wild[4][kLoadWarps];
+  int wild[4][8];
 };
-static_assert(sizeof(Bars) <= 512, "barriers overflow their place");
+static_assert(sizeof(Bars) <= 768, "barriers overflow their place");
 
 // ---------------------------------------------------------------- instructions
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// The upper half of the operands' descriptors: 8-row groups 1024 bytes apart,
+// version 1, 128-byte swizzle.  The lower half is the address / 16, and for
+// values the distance of the next 64 dimensions.
+constexpr uint32_t kDescHigh = (1024u >> 4) | 1u << 14 | 2u << 29;
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-      "r"(accumulate ? 1 : 0)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "r"(kDescHigh)
       : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
-      "r"(accumulate ? 1 : 0)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(d), "r"(a), "r"(b), "r"(idesc),
+      "r"(accumulate), "r"(kDescHigh)
       : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xFFFFFFFF;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]) {
   asm volatile(
@@ -98,18 +131,25 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-      "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// Whether the phase has completed, without waiting.
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
 // Bounded wait: a barrier that has not completed after two seconds is a fault
 // of this kernel; every role then leaves and the error flag is set.
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
@@ -128,14 +168,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
   }
 }
 
-// Values stored as rows of 128 bytes (64 dimensions) with the 128-byte swizzle,
-// one row per key, as the right operand keys x dimensions with dimensions
+// Lower half of the descriptor of values: rows of 128 bytes (64 dimensions),
+// one per key, as the right operand keys x dimensions with the dimensions
 // contiguous: 8-key groups 1024 bytes apart (stride byte offset), the next 64
 // dimensions 128 keys further (leading byte offset).
-__device__ __forceinline__ uint64_t desc_values(uint32_t addr) {
-  uint64_t d = smem_desc_k128(addr) & ~(0x3FFFull << 16);
-  return d | static_cast<uint64_t>((kTile * 128) >> 4) << 16;
-}
+constexpr uint32_t kValuesLead = static_cast<uint32_t>((kTile * 128) >> 4) << 16;
 // Instruction descriptor: fp32 sums, 16-bit operands, 128 x N, left operand
 // (and right, unless values) with the summed index contiguous.
 __device__ __forceinline__ constexpr uint32_t idesc(bool bf16, int N, bool values) {
@@ -188,6 +225,42 @@ __device__ __forceinline__ void order(int s, int nt, int lead, bool& is_v, int& 
 }
 
 // ---------------------------------------------------------------- loaders
+// A row of a tile in the pages, found one tile ahead: the block table's
+// latency passes under the previous tile's work.
+struct Place {
+  int id, slot;
+  bool valid;
+};
+__device__ __forceinline__ Place look(const Params& p, const Pieces& pc, int tile, int row) {
+  Place at{0, 0, false};
+  const int key = (pc.tile0 + tile) * kTile + row;
+  if (key < pc.w.r.len) {
+    const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
+    at.slot = key - page * p.c.block_size;
+    at.id = p.table[pc.w.b * p.table_stride + page];
+    at.valid = true;
+  }
+  return at;
+}
+
+// 8 values of a row: those that are not finite become 0 and are noted.
+template <bool BF16>
+__device__ __forceinline__ bool clean(uint8_t* bits, int row, int chunk, uint32_t* w) {
+  uint32_t plus = 0, minus = 0, any = 0;
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    uint32_t cl, pl, mi;
+    split_finite<BF16>(w[x], cl, pl, mi);
+    any |= pl | mi;
+    w[x] = cl;
+    plus |= ((pl & 0xFFFFu ? 1u : 0u) | (pl >> 16 ? 2u : 0u)) << (2 * x);
+    minus |= ((mi & 0xFFFFu ? 1u : 0u) | (mi >> 16 ? 2u : 0u)) << (2 * x);
+  }
+  bits[row * 32 + chunk] = static_cast<uint8_t>(plus);
+  bits[row * 32 + 16 + chunk] = static_cast<uint8_t>(minus);
+  return any != 0;
+}
+
 template <typename C>
 struct Loader {
   const Params& p;
@@ -198,176 +271,260 @@ struct Loader {
   int nq, depth, lw, lane;
   volatile int* abort;
 
-  // where the lane's row (32 lw + lane) of a tile lies
-  __device__ __forceinline__ bool row_at(const Pieces& pc, int tile, long long& block, int& slot) const {
-    const int key = (pc.tile0 + tile) * kTile + 32 * lw + lane;
-    block = 0, slot = 0;
-    if (key >= pc.w.r.len) return false;
-    const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
-    slot = key - page * p.c.block_size;
-    block = kv::checked_block(p.table[pc.w.b * p.table_stride + page], p.c.num_blocks, &g_attn_error);
-    return true;
-  }
-
-  // Starts the copies of one tile; count = tiles of this block before it, t = key tiles before its own.
-  __device__ __forceinline__ bool issue(const Pieces& pc, bool is_v, int tile, uint32_t count, uint32_t t) const {
-    long long block;
-    int slot;
-    const bool valid = row_at(pc, tile, block, slot);
-    const unsigned rows_valid = __ballot_sync(kFull, valid);
-    const int h = pc.w.item / row_tiles(p, pc.w.r);
-    const int64_t* st = is_v ? p.c.value_stride : p.c.key_stride;
-    constexpr int kSize = C::kSmall ? 1 : 2;
-    const unsigned long long off = static_cast<unsigned long long>((block * st[0] + slot * st[1]) * kSize);
-    const uint8_t* from = static_cast<const uint8_t*>(is_v ? p.c.value : p.c.key) + h * st[2] * kSize;
-    if constexpr (C::TOKEN) {
-      const int64_t* ss = is_v ? p.c.v_scale_stride : p.c.k_scale_stride;
-      const float* src = (is_v ? p.c.v_scale : p.c.k_scale) + block * ss[0] + slot * ss[1] + h * ss[2];
-      cp_async4(base + C::kOffScale + (((t & (kScaleRing - 1)) * 2 + is_v) * kTile + 32 * lw + lane) * 4, src, valid);
-    }
-    uint32_t dst;
-    if constexpr (C::kSmall) {
-      dst = raw + (count % depth) * C::kRaw;
-    } else {
-      const uint32_t s = count % C::kSlots;
-      if (!wait(&bars->kv_empty[s], ((count / C::kSlots) & 1) ^ 1, abort)) return false;
-      dst = base + s * C::kSlot;
-    }
-    constexpr int kChunks = C::D * kSize / 16, kRows = 32 / kChunks;
-    const int c = lane % kChunks;
+  // Value tiles with new tokens that some of the request's rows may not see: a lane looks through the values it wrote.
+  __device__ __forceinline__ void clean_tail(const Pieces& pc, int tile, uint32_t s) const {
+    if (C::KIND == kInt8 || pc.w.r.n <= 1 || (pc.tile0 + tile + 1) * kTile <= pc.w.r.len - pc.w.r.n) return;
+    constexpr int kChunks = C::D * (C::kSmall ? 1 : 2) / 16, kRows = 32 / kChunks, kSteps = C::kRowsPerWarp / kRows;
+    constexpr uint32_t kExp = C::BF16 ? 0x7F807F80u : 0x7C007C00u;
+    const int c = lane % kChunks, row0 = C::kRowsPerWarp * lw + lane / kChunks;
+    const uint8_t* slot = mem + s * C::kSlot;
+    uint32_t any = 0;
+#pragma unroll 4
+    for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-    for (int i = 0; i < 32 / kRows; ++i) {
-      const int row = i * kRows + lane / kChunks;
-      const unsigned long long o = __shfl_sync(kFull, off, row);
-      const uint32_t at = C::kSmall ? ((32 * lw + row) * kChunks + c) * 16 : place16(32 * lw + row, c);
-      cp_async16(dst + at, from + o + c * 16, (rows_valid >> row) & 1);
-    }
-    return true;
-  }
-
-  // The copies have landed: widen, look for values that are not finite, hand the tile over.
-  __device__ __forceinline__ bool finish(const Pieces& pc, bool is_v, int tile, uint32_t count, uint32_t t) const {
-    const uint32_t s = count % C::kSlots;
-    uint8_t* slot = mem + s * C::kSlot;
-    constexpr int kSize = C::kSmall ? 1 : 2;
-    constexpr int kChunks = C::D * kSize / 16, kRows = 32 / kChunks;
-    const int c = lane % kChunks;
-    // new tokens in this tile that some of the request's rows may not see
-    const bool tail = C::KIND != kInt8 && is_v && pc.w.r.n > 1 &&
-                      (pc.tile0 + tile + 1) * kTile > pc.w.r.len - pc.w.r.n;
-    bool wild = false;
-    uint8_t* bits = mem + C::kOffWild + s * C::kWild;
-    if constexpr (C::kSmall) {
-      if (!wait(&bars->kv_empty[s], ((count / C::kSlots) & 1) ^ 1, abort)) return false;
-      const uint8_t* from = mem + (raw - base) + (count % depth) * C::kRaw;
-#pragma unroll
-      for (int i = 0; i < 32 / kRows; ++i) {
-        const int row = 32 * lw + i * kRows + lane / kChunks;
-        const uint4 u = *reinterpret_cast<const uint4*>(from + (row * kChunks + c) * 16);
-        uint32_t w[4] = {u.x, u.y, u.z, u.w}, o[8];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (C::KIND == kInt8) w[x] ^= 0x80808080u;
-          o[2 * x] = widen<C::KIND, 0, 1>(w[x]);
-          o[2 * x + 1] = widen<C::KIND, 2, 3>(w[x]);
-        }
-        if (tail) {
-#pragma unroll
-          for (int hlf = 0; hlf < 2; ++hlf) wild |= clean(bits, row, 2 * c + hlf, &o[4 * hlf]);
-        }
-        *reinterpret_cast<uint4*>(slot + place16(row, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(slot + place16(row, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+      for (int y = 0; y < (C::kSmall ? 2 : 1); ++y) {
+        const uint4 u = *reinterpret_cast<const uint4*>(slot + place16(row0 + i * kRows, C::kSmall ? 2 * c + y : c));
+        any |= __vcmpeq2(u.x & kExp, kExp) | __vcmpeq2(u.y & kExp, kExp) | __vcmpeq2(u.z & kExp, kExp) | __vcmpeq2(u.w & kExp, kExp);
       }
-    } else if (tail) {
-      for (int i = 0; i < 32 / kRows; ++i) {
-        const int row = 32 * lw + i * kRows + lane / kChunks;
-        uint4* at = reinterpret_cast<uint4*>(slot + place16(row, c));
+    const bool wild = __any_sync(kFull, any != 0);
+    if (lane == 0) bars->wild[s][lw] = wild;
+    if (!wild) return;  // the notes of these rows are not read
+    for (int i = 0; i < kSteps; ++i)
+      for (int y = 0; y < (C::kSmall ? 2 : 1); ++y) {
+        const int row = row0 + i * kRows, c2 = C::kSmall ? 2 * c + y : c;
+        uint4* at = reinterpret_cast<uint4*>(mem + s * C::kSlot + place16(row, c2));
         const uint4 u = *at;
         uint32_t w[4] = {u.x, u.y, u.z, u.w};
-        if (clean(bits, row, c, w)) {
-          wild = true;
-          *at = make_uint4(w[0], w[1], w[2], w[3]);
-        }
+        if (clean<C::BF16>(mem + C::kOffWild + s * C::kWild, row, c2, w)) *at = make_uint4(w[0], w[1], w[2], w[3]);
       }
-    }
-    if (tail) {
-      const bool any = __any_sync(kFull, wild);
-      if (lane == 0) bars->wild[s][lw] = any;
-    }
-    if constexpr (C::TOKEN) {
-      if (is_v) {  // the tile's largest finite scale of values, one number per warp
-        const float* sc = reinterpret_cast<const float*>(mem + C::kOffScale) + ((t & (kScaleRing - 1)) * 2 + 1) * kTile;
-        const float mine = sc[32 * lw + lane];
-        unsigned top = __float_as_uint(mine > 0.0f && mine < 1e30f ? mine : 0.0f);
-        top = __reduce_max_sync(kFull, top);
-        if (lane == 0)
-          reinterpret_cast<uint32_t*>(mem + C::kOffScale + kScaleRing * 2 * kTile * 4)[(t & (kScaleRing - 1)) * 4 + lw] = top;
-      }
-    }
+  }
+  __device__ __forceinline__ void hand_over(uint32_t s) const {
     fence_async();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars->kv_full[s]);
-    return true;
   }
 
-  // 8 values of a row: those that are not finite become 0 and are noted.
-  static __device__ __forceinline__ bool clean(uint8_t* bits, int row, int chunk, uint32_t* w) {
-    uint32_t plus = 0, minus = 0, any = 0;
+  // ---- 16-bit caches: asynchronous copies straight into the tiles.  A tile is started when its place is free, else the
+  // oldest one under way is waited for and handed over.
+  __device__ __forceinline__ void copy(const Pieces& pc, const Place& at, bool is_v, uint32_t dst) const {
+    const unsigned rows_valid = __ballot_sync(kFull, at.valid);
+    const int h = pc.w.item / row_tiles(p, pc.w.r);
+    const uint32_t off = offset16(at, is_v ? p.c.value_stride : p.c.key_stride);
+    constexpr int kChunks = C::D * 2 / 16, kRows = 32 / kChunks;
+    const int c = lane % kChunks;
+    const uint4* from = static_cast<const uint4*>(is_v ? p.c.value : p.c.key) +
+                        (h * (is_v ? p.c.value_stride[2] : p.c.key_stride[2]) / 8 + c);
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      uint32_t cl, pl, mi;
-      split_finite<C::BF16>(w[x], cl, pl, mi);
-      any |= pl | mi;
-      w[x] = cl;
-      plus |= ((pl & 0xFFFFu ? 1u : 0u) | (pl >> 16 ? 2u : 0u)) << (2 * x);
-      minus |= ((mi & 0xFFFFu ? 1u : 0u) | (mi >> 16 ? 2u : 0u)) << (2 * x);
+    for (int i = 0; i < C::kRowsPerWarp / kRows; ++i) {
+      const int row = i * kRows + lane / kChunks;
+      const uint32_t o = __shfl_sync(kFull, off, row);
+      cp_async16(dst + place16(C::kRowsPerWarp * lw + row, c), from + o, (rows_valid >> row) & 1);
     }
-    bits[row * 32 + chunk] = static_cast<uint8_t>(plus);
-    bits[row * 32 + 16 + chunk] = static_cast<uint8_t>(minus);
-    return any != 0;
   }
-
-  template <int LAG>
-  __device__ __forceinline__ void run(int b0, int offset, int count) {
-    const int lead = nq == 1 ? 2 : 1;
-    Pieces a, f;  // tiles being started, tiles being handed over
+  // A row's place in 16-byte units: 32 bits reach 64 GB, which the entry point makes sure of.
+  __device__ __forceinline__ uint32_t offset16(const Place& at, const int64_t* st) const {
+    constexpr int kPer = C::kSmall ? 16 : 8;
+    const int block = static_cast<int>(kv::checked_block(at.id, p.c.num_blocks, &g_attn_error));
+    return static_cast<uint32_t>(block) * static_cast<uint32_t>(st[0] / kPer) +
+           static_cast<uint32_t>(at.slot) * static_cast<uint32_t>(st[1] / kPer);
+  }
+  __device__ __forceinline__ void run_copies(int b0, int offset, int count) {
+    const int lead = nq == 1 ? 2 : 1, row = C::kRowsPerWarp * lw + lane;
+    Pieces a, f, k;  // tiles being started, being handed over, being looked up (two ahead)
     a.start(p, b0, offset, count);
-    f.start(p, b0, offset, count);
-    int as = 0, fs = 0;
-    uint32_t ac = 0, fc = 0, at = 0, ft = 0;  // tiles so far, key tiles before the piece
-    bool more = true;
+    f = a, k = a;
+    int as = 0, fs = 0, ks = 0;
+    uint32_t ac = 0, fc = 0;
+    bool more = true, known = true;
+    auto look_up = [&]() {
+      Place at{0, 0, false};
+      if (!known) return at;
+      bool v;
+      int tile;
+      order(ks, k.nt, lead, v, tile);
+      at = look(p, k, tile, row);
+      if (++ks == 2 * k.nt) {
+        ks = 0;
+        known = k.next(p);
+      }
+      return at;
+    };
+    Place here = look_up(), then = look_up();
     while (true) {
-      if (more) {
-        bool is_v;
-        int tile;
-        order(as, a.nt, lead, is_v, tile);
-        if (!issue(a, is_v, tile, ac, at + tile)) break;
-        ++ac;
-        if (++as == 2 * a.nt) {
-          as = 0;
-          at += a.nt;
-          more = a.next(p);
+      const uint32_t pending = ac - fc;
+      if (more && pending < C::kSlots) {
+        uint64_t* bar = &bars->kv_empty[ac % C::kSlots];
+        const uint32_t parity = ((ac / C::kSlots) & 1) ^ 1;
+        bool free = __all_sync(kFull, mbar_test(bar, parity));
+        if (!free && pending == 0) {
+          if (!wait(bar, parity, abort)) break;
+          free = true;
+        }
+        if (free) {
+          bool is_v;
+          int tile;
+          order(as, a.nt, lead, is_v, tile);
+          copy(a, here, is_v, base + (ac % C::kSlots) * C::kSlot);
+          cp_commit();
+          here = then;
+          then = look_up();
+          ++ac;
+          if (++as == 2 * a.nt) {
+            as = 0;
+            more = a.next(p);
+          }
+          continue;
         }
       }
-      cp_commit();  // empty groups behind the last tile keep the count
-      if (static_cast<int>(ac - fc) > LAG || !more) {
-        if (more)
-          cp_wait<LAG>();
-        else
-          cp_wait<0>();
-        bool is_v;
-        int tile;
-        order(fs, f.nt, lead, is_v, tile);
-        if (!finish(f, is_v, tile, fc, ft + tile)) break;
-        ++fc;
-        if (++fs == 2 * f.nt) {
-          fs = 0;
-          ft += f.nt;
-          if (!f.next(p)) break;
-        }
+      if (pending == 0) break;
+      switch (pending) {
+        case 1: cp_wait<0>(); break;
+        case 2: cp_wait<1>(); break;
+        case 3: cp_wait<2>(); break;
+        default: cp_wait<3>(); break;
+      }
+      bool fv;
+      int ftile;
+      order(fs, f.nt, lead, fv, ftile);
+      if (fv) clean_tail(f, ftile, fc % C::kSlots);
+      hand_over(fc % C::kSlots);
+      ++fc;
+      if (++fs == 2 * f.nt) {
+        fs = 0;
+        if (!f.next(p)) break;
       }
     }
     cp_wait<0>();
+  }
+
+  // ---- 8-bit caches, fetching: one warp takes the key tiles, one the value tiles.
+  __device__ __forceinline__ void run_fetch(bool values, int b0, int offset, int count) {
+    const int lead = nq == 1 ? 2 : 1;
+    const int64_t* st = values ? p.c.value_stride : p.c.key_stride;
+    const int64_t* ss = values ? p.c.v_scale_stride : p.c.k_scale_stride;
+    Pieces pc;
+    pc.start(p, b0, offset, count);
+    uint32_t n0 = 0, t0 = 0;  // tiles and key tiles before the piece
+    bool ok = true;
+    do {
+      const int nt = pc.nt, first = min(lead, nt);
+      const int h = pc.w.item / row_tiles(p, pc.w.r);
+      constexpr int kChunks = C::D / 16, kRows = 32 / kChunks;  // rows a copy of the whole warp takes
+      const int c = lane % kChunks;
+      const uint4* from = static_cast<const uint4*>(values ? p.c.value : p.c.key) + (h * st[2] / 16 + c);
+      const float* scales = (values ? p.c.v_scale : p.c.k_scale) + h * ss[2];
+      Place next[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) next[i] = look(p, pc, 0, 32 * i + lane);
+      for (int j = 0; j < nt && ok; ++j) {
+        Place now[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          now[i] = next[i];
+          if (j + 1 < nt) next[i] = look(p, pc, j + 1, 32 * i + lane);
+        }
+        // its number in the order of loads
+        const uint32_t n = n0 + (values ? (j + lead < nt ? lead + 2 * j : nt + j) : (j < first ? j : 2 * j - lead + 1));
+        const uint32_t r = n & (depth - 1);
+        ok = wait(&bars->raw_empty[r], ((n / depth) & 1) ^ 1, abort);
+        if (!ok) break;
+        const uint32_t dst = raw + r * C::kRaw;
+        const uint32_t sc = base + C::kOffScale + ((((t0 + j) & (kScaleRing - 1)) * 2 + values) * kTile + lane) * 4;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned valid = __ballot_sync(kFull, now[i].valid);
+          const uint32_t off = offset16(now[i], st);
+#pragma unroll
+          for (int k = 0; k < 32 / kRows; ++k) {
+            const int row = k * kRows + lane / kChunks;
+            const uint32_t o = __shfl_sync(kFull, off, row);
+            cp_async16(dst + ((32 * i + row) * kChunks + c) * 16, from + o, (valid >> row) & 1);
+          }
+          if constexpr (C::TOKEN) {
+            const long long block = kv::checked_block(now[i].id, p.c.num_blocks, &g_attn_error);
+            cp_async4(sc + 128 * i, scales + block * ss[0] + now[i].slot * ss[1], now[i].valid);
+          }
+        }
+        if (C::TOKEN && values) cp_arrive(&bars->sc_full[(t0 + j) & (kScaleRing - 1)]);
+        cp_arrive(&bars->raw_full[r]);
+      }
+      n0 += 2 * nt;
+      t0 += nt;
+    } while (ok && pc.next(p));
+    cp_wait<0>();
+  }
+  // Arrives when this lane's copies so far have landed.
+  static __device__ __forceinline__ void cp_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+  }
+
+  // ---- token scales: the largest finite one of each tile's values, for the reference the probabilities are scaled by.
+  __device__ __forceinline__ void run_scales(int b0, int offset, int count) {
+    Pieces pc;
+    pc.start(p, b0, offset, count);
+    uint32_t t = 0;
+    bool ok = true;
+    do {
+      for (int j = 0; j < pc.nt && ok; ++j, ++t) {
+        const int ring = t & (kScaleRing - 1);
+        ok = wait(&bars->sc_full[ring], (t / kScaleRing) & 1, abort);
+        if (!ok) break;
+        const float4 s4 = *reinterpret_cast<const float4*>(mem + C::kOffScale + ((ring * 2 + 1) * kTile + 4 * lane) * 4);
+        const float v[4] = {s4.x, s4.y, s4.z, s4.w};
+        unsigned top = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i] > 0.0f && v[i] < 1e30f ? v[i] : 0.0f));
+        top = __reduce_max_sync(kFull, top);
+        if (lane == 0) {
+          *reinterpret_cast<uint32_t*>(mem + C::kOffScale + kScaleRing * 2 * kTile * 4 + ring * 4) = top;
+          mbar_arrive(&bars->sc_top[ring]);
+        }
+      }
+    } while (ok && pc.next(p));
+  }
+
+  // ---- 8-bit caches, widening: raw rows to fp16 in the swizzled tiles.
+  __device__ __forceinline__ void run_widen(int b0, int offset, int count) {
+    const int lead = nq == 1 ? 2 : 1;
+    constexpr int kChunks = C::D / 16, kRows = 32 / kChunks, kSteps = C::kRowsPerWarp / kRows;
+    const int c = lane % kChunks, row0 = C::kRowsPerWarp * lw + lane / kChunks;
+    Pieces pc;
+    pc.start(p, b0, offset, count);
+    uint32_t n = 0;
+    bool ok = true;
+    do {
+      for (int st = 0; st < 2 * pc.nt && ok; ++st, ++n) {
+        bool is_v;
+        int tile;
+        order(st, pc.nt, lead, is_v, tile);
+        const uint32_t r = n & (depth - 1), s = n % C::kSlots;
+        ok = wait(&bars->raw_full[r], (n / depth) & 1, abort);
+        if (!ok) break;
+        const uint8_t* from = mem + (raw - base) + r * C::kRaw + (row0 * kChunks + c) * 16;
+        uint4 u[kSteps];
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) u[i] = *reinterpret_cast<const uint4*>(from + i * kRows * kChunks * 16);
+        ok = wait(&bars->kv_empty[s], ((n / C::kSlots) & 1) ^ 1, abort);
+        if (!ok) break;
+        uint8_t* slot = mem + s * C::kSlot;
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int row = row0 + i * kRows;
+          uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w}, o[8];
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            if (C::KIND == kInt8) w[x] ^= 0x80808080u;
+            o[2 * x] = widen<C::KIND, 0, 1>(w[x]);
+            o[2 * x + 1] = widen<C::KIND, 2, 3>(w[x]);
+          }
+          *reinterpret_cast<uint4*>(slot + place16(row, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
+          *reinterpret_cast<uint4*>(slot + place16(row, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+        }
+        if (is_v) clean_tail(pc, tile, s);
+        hand_over(s);
+        if (lane == 0) mbar_arrive(&bars->raw_empty[r]);
+      }
+    } while (ok && pc.next(p));
   }
 };
 
@@ -398,6 +555,29 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
   return r;
 }
 
+// 2^x of two values on the multiply-add pipe, where the special-function unit
+// (16 results per cycle and SM) is what the softmax waits for: the whole part
+// by adding 1.5 * 2^23, 2^f on [-1/2, 1/2] by a polynomial of degree 5 fitted
+// for the least relative error (8e-8), the whole part added to the exponent.
+// x <= 2^7; below -126 the result is under 2^-125; NaN stays NaN.
+__device__ __forceinline__ float2 exp2_pair(unsigned long long x) {
+  float2 c = unpair(x);
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.x));
+  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.y));
+  x = pair(c.x, c.y);
+  const unsigned long long t = add2(x, pair(12582912.0f, 12582912.0f));
+  const unsigned long long f = add2(x, mul2(add2(t, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f)));
+  unsigned long long r = pair(0.0013276472454890609f, 0.0013276472454890609f);
+  r = fma2(r, f, pair(0.009675540961325169f, 0.009675540961325169f));
+  r = fma2(r, f, pair(0.05550713092088699f, 0.05550713092088699f));
+  r = fma2(r, f, pair(0.24022120237350464f, 0.24022120237350464f));
+  r = fma2(r, f, pair(0.6931469440460205f, 0.6931469440460205f));
+  r = fma2(r, f, pair(1.0000001192092896f, 1.0000001192092896f));
+  const float2 tt = unpair(t), rr = unpair(r);
+  return make_float2(__uint_as_float(__float_as_uint(rr.x) + (__float_as_uint(tt.x) << 23)),
+                     __uint_as_float(__float_as_uint(rr.y) + (__float_as_uint(tt.y) << 23)));
+}
+
 // One thread's row of the softmax.
 template <typename C>
 struct Soft {
@@ -409,40 +589,41 @@ struct Soft {
   float m, l, vref, qscale;  // reference maximum and sum; reference scale of the values
   bool wild;
 
-  // The row of queries into shared memory: chunks [c0, c1) of 8 dimensions.
-  // bf16 queries of an 8-bit cache become fp16 after a power of two brings the
-  // row's largest value to [1, 2): exact for all that count beside it.
+  // Chunks [c0, c1) of 8 dimensions of a row of queries into shared memory.  bf16 queries of an 8-bit cache become fp16 after a power of two brings the row's
+  // largest value to [1, 2): exact for all that count beside it.
   __device__ __forceinline__ void load_q(uint8_t* q_tile, int row, const void* src, bool ok, int c0, int c1) {
     const float scale = p.scale_log2;
     qscale = fabsf(scale);
+    uint4 q[C::D / 8];
+#pragma unroll
+    for (int c = 0; c < C::D / 8; ++c) q[c] = ok ? static_cast<const uint4*>(src)[c] : make_uint4(0u, 0u, 0u, 0u);
     const uint32_t flip = scale < 0.0f ? 0x80008000u : 0u;  // the sign goes onto the queries: maxima stay maxima
-    const uint4* from = static_cast<const uint4*>(src);
-    float down = 1.0f;
-    const bool convert = C::kSmall && p.bf16;
-    if (convert && ok) {
+    if (C::kSmall && p.bf16) {
       float top = 0.0f;
+#pragma unroll
       for (int c = 0; c < C::D / 8; ++c) {
-        const uint4 u = from[c];
-        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
 #pragma unroll
         for (int x = 0; x < 4; ++x)
           top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[x] << 16)), fabsf(__uint_as_float(w[x] & 0xFFFF0000u))));
       }
       const uint32_t ex = min(max(__float_as_uint(top) & 0x7F800000u, 0x0A000000u), 0x75000000u);
-      down = __uint_as_float(0x7F000000u - ex);
+      const float down = __uint_as_float(0x7F000000u - ex);
       qscale *= __uint_as_float(ex);
-    }
-    for (int c = c0; c < c1; ++c) {
-      uint4 u = make_uint4(0u, 0u, 0u, 0u);
-      if (ok) u = from[c];
-      uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      if (convert) {
+#pragma unroll
+      for (int c = 0; c < C::D / 8; ++c) {
+        uint32_t w[4] = {q[c].x, q[c].y, q[c].z, q[c].w};
 #pragma unroll
         for (int x = 0; x < 4; ++x)
           w[x] = pack2<false>(__uint_as_float(w[x] << 16) * down, __uint_as_float(w[x] & 0xFFFF0000u) * down);
+        q[c] = make_uint4(w[0], w[1], w[2], w[3]);
       }
-      *reinterpret_cast<uint4*>(q_tile + place16(row, c)) = make_uint4(w[0] ^ flip, w[1] ^ flip, w[2] ^ flip, w[3] ^ flip);
     }
+#pragma unroll
+    for (int c = 0; c < C::D / 8; ++c)
+      if (c >= c0 && c < c1)
+        *reinterpret_cast<uint4*>(q_tile + place16(row, c)) =
+            make_uint4(q[c].x ^ flip, q[c].y ^ flip, q[c].z ^ flip, q[c].w ^ flip);
   }
 
   __device__ __forceinline__ void begin() {
@@ -450,31 +631,61 @@ struct Soft {
     wild = false;
   }
 
-  // Scores of one key tile to probabilities.  tail: some keys are not seen (a bit each in seen).
+  // Scores 32 c .. 32 c + 31 times the keys' own scales, unseen ones -inf.
+  template <bool TAIL>
+  static __device__ __forceinline__ void scaled(uint32_t (&s)[32], const float* ks, uint32_t seen) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      if constexpr (C::TOKEN) {
+        const float4 k = *reinterpret_cast<const float4*>(ks + i);
+        const float2 a = unpair(mul2(pair(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), pair(k.x, k.y)));
+        const float2 b = unpair(mul2(pair(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), pair(k.z, k.w)));
+        s[i] = __float_as_uint(a.x), s[i + 1] = __float_as_uint(a.y);
+        s[i + 2] = __float_as_uint(b.x), s[i + 3] = __float_as_uint(b.y);
+      }
+      if (TAIL) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (!((seen >> (i + x)) & 1)) s[i + x] = 0xFF800000u;
+      }
+    }
+  }
+  static __device__ __forceinline__ float top_of(const uint32_t (&s)[32], float top) {
+    float t0 = top, t1 = __uint_as_float(s[1]);
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      t0 = fmaxf(fmaxf(t0, __uint_as_float(s[i])), __uint_as_float(s[i + 2]));
+      t1 = fmaxf(fmaxf(t1, __uint_as_float(s[i + 1])), __uint_as_float(s[i + 3]));
+    }
+    return fmaxf(t0, t1);
+  }
+
+  // Scores of one key tile to probabilities.  TAIL: some keys are not seen (a bit each in seen).
   template <bool TAIL>
   __device__ __forceinline__ void tile(const uint32_t (&seen)[4], const float* ks, const float* vs, float vmax, bool first) {
+    // 16-bit caches hold the row in registers; with 8-bit ones, whose loaders need the registers, it is read twice
+    constexpr bool kHold = !C::kSmall;
+    uint32_t s[kHold ? 4 : 2][32];
     float top = -INFINITY;
+    if constexpr (kHold) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t s[32];
-      tmem_ld32(tmem_s + 32 * c, s);
+      for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + 32 * c, s[c]);
       tmem_ld_wait();
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        float v[4];
-#pragma unroll
-        for (int x = 0; x < 4; ++x) v[x] = __uint_as_float(s[i + x]);
-        if constexpr (C::TOKEN) {
-          const float4 k = *reinterpret_cast<const float4*>(ks + 32 * c + i);
-          const float2 a = unpair(mul2(pair(v[0], v[1]), pair(k.x, k.y))), b = unpair(mul2(pair(v[2], v[3]), pair(k.z, k.w)));
-          v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
-        }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (TAIL && !((seen[c] >> (i + x)) & 1)) v[x] = -INFINITY;
-          top = fmaxf(top, v[x]);
-        }
+      for (int c = 0; c < 4; ++c) {
+        scaled<TAIL>(s[c], ks, seen[c]);
+        top = top_of(s[c], top);
       }
+    } else {
+      tmem_ld32(tmem_s, s[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tmem_ld_wait();
+        if (c < 3) tmem_ld32(tmem_s + 32 * (c + 1), s[(c + 1) & 1]);
+        scaled<TAIL>(s[c & 1], ks + 32 * c, seen[c]);
+        top = top_of(s[c & 1], top);
+      }
+      tmem_ld32(tmem_s, s[0]);
     }
     top *= qscale;
     // the reference moves when the maximum left it by more than 2^kGrow
@@ -492,46 +703,52 @@ struct Soft {
       }
     }
     if (!first && __any_sync(kFull, alpha != 1.0f)) {
-#pragma unroll
-      for (int c = 0; c < C::D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(tmem_o + 32 * c, o);
+#pragma unroll 1
+      for (int c = 0; c < C::D / 16; ++c) {
+        uint32_t o[16];
+        tmem_ld16(tmem_o + 16 * c, o);
         tmem_ld_wait();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-        tmem_st32(tmem_o + 32 * c, o);
+        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+        tmem_st16(tmem_o + 16 * c, o);
       }
     }
     const float sub = m == -INFINITY ? 0.0f : m;
     const unsigned long long q2 = pair(qscale, qscale), m2 = pair(-sub, -sub);
     const float inv = C::TOKEN ? __uint_as_float(0x7F000000u - __float_as_uint(vref)) : 1.0f;
+    const unsigned long long i2 = pair(inv, inv);
     unsigned long long sum0 = pair(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      uint32_t s[32], out[16];
-      tmem_ld32(tmem_s + 32 * c, s);
-      tmem_ld_wait();
+      uint32_t(&v)[32] = s[kHold ? c : c & 1];
+      uint32_t out[16];
+      if constexpr (!kHold) {
+        tmem_ld_wait();
+        if (c < 3) tmem_ld32(tmem_s + 32 * (c + 1), s[(c + 1) & 1]);
+        scaled<TAIL>(v, ks + 32 * c, seen[c]);
+      }
 #pragma unroll
       for (int i = 0; i < 32; i += 4) {
-        unsigned long long a = pair(__uint_as_float(s[i]), __uint_as_float(s[i + 1]));
-        unsigned long long b = pair(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3]));
-        if constexpr (C::TOKEN) {
-          const float4 k = *reinterpret_cast<const float4*>(ks + 32 * c + i);
-          a = mul2(a, pair(k.x, k.y)), b = mul2(b, pair(k.z, k.w));
+        const unsigned long long xa = fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), q2, m2);
+        const unsigned long long xb = fma2(pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), q2, m2);
+        float2 ea = unpair(xa), eb;
+        ea = make_float2(exp2_fast(ea.x), exp2_fast(ea.y));
+        if ((i / 4) % 4 < kPolyOf4) {
+          eb = exp2_pair(xb);
+        } else {
+          eb = unpair(xb);
+          eb = make_float2(exp2_fast(eb.x), exp2_fast(eb.y));
         }
-        const float2 ea = unpair(fma2(a, q2, m2)), eb = unpair(fma2(b, q2, m2));
         float e[4] = {ea.x, ea.y, eb.x, eb.y};
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          e[x] = exp2_fast(e[x]);
-          if (TAIL && !((seen[c] >> (i + x)) & 1)) e[x] = 0.0f;
+          if (TAIL && !((seen[c] >> (i + x)) & 1)) e[x] = 0.0f;  // a scale of 0 makes -inf NaN
         }
-        a = pair(e[0], e[1]), b = pair(e[2], e[3]);
+        unsigned long long a = pair(e[0], e[1]), b = pair(e[2], e[3]);
         sum0 = add2(sum0, a), sum1 = add2(sum1, b);
         if constexpr (C::TOKEN) {
-          const float4 v = *reinterpret_cast<const float4*>(vs + 32 * c + i);
-          const unsigned long long i2 = pair(inv, inv);
-          a = mul2(a, mul2(pair(v.x, v.y), i2)), b = mul2(b, mul2(pair(v.z, v.w), i2));
+          const float4 vv = *reinterpret_cast<const float4*>(vs + 32 * c + i);
+          a = mul2(a, mul2(pair(vv.x, vv.y), i2)), b = mul2(b, mul2(pair(vv.z, vv.w), i2));
           const float2 fa = unpair(a), fb = unpair(b);
           e[0] = fa.x, e[1] = fa.y, e[2] = fb.x, e[3] = fb.y;
           if (TAIL) {
@@ -543,6 +760,7 @@ struct Soft {
         out[i / 2] = pack2<C::BF16>(e[0], e[1]);
         out[i / 2 + 1] = pack2<C::BF16>(e[2], e[3]);
       }
+      // over the scores 16 c .. 16 c + 15, which have been read
       tmem_st16(tmem_s + 16 * c, out);
     }
     const float2 sa = unpair(add2(sum0, sum1));
@@ -557,7 +775,7 @@ struct Soft {
       for (int x = 0; x < 8; ++x) mine[x] = 0;
     }
     for (int j = 0; j < kTile; ++j) {
-      if (!((seen[j >> 5] >> (j & 31)) & 1)) continue;
+      if (!((seen[j >> 5] >> (j & 31)) & 1) || !bars->wild[slot][j / C::kRowsPerWarp]) continue;
       const uint32_t* bits = reinterpret_cast<const uint32_t*>(mem + C::kOffWild + slot * C::kWild + j * 32);
       for (int x = 0; x < 8; ++x)
         if ((x & 3) < C::D / 32) mine[x] |= bits[x];
@@ -565,39 +783,50 @@ struct Soft {
   }
 };
 
+// A warp's staged lines (PARTS x 16 bytes of each of its 32 rows, parts exclusive-ored with the row) to the rows' places.
+template <int PARTS>
+__device__ __forceinline__ void put_lines(const uint8_t* stage, uint8_t* mine, unsigned rows_ok, int lane) {
+  constexpr int kPer = 32 / PARTS;  // rows a store of the whole warp takes
+  __syncwarp();
+  const int part = lane % PARTS;
+  uint4 u[PARTS];
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const int row = i * kPer + lane / PARTS;
+    u[i] = *reinterpret_cast<const uint4*>(stage + row * 128 + ((part ^ (row & 7)) << 4));
+  }
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) {
+    const int row = i * kPer + lane / PARTS;
+    uint8_t* to = reinterpret_cast<uint8_t*>(__shfl_sync(kFull, reinterpret_cast<unsigned long long>(mine), row));
+    if ((rows_ok >> row) & 1) *reinterpret_cast<uint4*>(to + part * 16) = u[i];
+  }
+  __syncwarp();
+}
+
 template <typename C>
-__global__ void __launch_bounds__(kThreadsTc, 1) attend_tc_kernel(const __grid_constant__ Params p, int nq) {
+__global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_constant__ Params p, int nq) {
   constexpr int D = C::D;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw_addr = smem_u32(smem_raw);
   uint8_t* mem = smem_raw + ((1024 - (raw_addr & 1023)) & 1023);
   const uint32_t base = smem_u32(mem);
   Bars* bars = reinterpret_cast<Bars*>(mem + C::kOffBars);
-  __shared__ int red[kWarpsTc + 2];
+  __shared__ int red[C::kWarps + 2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   volatile int* abort = &bars->abort;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  if (p.bf16)
-    clear_idle_requests<__nv_bfloat16, kThreadsTc>(p, D);
-  else
-    clear_idle_requests<__half, kThreadsTc>(p, D);
-
-  int total, unit, b0, before, share = 0;
-  locate<kThreadsTc>(
-      p,
-      [&](int tot) {
-        share = share_of(p, tot, gridDim.x);
-        return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
-      },
-      red, total, unit, b0, before);
-  if (unit >= total) return;
-  const int count = min(share, total - unit), offset = unit - before;
-
   if (tid == 0) {
     for (int i = 0; i < 4; ++i) {
-      mbar_init(&bars->kv_full[i], kLoadWarps);
+      mbar_init(&bars->kv_full[i], C::kLoadWarps);
       mbar_init(&bars->kv_empty[i], 1);
+      mbar_init(&bars->raw_full[i], 32);
+      mbar_init(&bars->raw_empty[i], C::kLoadWarps);
+    }
+    for (int i = 0; i < kScaleRing; ++i) {
+      mbar_init(&bars->sc_full[i], 32);
+      mbar_init(&bars->sc_top[i], 1);
     }
     mbar_init(&bars->q_full, kSoftWarps);
     for (int i = 0; i < 2; ++i) {
@@ -610,105 +839,136 @@ __global__ void __launch_bounds__(kThreadsTc, 1) attend_tc_kernel(const __grid_c
     bars->abort = 0;
     fence_barrier_init();
   }
-  if (warp == kWarpsTc - 1) {
+  if (warp == C::kWarps - 4) {
     tmem_alloc(&bars->tmem, kTmemCols);
     tmem_relinquish();
   }
+  int total, unit, b0, before, share = 0;
+  locate<C::kThreads>(
+      p,
+      [&](int tot) {
+        share = share_of(p, tot, gridDim.x);
+        return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
+      },
+      red, total, unit, b0, before);
+  const int count = min(share, total - unit), offset = unit - before;
+  const bool busy = unit < total;
+
+  clear_idle_requests<C::kThreads>(p, D);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = bars->tmem;
   const uint32_t q_addr = base + C::kOffQ;
 
-  if (warp >= kSoftWarps && warp < kSoftWarps + kLoadWarps) {
+  Loader<C> ld{p, bars, base, mem, q_addr + C::q_bytes(nq), nq, C::raw_depth(nq), warp - kSoftWarps, lane, abort};
+  if (!busy) {
+    // fewer units than blocks
+  } else if (warp >= kSoftWarps && warp < kSoftWarps + C::kLoadWarps) {
     // ------------------------------------------------ loaders
-    Loader<C> ld{p, bars, base, mem, q_addr + nq * C::kSlot, nq, C::raw_depth(nq), warp - kSoftWarps, lane, abort};
-    if constexpr (!C::kSmall) {
-      ld.template run<2>(b0, offset, count);
-    } else if (nq == 1) {
-      ld.template run<3>(b0, offset, count);
-    } else {
-      ld.template run<1>(b0, offset, count);
-    }
-  } else if (warp == kWarpsTc - 1 && lane == 0) {
+    regs_down<C::kLoadRegs>();
+    if constexpr (C::kSmall)
+      ld.run_widen(b0, offset, count);
+    else
+      ld.run_copies(b0, offset, count);
+  } else if (warp >= kSoftWarps + C::kLoadWarps) {
     // ------------------------------------------------ products
-    Pieces pc;
-    pc.start(p, b0, offset, count);
-    const int lead = nq == 1 ? 2 : 1;
-    uint32_t kv = 0, piece = 0, pp[2] = {0, 0};  // tiles taken, pieces, probabilities taken
-    auto scores = [&](int x, uint32_t s) {        // S_x = Q_x K^T
-      const uint32_t q = q_addr + (nq == 1 ? 0 : x) * C::kSlot, k = base + s * C::kSlot;
+    regs_down<C::kIssueRegs>();
+    if (warp == C::kWarps - 4) {
+      // the whole warp walks the tiles, one lane issues: addresses stay in uniform registers
+      const bool leader = elect_one();
+      Pieces pc;
+      pc.start(p, b0, offset, count);
+      const int lead = nq == 1 ? 2 : 1;
+      uint32_t kv = 0, piece = 0, pp0 = 0, pp1 = 0;  // tiles taken, pieces, probabilities taken
+      const uint32_t q16 = q_addr >> 4, kv16 = base >> 4;
+      auto scores = [&](int x, uint32_t s) {  // S_x = Q_x K^T
+        const uint32_t q = q16 + (nq == 1 ? 0 : x) * (C::kSlot >> 4), k = kv16 + s * (C::kSlot >> 4);
+        const uint32_t d = tmem + x * kTile;
+        if (leader) {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t o = (kk >> 2) * C::kBlock + (kk & 3) * 32;
-        mma_ss(tmem + x * kTile, smem_desc_k128(q + o), smem_desc_k128(k + o), idesc(C::BF16, kTile, false), kk > 0);
-      }
-      umma_commit(&bars->s_full[x]);
-    };
-    auto outputs = [&](int x, uint32_t s, bool accumulate) {  // O_x += P_x V
-      const uint32_t v = base + s * C::kSlot;
-#pragma unroll
-      for (int kk = 0; kk < kTile / 16; ++kk)
-        mma_ts(tmem + 2 * kTile + x * D, tmem + x * kTile + kk * 8, desc_values(v + kk * 2048), idesc(C::BF16, D, true),
-               accumulate || kk > 0);
-    };
-    auto take = [&](uint32_t n) { return wait(&bars->kv_full[n % C::kSlots], (n / C::kSlots) & 1, abort); };
-    bool ok = true;
-    do {
-      const int nt = pc.nt;
-      ok = wait(&bars->q_full, piece & 1, abort);
-      ++piece;
-      if (!ok) break;
-      for (int j = 0; j < min(lead, nt) && ok; ++j) {
-        ok = take(kv);
-        if (!ok) break;
-        tc_fence_after();
-        if (nq == 1) {
-          scores(j, kv % C::kSlots);
-        } else {
-          scores(0, kv % C::kSlots);
-          scores(1, kv % C::kSlots);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t o = ((kk >> 2) * C::kBlock + (kk & 3) * 32) >> 4;
+            mma_ss(d, q + o, k + o, idesc(C::BF16, kTile, false), kk > 0);
+          }
+          umma_commit(&bars->s_full[x]);
         }
-        umma_commit(&bars->kv_empty[kv % C::kSlots]);
-        ++kv;
-      }
-      for (int j = 0; j < nt && ok; ++j) {
-        const uint32_t v = kv++;
-        const bool more = j + lead < nt;
-        const uint32_t k = more ? kv++ : 0;
-        ok = take(v);
-        for (int y = 0; y < nq && ok; ++y) {
-          const int x = nq == 1 ? j & 1 : y;
-          ok = wait(&bars->p_full[x], pp[x] & 1, abort);
-          ++pp[x];
+      };
+      auto outputs = [&](int x, uint32_t s, bool accumulate) {  // O_x += P_x V
+        const uint32_t v = (kv16 + s * (C::kSlot >> 4)) | kValuesLead;
+        const uint32_t d = tmem + 2 * kTile + x * D, a = tmem + x * kTile;
+        if (leader) {
+#pragma unroll
+          for (int kk = 0; kk < kTile / 16; ++kk)
+            mma_ts(d, a + kk * 8, v + kk * (2048 >> 4), idesc(C::BF16, D, true), accumulate || kk > 0);
+        }
+      };
+      auto give = [&](uint64_t* bar) {
+        if (leader) umma_commit(bar);
+      };
+      auto take = [&](uint32_t n) { return wait(&bars->kv_full[n % C::kSlots], (n / C::kSlots) & 1, abort); };
+      bool ok = true;
+      do {
+        const int nt = pc.nt;
+        ok = wait(&bars->q_full, piece & 1, abort);
+        ++piece;
+        if (!ok) break;
+        for (int j = 0; j < min(lead, nt) && ok; ++j) {
+          ok = take(kv);
           if (!ok) break;
           tc_fence_after();
-          outputs(x, v % C::kSlots, nq == 1 ? j > 1 : j > 0);
-          if (nq == 1 ? j + 2 >= nt : j + 1 == nt) umma_commit(&bars->o_done[x]);
-          if (y == nq - 1) umma_commit(&bars->kv_empty[v % C::kSlots]);
-          if (more) {
-            if (y == 0) ok = take(k);
+          if (nq == 1) {
+            scores(j, kv % C::kSlots);
+          } else {
+            scores(0, kv % C::kSlots);
+            scores(1, kv % C::kSlots);
+          }
+          give(&bars->kv_empty[kv % C::kSlots]);
+          ++kv;
+        }
+        for (int j = 0; j < nt && ok; ++j) {
+          const uint32_t v = kv++;
+          const bool more = j + lead < nt;
+          const uint32_t k = more ? kv++ : 0;
+          ok = take(v);
+          for (int y = 0; y < nq && ok; ++y) {
+            const int x = nq == 1 ? j & 1 : y;
+            ok = wait(&bars->p_full[x], (x ? pp1 : pp0) & 1, abort);
+            x ? ++pp1 : ++pp0;
             if (!ok) break;
             tc_fence_after();
-            scores(x, k % C::kSlots);
-            if (y == nq - 1) umma_commit(&bars->kv_empty[k % C::kSlots]);
+            outputs(x, v % C::kSlots, nq == 1 ? j > 1 : j > 0);
+            if (nq == 1 ? j + 2 >= nt : j + 1 == nt) give(&bars->o_done[x]);
+            if (y == nq - 1) give(&bars->kv_empty[v % C::kSlots]);
+            if (more) {
+              if (y == 0) ok = take(k);
+              if (!ok) break;
+              tc_fence_after();
+              scores(x, k % C::kSlots);
+              if (y == nq - 1) give(&bars->kv_empty[k % C::kSlots]);
+            }
           }
         }
+      } while (ok && pc.next(p));
+      // every product issued has ended before the block gives its memory back
+      give(&bars->drain);
+      for (uint32_t n = 0; n < (1u << 22) && !mbar_try_wait(&bars->drain, 0); ++n) {
       }
-    } while (ok && pc.next(p));
-    // every product issued has ended before the block gives its memory back
-    umma_commit(&bars->drain);
-    for (uint32_t n = 0; n < (1u << 22) && !mbar_try_wait(&bars->drain, 0); ++n) {
+    } else if (C::kSmall && warp < C::kWarps - 1) {
+      ld.run_fetch(warp == C::kWarps - 2, b0, offset, count);
+    } else if (C::TOKEN) {
+      ld.run_scales(b0, offset, count);
     }
   } else if (warp < kSoftWarps) {
     // ------------------------------------------------ softmax and output
+    regs_up<C::kSoftRegs>();
     const int x = warp >> 2, wrow = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     Soft<C> so{p, bars, mem, tmem + lanes + x * kTile, tmem + lanes + 2 * kTile + x * D, abort};
-    float2* ml = reinterpret_cast<float2*>(mem + C::kOffMl);
+    float4* ml = reinterpret_cast<float4*>(mem + C::kOffMl);  // a row's maximum, sum, scale of values, note
     const float* scales = reinterpret_cast<const float*>(mem + C::kOffScale);
     const float* vtop = scales + kScaleRing * 2 * kTile;
-    uint32_t kv = 0, t0 = 0, sp = 0, op[2] = {0, 0}, meets = 0;
+    uint32_t kv = 0, t0 = 0, sp = 0, op0 = 0, op1 = 0, meets = 0;
     auto meet = [&]() {  // the two streams' warps
       __syncwarp();
       if (lane == 0) mbar_arrive(&bars->both);
@@ -717,21 +977,35 @@ __global__ void __launch_bounds__(kThreadsTc, 1) attend_tc_kernel(const __grid_c
     const int lead = nq == 1 ? 2 : 1;
     Pieces pc;
     pc.start(p, b0, offset, count);
-    bool ok = true;
+    // the thread's row of a piece, and its queries
+    struct Row {
+      int h, qi, head, t;
+      bool ok, warp_ok;
+      const uint8_t* q;
+    };
+    auto row_of = [&](const Pieces& at) {
+      const int rts = row_tiles(p, at.w.r), rows = at.w.r.n * p.group;
+      Row o;
+      o.h = at.w.item / rts;
+      const int row = ((at.w.item - o.h * rts) << p.rows_log2) + (nq == 1 ? 0 : x * kTile) + wrow;
+      o.ok = row < rows;
+      o.warp_ok = row - lane < rows;
+      o.qi = row / p.group;
+      o.head = o.h * p.group + row - o.qi * p.group;
+      o.t = at.w.r.first + o.qi;
+      o.q = static_cast<const uint8_t*>(p.q) + (o.t * p.q_tok + o.head * p.q_head) * 2;
+      return o;
+    };
+    bool ok = true, more = true;
+    Row me = row_of(pc);
     do {
       const Request r = pc.w.r;
-      const int rts = row_tiles(p, r);
-      const int h = pc.w.item / rts, rt = pc.w.item - h * rts;
-      const int row = (rt << p.rows_log2) + (nq == 1 ? 0 : x * kTile) + wrow;
-      const int rows = r.n * p.group;
-      const bool row_ok = row < rows;
-      const bool warp_ok = row - lane < rows;
-      const int qi = row / p.group, head = h * p.group + row - qi * p.group, t = r.first + qi;
+      const int h = me.h, qi = me.qi, head = me.head, t = me.t;
+      const bool row_ok = me.ok, warp_ok = me.warp_ok;
       so.begin();
       {
         const int half = D / 16;  // with one row tile the two warps of a row share the copy
-        const uint8_t* src = static_cast<const uint8_t*>(p.q) + (t * p.q_tok + head * p.q_head) * 2;
-        so.load_q(mem + C::kOffQ + (nq == 1 ? 0 : x) * C::kSlot, wrow, src, row_ok, nq == 1 ? x * half : 0,
+        so.load_q(mem + C::kOffQ + (nq == 1 ? 0 : x) * C::kSlot, wrow, me.q, row_ok, nq == 1 ? x * half : 0,
                   nq == 1 ? x * half + half : D / 8);
         if constexpr (C::kSmall && !C::TOKEN) so.qscale *= p.c.k_scale[h * p.c.k_scale_stride[2]];
         fence_async();
@@ -752,25 +1026,28 @@ __global__ void __launch_bounds__(kThreadsTc, 1) attend_tc_kernel(const __grid_c
           float vmax = 0.0f;
           uint32_t seen[4] = {kFull, kFull, kFull, kFull};
           int slot = 0;
-          if (C::TOKEN || (C::KIND != kInt8 && tail && r.n > 1)) {
-            // the value tile's scales and notes are needed: its place in the order of loads
-            const uint32_t n = kv + (j + lead < pc.nt ? lead + 2 * j : min(lead, pc.nt) + max(pc.nt - lead, 0) + j);
+          if constexpr (C::TOKEN) {
+            const int ring = (t0 + j) & (kScaleRing - 1);
+            ok = wait(&bars->sc_top[ring], ((t0 + j) / kScaleRing) & 1, abort);
+            if (!ok) break;
+            ks = scales + ring * 2 * kTile, vs = ks + kTile;
+            vmax = vtop[ring];
+          }
+          if (C::KIND != kInt8 && tail && r.n > 1) {
+            // the value tile's notes are needed: its place in the order of loads
+            const uint32_t n = kv + (j + lead < pc.nt ? lead + 2 * j : pc.nt + j);
             slot = n % C::kSlots;
             ok = wait(&bars->kv_full[slot], (n / C::kSlots) & 1, abort);
             if (!ok) break;
-            if constexpr (C::TOKEN) {
-              const int ring = (t0 + j) & (kScaleRing - 1);
-              ks = scales + ring * 2 * kTile, vs = ks + kTile;
-              const float4 v4 = *reinterpret_cast<const float4*>(vtop + 4 * ring);
-              vmax = fmaxf(fmaxf(v4.x, v4.y), fmaxf(v4.z, v4.w));
-            }
           }
           if (tail) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) seen[c] = row_ok ? seen32(p, r, t, qi, key0 + 32 * c) : kFull;
             if (C::KIND != kInt8 && r.n > 1) {
-              const int* w = bars->wild[slot];
-              if (w[0] | w[1] | w[2] | w[3]) so.note_wild(seen, slot, x * kTile + wrow);
+              int any = 0;
+#pragma unroll
+              for (int i = 0; i < C::kLoadWarps; ++i) any |= bars->wild[slot][i];
+              if (any) so.note_wild(seen, slot, x * kTile + wrow);
             }
             so.template tile<true>(seen, ks, vs, vmax, first);
           } else {
@@ -789,38 +1066,41 @@ __global__ void __launch_bounds__(kThreadsTc, 1) attend_tc_kernel(const __grid_c
       const bool whole = pc.tile0 == 0 && pc.nt == pc.w.tiles;
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + (pc.tile0 == 0 ? 1 : 0)) << p.rows_log2;
       const bool two = nq == 1 && pc.nt > 1;  // both streams hold sums of these rows
-      const int streams = nq == 1 ? (two ? 2 : 1) : 0;
+      kv += 2 * pc.nt;
+      t0 += pc.nt;
+      more = pc.next(p);
+      if (more) {
+        me = row_of(pc);
+        if (me.ok) {  // the next queries come to L2 while these outputs go out
+#pragma unroll
+          for (int i = 0; i < D * 2; i += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(me.q + i));
+        }
+      }
       if (nq == 1) {
-        for (int y = 0; y < streams && ok; ++y) ok = wait(&bars->o_done[y], op[y]++ & 1, abort);
+        ok = wait(&bars->o_done[0], op0++ & 1, abort);
+        if (two && ok) ok = wait(&bars->o_done[1], op1++ & 1, abort);
       } else {
-        ok = wait(&bars->o_done[x], op[x]++ & 1, abort);
+        ok = wait(&bars->o_done[x], op0++ & 1, abort);
       }
       if (!ok) break;
       tc_fence_after();
       float f0, f1 = 0.0f, m = so.m, l = so.l;
       int c0 = 0, c1 = D / 32;
       uint32_t o0 = so.tmem_o, o1 = so.tmem_o;
-      bool wild = so.wild;
+      bool noted0 = so.wild, noted1 = false;
       const float vscale = C::kSmall ? (C::TOKEN ? so.vref : p.c.v_scale[h * p.c.v_scale_stride[2]]) : 1.0f;
       f0 = vscale;
       if (nq == 1) {
         // each stream's warps write half of the dimensions, joining both streams' sums
-        ml[x * kTile + wrow] = make_float2(so.m, so.l);
-        float* vr = reinterpret_cast<float*>(mem + C::kOffQ);  // every score is done: the queries' place is free
-        if (C::TOKEN) vr[x * kTile + wrow] = so.vref;
-        if (C::KIND != kInt8) reinterpret_cast<int*>(vr)[2 * kTile + x * kTile + wrow] = so.wild;
+        ml[x * kTile + wrow] = make_float4(so.m, so.l, so.vref, so.wild ? 1.0f : 0.0f);
         ok = meet();
         if (!ok) break;
-        const float2 a = ml[wrow], b = two ? ml[kTile + wrow] : make_float2(-INFINITY, 0.0f);
+        const float4 a = ml[wrow], b = two ? ml[kTile + wrow] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
         m = fmaxf(a.x, b.x);
         const float wa = a.x == -INFINITY ? 1.0f : exp2_fast(a.x - m), wb = b.x == -INFINITY ? 1.0f : exp2_fast(b.x - m);
         l = a.y * wa + b.y * wb;
-        const float va = C::TOKEN ? vr[wrow] : vscale, vb = C::TOKEN ? (two ? vr[kTile + wrow] : 0.0f) : vscale;
-        f0 = wa * va, f1 = wb * vb;
-        if (C::KIND != kInt8) {
-          const int* wl = reinterpret_cast<const int*>(vr) + 2 * kTile;
-          wild = wl[wrow] || (two && wl[kTile + wrow]);
-        }
+        f0 = wa * (C::TOKEN ? a.z : vscale), f1 = wb * (C::TOKEN ? b.z : vscale);
+        noted0 = a.w != 0.0f, noted1 = b.w != 0.0f;
         o0 = tmem + lanes + 2 * kTile, o1 = o0 + D;
         c0 = x * (D / 64), c1 = c0 + D / 64;
       }
@@ -830,48 +1110,66 @@ __global__ void __launch_bounds__(kThreadsTc, 1) attend_tc_kernel(const __grid_c
       }
       const int at_row = (nq == 1 ? 0 : x * kTile) + wrow;
       if (warp_ok) {
-        for (int c = c0; c < c1; ++c) {
-          uint32_t a[32], b[32];
-          tmem_ld32(o0 + 32 * c, a);
-          if (two) tmem_ld32(o1 + 32 * c, b);
+        // Rows go out through the queries' place (every score is done): 128 bytes of each of the warp's rows at a time,
+        // so that a store fills whole lines
+        uint8_t* stage = mem + C::kOffQ + (nq == 1 ? 0 : x) * C::kSlot + (nq == 1 ? warp : warp & 3) * 4096;
+        uint8_t* mine = whole ? static_cast<uint8_t*>(p.out) + (t * p.o_tok + head * p.o_head) * 2
+                              : reinterpret_cast<uint8_t*>(p.part_o + (part + at_row) * D);
+        const unsigned rows_ok = __ballot_sync(kFull, row_ok);
+        const uint32_t* bits = reinterpret_cast<const uint32_t*>(mem + C::kOffRowWild);
+        uint8_t* line = stage + lane * 128;
+        auto take = [&](int c, float (&v)[16]) {  // dimensions 16 c .. 16 c + 15 of the thread's row
+          uint32_t a[16], b[16];
+          tmem_ld16(o0 + 16 * c, a);
+          if (two) tmem_ld16(o1 + 16 * c, b);
           tmem_ld_wait();
-          float v[32];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
+          for (int i = 0; i < 16; ++i) {
             v[i] = __uint_as_float(a[i]) * f0;
             if (two) v[i] += __uint_as_float(b[i]) * f1;
           }
-          if (C::KIND != kInt8 && wild) {
-            const uint32_t* bits = reinterpret_cast<const uint32_t*>(mem + C::kOffRowWild);
+          if (C::KIND != kInt8 && (noted0 || noted1)) {
             uint32_t plus = 0, minus = 0;
-            for (int y = nq == 1 ? 0 : x; y < (nq == 1 ? 2 : x + 1); ++y) {
-              const bool noted = nq == 1 ? reinterpret_cast<const int*>(mem + C::kOffQ)[2 * kTile + y * kTile + wrow] != 0 : true;
-              if (!noted || (y == 1 && nq == 1 && !two)) continue;
-              plus |= bits[(y * kTile + wrow) * 8 + c];
-              minus |= bits[(y * kTile + wrow) * 8 + 4 + c];
-            }
+            const uint32_t* n0 = bits + ((nq == 1 ? 0 : x * kTile) + wrow) * 8 + (c >> 1);
+            if (noted0) plus |= n0[0], minus |= n0[4];
+            if (noted1) plus |= n0[kTile * 8], minus |= n0[kTile * 8 + 4];
+            plus >>= 16 * (c & 1), minus >>= 16 * (c & 1);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
+            for (int i = 0; i < 16; ++i) {
               if ((plus >> i) & 1) v[i] += INFINITY;
               if ((minus >> i) & 1) v[i] -= INFINITY;
             }
           }
-          if (!row_ok) continue;
-          if (!whole) {
-            float4* to = reinterpret_cast<float4*>(p.part_o + (part + at_row) * D + 32 * c);
+        };
+        // a line is 64 dimensions of 16 bits or 32 sums (half a line of outputs where a stream's warps write 32 dimensions)
+        const int steps = whole ? min(4, 2 * (c1 - c0)) : 2;
+#pragma unroll 1
+        for (int c = 2 * c0; c < 2 * c1; c += steps) {
+#pragma unroll 1
+          for (int y = 0; y < steps; ++y) {
+            float v[16];
+            take(c + y, v);
+            if (whole) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) to[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-          } else {
-            uint4* to = reinterpret_cast<uint4*>(static_cast<uint8_t*>(p.out) + (t * p.o_tok + head * p.o_head) * 2 + 64 * c);
+              for (int i = 0; i < 2; ++i) {
+                uint32_t w[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              uint32_t w[4];
+                for (int z = 0; z < 4; ++z)
+                  w[z] = p.bf16 ? pack2<true>(v[8 * i + 2 * z], v[8 * i + 2 * z + 1]) : pack2<false>(v[8 * i + 2 * z], v[8 * i + 2 * z + 1]);
+                *reinterpret_cast<uint4*>(line + (((2 * y + i) ^ (lane & 7)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+              }
+            } else {
 #pragma unroll
-              for (int y = 0; y < 4; ++y)
-                w[y] = p.bf16 ? pack2<true>(v[8 * i + 2 * y], v[8 * i + 2 * y + 1]) : pack2<false>(v[8 * i + 2 * y], v[8 * i + 2 * y + 1]);
-              to[i] = make_uint4(w[0], w[1], w[2], w[3]);
+              for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(line + (((4 * y + i) ^ (lane & 7)) << 4)) =
+                    make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
             }
           }
+          uint8_t* to = mine + c * (whole ? 32 : 64);
+          if (whole && steps == 2)
+            put_lines<4>(stage, to, rows_ok, lane);
+          else
+            put_lines<8>(stage, to, rows_ok, lane);
         }
         if (row_ok && (nq == 2 || x == 0)) {
           if (!whole) {
@@ -887,15 +1185,13 @@ __global__ void __launch_bounds__(kThreadsTc, 1) attend_tc_kernel(const __grid_c
         ok = meet();
         if (!ok) break;
       }
-      kv += 2 * pc.nt;
-      t0 += pc.nt;
-    } while (pc.next(p));
+    } while (more);
   }
 
   tc_fence_before();
   __syncthreads();
   if (tid == 0 && *abort) atomicOr(&g_attn_error, 2);
-  if (warp == kWarpsTc - 1) {
+  if (warp == C::kWarps - 4) {
     tc_fence_after();
     tmem_dealloc(tmem, kTmemCols);
   }
@@ -905,7 +1201,7 @@ template <typename C>
 orError_t launch(Params& p, int nq, cudaStream_t st, int sms) {
   const void* fn = reinterpret_cast<const void*>(&attend_tc_kernel<C>);
   MCPU_CUDA_TRY(ensure_dynamic_smem(fn, C::smem(nq)), "tree_attention");
-  attend_tc_kernel<C><<<sms, kThreadsTc, C::smem(nq), st>>>(p, nq);
+  attend_tc_kernel<C><<<sms, C::kThreads, C::smem(nq), st>>>(p, nq);
   return from_cuda(cudaGetLastError(), "tree_attention launch");
 }
 
