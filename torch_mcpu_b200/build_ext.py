@@ -83,6 +83,43 @@ def build(verbose: bool = False) -> str:
     return SO
 
 
+# ---- Python functions of the attention path on CUDA tensors: a module of its
+# own, so that using them does not register the mcpu device
+OPS_SRC = os.path.join(SRC, "cuda", "attention_module.cpp")
+OPS_NAME = "torch_mcpu_b200_ops"
+OPS_SO = os.path.join(OUT, OPS_NAME + ".so")
+
+
+def ops_up_to_date() -> bool:
+    deps = [OPS_SRC, os.path.join(SRC, "attention_ops.h")] + glob.glob(os.path.join(ROOT, "include", "*.h"))
+    return os.path.exists(OPS_SO) and os.path.getmtime(OPS_SO) >= max(os.path.getmtime(f) for f in deps)
+
+
+def build_ops() -> str:
+    if ops_up_to_date():
+        return OPS_SO
+    import subprocess
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    _use_shared_libstdcxx_compiler()
+    os.makedirs(OUT, exist_ok=True)
+    cuda_inc = os.path.join(os.environ.get("CUDA_HOME", "/usr/local/cuda"), "include")
+    inc = [os.path.join(ROOT, "include"), SRC, cuda_inc, sysconfig.get_paths()["include"], *cpp_extension.include_paths()]
+    lib = os.path.join(os.path.dirname(torch.__file__), "lib")
+    tmp = f"{OPS_SO}.{os.getpid()}.tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{i}" for i in inc), OPS_SRC, "-o", tmp,
+           f"-L{lib}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building {OPS_NAME} failed:\n{r.stderr[-4000:]}")
+    os.replace(tmp, OPS_SO)
+    return OPS_SO
+
+
 CHECK_SRC = os.path.join(ROOT, "tests", "launch_api", "launch_check.cu")
 CHECK_NAME = "mcpu_launch_check"
 CHECK_SO = os.path.join(OUT, CHECK_NAME + ".so")
@@ -116,5 +153,6 @@ def build_launch_check(verbose: bool = False) -> str:
 
 if __name__ == "__main__":
     print(build(verbose="-v" in sys.argv))
+    print(build_ops())
     if "--launch-check" in sys.argv:
         print(build_launch_check(verbose="-v" in sys.argv))

@@ -27,16 +27,21 @@
 // exactly: the scales of the keys go onto the scores, those of the values onto
 // the probabilities.
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 
 #include "tree_attention.cuh"
 
+#ifndef MINSHARE
+#define MINSHARE 2
+#endif
 namespace mcpu {
 namespace attn {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kJoinThreads = 128;  // 16 rows a block
+constexpr int kRows = 16;  // rows of a tile: a matrix instruction's
+constexpr int kJoinThreads = 256;  // 32 rows a block
 
 // ---------------------------------------------------------------- instructions
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -88,21 +93,19 @@ __device__ __forceinline__ void mma_seen(float (&acc)[4], const uint32_t (&p)[4]
 }
 
 // ---------------------------------------------------------------- main kernel
-template <typename T, int KIND_, int D_, int MT_, int TN_, int STAGES_>
+template <typename T, int KIND_, int D_, int STAGES_>
 struct Cfg {
-  static constexpr int KIND = KIND_, D = D_, MT = MT_, TN = TN_, STAGES = STAGES_;
+  static constexpr int KIND = KIND_, D = D_, STAGES = STAGES_;
   static constexpr bool kSmall = KIND != kSame;
   static constexpr bool kBf16 = !kSmall && std::is_same<T, __nv_bfloat16>::value;  // type of the products
   static constexpr int kRow = D * (kSmall ? 1 : 2);                                // bytes of a key row
   static constexpr int kChunks = kRow / 16;
-  static constexpr int kTile = TN * kRow;
-  static constexpr int kScales = kSmall ? 2 * TN * 4 : 0;
-  static constexpr int kStage = 2 * kTile + kScales;
-  static constexpr int WM = MT / 16, WK = kWarps / WM;  // warps over rows and over keys
-  static constexpr int KW = TN / WK;                    // keys of a tile per warp
-  static constexpr int kScratch = WK > 1 ? kWarps * 16 * 32 * 4 : 0;  // joining the warps' sums, 32 dimensions a turn
-  static constexpr int kSmem = STAGES * kStage + kScratch + kWarps * 16 * 8 + 64;
-  static_assert(KW % 16 == 0, "a warp takes whole steps of 16 keys");
+  static constexpr int KW = kSmall ? 32 : 16;                                      // keys of a warp's step
+  static constexpr int TN = kWarps * KW;                                           // keys of a unit
+  static constexpr int kHalf = KW * kRow;                                          // keys, or values, of a step
+  static constexpr int kStage = 2 * kHalf + (kSmall ? 2 * KW * 4 : 0);
+  static constexpr int kScratch = kWarps * kRows * 32 * 4;  // joining the warps' sums, 32 dimensions a turn
+  static constexpr int kSmem = kWarps * STAGES * kStage + kScratch + kWarps * kRows * 16;
 };
 
 // Byte offset of 16-byte chunk c of a row: rows shifted against one another so
@@ -115,57 +118,62 @@ __device__ __forceinline__ uint32_t place(int row, int c) {
     return row * C::kRow + ((c ^ ((row >> 1) & 3)) << 4);
 }
 
+// A lane's key of a warp's step in the pages, found one step ahead of its copy.
+struct Place {
+  int id, slot;
+  bool valid;
+};
 template <typename C>
-__device__ __forceinline__ void load_tile(const Params& p, const Walk& w, uint32_t stage) {
-  constexpr int kRowsPerTurn = kThreads / C::kChunks;
-  const int tid = threadIdx.x;
-  const int c = tid % C::kChunks;
-  const int key0 = w.tile * C::TN;
-  const int h = w.item / row_tiles(p, w.r);
-  const int* table = p.table + w.b * p.table_stride;
-  constexpr int kSize = C::kSmall ? 1 : 2;
-  const uint8_t* kb = static_cast<const uint8_t*>(p.c.key) + (h * p.c.key_stride[2]) * kSize + c * 16;
-  const uint8_t* vb = static_cast<const uint8_t*>(p.c.value) + (h * p.c.value_stride[2]) * kSize + c * 16;
+__device__ __forceinline__ Place look(const Params& p, const Walk& w, int warp, int lane) {
+  Place at{0, 0, false};
+  const int key = w.tile * C::TN + warp * C::KW + lane;
+  if (lane < C::KW && key < w.r.len) {
+    const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
+    at.slot = key - page * p.c.block_size;
+    at.id = p.table[w.b * p.table_stride + page];
+    at.valid = true;
+  }
+  return at;
+}
+
+// Starts a warp's copies of its keys and values of a unit.
+template <typename C>
+__device__ __forceinline__ void copy_step(const Params& p, const Walk& w, const Place& at, uint32_t stage, int lane) {
+  constexpr int kPer = C::kSmall ? 16 : 8;  // values in 16 bytes
+  constexpr int kAtOnce = 32 / C::kChunks;  // rows a copy of the whole warp takes
+  const int h = w.item;                     // up to 16 rows: items are key / value heads
+  const int block = static_cast<int>(kv::checked_block(at.id, p.c.num_blocks, &g_attn_error));
+  // places in 16-byte units: 32 bits reach 64 GB, which the entry point makes sure of
+  const uint32_t ko = static_cast<uint32_t>(block) * static_cast<uint32_t>(p.c.key_stride[0] / kPer) +
+                      static_cast<uint32_t>(at.slot) * static_cast<uint32_t>(p.c.key_stride[1] / kPer);
+  const uint32_t vo = static_cast<uint32_t>(block) * static_cast<uint32_t>(p.c.value_stride[0] / kPer) +
+                      static_cast<uint32_t>(at.slot) * static_cast<uint32_t>(p.c.value_stride[1] / kPer);
+  const unsigned valid = __ballot_sync(kFull, at.valid);
+  const int c = lane % C::kChunks, r0 = lane / C::kChunks;
+  const uint4* kb = static_cast<const uint4*>(p.c.key) + (h * p.c.key_stride[2] / kPer + c);
+  const uint4* vb = static_cast<const uint4*>(p.c.value) + (h * p.c.value_stride[2] / kPer + c);
 #pragma unroll
-  for (int i = 0; i < C::TN / kRowsPerTurn; ++i) {
-    const int row = tid / C::kChunks + i * kRowsPerTurn;
-    const int key = key0 + row;
-    const bool valid = key < w.r.len;
-    long long ko = 0, vo = 0;
-    if (valid) {
-      const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
-      const int slot = key - page * p.c.block_size;
-      const long long id = kv::checked_block(table[page], p.c.num_blocks, &g_attn_error);
-      ko = (id * p.c.key_stride[0] + slot * p.c.key_stride[1]) * kSize;
-      vo = (id * p.c.value_stride[0] + slot * p.c.value_stride[1]) * kSize;
-    }
-    cp_async16(stage + place<C>(row, c), kb + ko, valid);
-    cp_async16(stage + C::kTile + place<C>(row, c), vb + vo, valid);
+  for (int i = 0; i < C::KW / kAtOnce; ++i) {
+    const int row = i * kAtOnce + r0;
+    const bool in = (valid >> row) & 1;
+    const uint32_t k = __shfl_sync(kFull, ko, row), v = __shfl_sync(kFull, vo, row);
+    cp_async16(stage + place<C>(row, c), kb + k, in);
+    cp_async16(stage + C::kHalf + place<C>(row, c), vb + v, in);
   }
   if constexpr (C::kSmall) {
-#pragma unroll
-    for (int i = tid; i < C::TN; i += kThreads) {
-      const int key = key0 + i;
-      const bool valid = key < w.r.len;
-      long long ko = 0, vo = 0;
-      if (valid) {
-        const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
-        const int slot = key - page * p.c.block_size;
-        const long long id = kv::checked_block(table[page], p.c.num_blocks, &g_attn_error);
-        ko = id * p.c.k_scale_stride[0] + slot * p.c.k_scale_stride[1] + h * p.c.k_scale_stride[2];
-        vo = id * p.c.v_scale_stride[0] + slot * p.c.v_scale_stride[1] + h * p.c.v_scale_stride[2];
-      }
-      cp_async4(stage + 2 * C::kTile + 4 * i, p.c.k_scale + ko, valid);
-      cp_async4(stage + 2 * C::kTile + 4 * (C::TN + i), p.c.v_scale + vo, valid);
-    }
+    const long long b = block, sl = at.slot;
+    cp_async4(stage + 2 * C::kHalf + 4 * lane,
+              p.c.k_scale + b * p.c.k_scale_stride[0] + sl * p.c.k_scale_stride[1] + h * p.c.k_scale_stride[2], at.valid);
+    cp_async4(stage + 2 * C::kHalf + 4 * (C::KW + lane),
+              p.c.v_scale + b * p.c.v_scale_stride[0] + sl * p.c.v_scale_stride[1] + h * p.c.v_scale_stride[2], at.valid);
   }
 }
 
-// Whether any of a warp's KW value rows holds an infinity or a NaN.
+// Whether any of a warp's value rows holds an infinity or a NaN.
 template <typename C>
-__device__ __forceinline__ bool any_wild(const uint8_t* values, int row0) {
-  bool wild = false;
-  const uint4* v = reinterpret_cast<const uint4*>(values + row0 * C::kRow);  // rows are whole, their order is no matter
+__device__ __forceinline__ bool any_wild(const uint8_t* values) {
+  uint32_t wild = 0;
+  const uint4* v = reinterpret_cast<const uint4*>(values);  // rows are whole, their order is no matter
 #pragma unroll 4
   for (int i = threadIdx.x & 31; i < C::KW * C::kChunks; i += 32) {
     const uint4 u = v[i];
@@ -173,65 +181,64 @@ __device__ __forceinline__ bool any_wild(const uint8_t* values, int row0) {
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       if constexpr (C::KIND == kE4M3)
-        wild = wild || ((((w[x] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u) != 0);
+        wild |= ((w[x] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
       else if constexpr (C::kBf16)
-        wild = wild || __vcmpeq2(w[x] & 0x7F807F80u, 0x7F807F80u) != 0;
+        wild |= __vcmpeq2(w[x] & 0x7F807F80u, 0x7F807F80u);
       else
-        wild = wild || __vcmpeq2(w[x] & 0x7C007C00u, 0x7C007C00u) != 0;
+        wild |= __vcmpeq2(w[x] & 0x7C007C00u, 0x7C007C00u);
     }
   }
-  return __any_sync(kFull, wild);
-}
-
-// Whether query i (token t of request r) sees key j < r.len.
-__device__ __forceinline__ bool sees(const Params& p, const Request& r, int t, int i, int key) {
-  const int d = key - (r.len - r.n);
-  if (key >= r.len) return false;
-  if (d < 0) return true;
-  if (p.mask == nullptr) return d <= i;
-  return (p.mask[t * p.mask_stride + (d >> 6)] >> (d & 63)) & 1;
+  return __any_sync(kFull, wild != 0);
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ Params p) {
-  constexpr int D = C::D, MT = C::MT, TN = C::TN, KW = C::KW, KIND = C::KIND;
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ Params p) {
+  constexpr int D = C::D, KW = C::KW, KIND = C::KIND;
   constexpr int kNT = KW / 8;   // 8-key tiles of the scores
   constexpr int kDT = D / 8;    // 8-dimension tiles of the output
   extern __shared__ __align__(128) uint8_t smem[];
-  const uint32_t stages = smem_u32(smem);
-  float* scratch = reinterpret_cast<float*>(smem + C::STAGES * C::kStage);
-  float2* warp_ml = reinterpret_cast<float2*>(smem + C::STAGES * C::kStage + C::kScratch);
   __shared__ int red[kWarps + 2];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, j4 = lane & 3;
-  const int wm = warp / C::WK, wk = warp % C::WK;
+  uint8_t* mine = smem + warp * (C::STAGES * C::kStage);  // the warp's own stages
+  const uint32_t stages = smem_u32(mine);
+  float* scratch = reinterpret_cast<float*>(smem + kWarps * C::STAGES * C::kStage);
+  float4* warp_ml = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(scratch) + C::kScratch);
 
   // the joining kernel may start; it waits for this one to end before it reads
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  clear_idle_requests<kThreads>(p, D);
-
   int total, unit, b0, before;
   int share = 0;
   locate<kThreads>(
-      p, [&](int tot) { share = share_of(p, tot, gridDim.x); return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll)); }, red,
-      total, unit, b0, before);
+      p,
+      [&](int tot) {
+        share = share_of(p, tot, gridDim.x);
+        return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
+      },
+      red, total, unit, b0, before);
+  clear_idle_requests<kThreads>(p, D);
   if (unit >= total) return;
   const int end = min(unit + share, total);
 
+  // every warp walks the units by itself: its copies, its steps, no barrier until an item ends
   Walk cur, ahead;
   cur.seek(p, b0, unit - before);
   ahead = cur;
   int loaded = unit;
-#pragma unroll
-  for (int s = 0; s < C::STAGES - 1; ++s) {
+  Place next = look<C>(p, ahead, warp, lane);
+  auto load = [&](int s) {
     if (loaded < end) {
-      load_tile<C>(p, ahead, stages + s * C::kStage);
-      ahead.next(p);
-      ++loaded;
+      copy_step<C>(p, ahead, next, stages + s * C::kStage, lane);
+      if (++loaded < end) {
+        ahead.next(p);
+        next = look<C>(p, ahead, warp, lane);
+      }
     }
     cp_commit();
-  }
+  };
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) load(s);
 
   uint32_t qf[D / 16][4];
   float qscale[2];
@@ -245,27 +252,22 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 
   for (int u = unit; u < end; ++u) {
     cp_wait<C::STAGES - 2>();
-    __syncthreads();
-    if (loaded < end) {
+    __syncwarp();
+    {
       int s = stage + C::STAGES - 1;
       if (s >= C::STAGES) s -= C::STAGES;
-      load_tile<C>(p, ahead, stages + s * C::kStage);
-      ahead.next(p);
-      ++loaded;
+      load(s);
     }
-    cp_commit();
 
     if (fresh) {
       fresh = false;
       first_tile = cur.tile;
-      const int rts = row_tiles(p, cur.r);
-      const int h = cur.item / rts, rt = cur.item - h * rts;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = rt * MT + wm * 16 + g + 8 * e;
+        const int row = g + 8 * e;
         row_ok[e] = row < cur.r.n * p.group;
         qi[e] = row / p.group;
-        head[e] = h * p.group + row - qi[e] * p.group;
+        head[e] = cur.item * p.group + row - qi[e] * p.group;
         tok[e] = cur.r.first + qi[e];
         m[e] = -INFINITY;
         l[e] = 0.0f;
@@ -276,8 +278,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
           uint32_t lo = 0, hi = 0;
           if (row_ok[e]) {
             if constexpr (C::kSmall) {  // dimensions 4j..4j+3, the order the 8-bit keys come in
-              const uint32_t* src = reinterpret_cast<const uint32_t*>(q + kk * 16 + 4 * j4);
-              lo = src[0], hi = src[1];
+              const uint2 q4 = *reinterpret_cast<const uint2*>(q + kk * 16 + 4 * j4);
+              lo = q4.x, hi = q4.y;
             } else {
               lo = *reinterpret_cast<const uint32_t*>(q + kk * 16 + 2 * j4);
               hi = *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8 + 2 * j4);
@@ -319,10 +321,10 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
         for (int x = 0; x < 4; ++x) acc[i][x] = 0.0f;
     }
 
-    // ---- scores of this warp's 16 rows and KW keys
-    const uint32_t ks = stages + stage * C::kStage, vs = ks + C::kTile;
-    const float* scale_k = reinterpret_cast<const float*>(smem + stage * C::kStage + 2 * C::kTile);
-    const float* scale_v = scale_k + TN;
+    // ---- scores of the 16 rows and the warp's KW keys
+    const uint32_t ks = stages + stage * C::kStage, vs = ks + C::kHalf;
+    const float* scale_k = reinterpret_cast<const float*>(mine + stage * C::kStage + 2 * C::kHalf);
+    const float* scale_v = scale_k + KW;
     float s[kNT][4];
 #pragma unroll
     for (int i = 0; i < kNT; ++i)
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 #pragma unroll
         for (int n = 0; n < kNT; n += 2) {
           uint32_t b[4];
-          ldsm4(b, ks + place<C>(wk * KW + n * 8 + (mi >> 1) * 8 + mr, kk * 2 + (mi & 1)));
+          ldsm4(b, ks + place<C>(n * 8 + (mi >> 1) * 8 + mr, kk * 2 + (mi & 1)));
           mma<C::kBf16>(s[n], qf[kk], b[0], b[1]);
           mma<C::kBf16>(s[n + 1], qf[kk], b[2], b[3]);
         }
@@ -345,7 +347,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 #pragma unroll
         for (int n = 0; n < kNT; n += 2) {
           uint32_t b[4];
-          ldsm4(b, ks + place<C>(wk * KW + n * 8 + (mi >> 1) * 8 + mr, kk + (mi & 1)));
+          ldsm4(b, ks + place<C>(n * 8 + (mi >> 1) * 8 + mr, kk + (mi & 1)));
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const uint32_t w = KIND == kInt8 ? b[x] ^ 0x80808080u : b[x];
@@ -355,28 +357,28 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
     }
 
     // ---- scale, mask, running maximum
-    const int key0 = cur.tile * TN + wk * KW;
-    const bool tail = (cur.tile + 1) * TN > cur.r.len - cur.r.n;
+    const int key0 = cur.tile * C::TN + warp * KW;
+    const bool tail = key0 + KW > cur.r.len - cur.r.n;
+    uint32_t view[2] = {kFull, kFull};  // the keys a row sees
+    if (tail) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        view[e] = seen32(p, cur.r, row_ok[e] ? tok[e] : cur.r.first, row_ok[e] ? qi[e] : 0, key0) >> (2 * j4);
+    }
     float top[2] = {-INFINITY, -INFINITY};
     float vmax = 0.0f;
-    uint32_t seen = 0;  // bit 4 n + x: tail tiles only
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
       float2 sk = make_float2(1.0f, 1.0f);
       if constexpr (C::kSmall) {
-        sk = *reinterpret_cast<const float2*>(scale_k + wk * KW + n * 8 + 2 * j4);
-        const float2 sv = *reinterpret_cast<const float2*>(scale_v + wk * KW + n * 8 + 2 * j4);
+        sk = *reinterpret_cast<const float2*>(scale_k + n * 8 + 2 * j4);
+        const float2 sv = *reinterpret_cast<const float2*>(scale_v + n * 8 + 2 * j4);
         vmax = fmaxf(vmax, fmaxf(sv.x < 1e30f ? sv.x : 0.0f, sv.y < 1e30f ? sv.y : 0.0f));
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         s[n][x] *= qscale[x >> 1] * ((x & 1) ? sk.y : sk.x);
-        if (tail) {
-          if (sees(p, cur.r, row_ok[x >> 1] ? tok[x >> 1] : cur.r.first, qi[x >> 1], key0 + n * 8 + 2 * j4 + (x & 1)))
-            seen |= 1u << (4 * n + x);
-          else
-            s[n][x] = -INFINITY;
-        }
+        if (tail && !((view[x >> 1] >> (8 * n + (x & 1))) & 1)) s[n][x] = -INFINITY;
         top[x >> 1] = fmaxf(top[x >> 1], s[n][x]);
       }
     }
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
         l[x >> 1] += pr[x];
       }
       if constexpr (C::kSmall) {
-        const float2 sv = *reinterpret_cast<const float2*>(scale_v + wk * KW + n * 8 + 2 * j4);
+        const float2 sv = *reinterpret_cast<const float2*>(scale_v + n * 8 + 2 * j4);
         const float f[2] = {sv.x * inv_vref, sv.y * inv_vref};
 #pragma unroll
         for (int x = 0; x < 4; ++x) pr[x] = pr[x] == 0.0f && tail ? 0.0f : pr[x] * f[x & 1];
@@ -432,23 +434,23 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
     }
 
     // ---- probabilities times values
-    if (KIND != kInt8 && tail && cur.r.n > 1 && any_wild<C>(smem + stage * C::kStage + C::kTile, wk * KW)) {
+    if (KIND != kInt8 && tail && cur.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf)) {
 #pragma unroll
       for (int kk = 0; kk < kNT / 2; ++kk) {
-        const int row = wk * KW + kk * 16 + (mi & 1) * 8 + mr;
-        uint32_t view[4];
+        const int row = kk * 16 + (mi & 1) * 8 + mr;
+        uint32_t ones[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const uint32_t two = seen >> (8 * kk + 4 * (x >> 1) + 2 * (x & 1));
-          view[x] = ((two & 1u) | (two & 2u) << 15) * (C::kBf16 ? 0x3F80u : 0x3C00u);
+          const uint32_t two = view[x & 1] >> (16 * kk + 8 * (x >> 1));
+          ones[x] = ((two & 1u) | (two & 2u) << 15) * (C::kBf16 ? 0x3F80u : 0x3C00u);
         }
         if constexpr (!C::kSmall) {
 #pragma unroll
           for (int n = 0; n < kDT; n += 2) {
             uint32_t b[4];
             ldsm4t(b, vs + place<C>(row, n + (mi >> 1)));
-            mma_seen<C::kBf16>(acc[n], pf[kk], view, b[0], b[1]);
-            mma_seen<C::kBf16>(acc[n + 1], pf[kk], view, b[2], b[3]);
+            mma_seen<C::kBf16>(acc[n], pf[kk], ones, b[0], b[1]);
+            mma_seen<C::kBf16>(acc[n + 1], pf[kk], ones, b[2], b[3]);
           }
         } else {
 #pragma unroll
@@ -457,8 +459,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
             ldsm4t(b, vs + place<C>(row, n + (mi >> 1)));
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              mma_seen<false>(acc[2 * (n + x)], pf[kk], view, widen<KIND, 0, 2>(b[2 * x]), widen<KIND, 0, 2>(b[2 * x + 1]));
-              mma_seen<false>(acc[2 * (n + x) + 1], pf[kk], view, widen<KIND, 1, 3>(b[2 * x]), widen<KIND, 1, 3>(b[2 * x + 1]));
+              mma_seen<false>(acc[2 * (n + x)], pf[kk], ones, widen<KIND, 0, 2>(b[2 * x]), widen<KIND, 0, 2>(b[2 * x + 1]));
+              mma_seen<false>(acc[2 * (n + x) + 1], pf[kk], ones, widen<KIND, 1, 3>(b[2 * x]), widen<KIND, 1, 3>(b[2 * x + 1]));
             }
           }
         }
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
     } else
 #pragma unroll
     for (int kk = 0; kk < kNT / 2; ++kk) {
-      const int row = wk * KW + kk * 16 + (mi & 1) * 8 + mr;
+      const int row = kk * 16 + (mi & 1) * 8 + mr;
       if constexpr (!C::kSmall) {
 #pragma unroll
         for (int n = 0; n < kDT; n += 2) {
@@ -492,6 +494,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
         }
       }
     }
+    __syncwarp();  // the stage is read before the next copies into it
 
     // ---- end of the item, or of this block's run: join the warps, write
     const bool last_tile = cur.tile + 1 == cur.tiles;
@@ -503,39 +506,31 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
       for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(kFull, l[e], 1);
         l[e] += __shfl_xor_sync(kFull, l[e], 2);
+        if (j4 == 0) warp_ml[warp * kRows + g + 8 * e] = make_float4(m[e], l[e], 0.0f, 0.0f);
       }
-      float f[2] = {1.0f, 1.0f};
-      if constexpr (C::WK > 1) {
-        if (j4 == 0) {
-          warp_ml[warp * 16 + g] = make_float2(m[0], l[0]);
-          warp_ml[warp * 16 + g + 8] = make_float2(m[1], l[1]);
-        }
-        __syncthreads();
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float mm = -INFINITY, ll = 0.0f;
-#pragma unroll
-          for (int w = 0; w < C::WK; ++w) mm = fmaxf(mm, warp_ml[(wm * C::WK + w) * 16 + g + 8 * e].x);
-#pragma unroll
-          for (int w = 0; w < C::WK; ++w) {
-            const float2 o = warp_ml[(wm * C::WK + w) * 16 + g + 8 * e];
-            ll += o.x == -INFINITY ? o.y : exp2_fast(o.x - mm) * o.y;
-          }
-          f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
-          m[e] = mm;
-          l[e] = ll;
-        }
-      }
+      __syncthreads();
+      float f[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
+        float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, warp_ml[w * kRows + g + 8 * e].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 o = warp_ml[w * kRows + g + 8 * e];
+          ll += o.x == -INFINITY ? o.y : exp2_fast(o.x - mm) * o.y;
+        }
+        f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
+        m[e] = mm;
+        l[e] = ll;
         if (C::kSmall) f[e] *= vref;
-        if (whole) f[e] = l[e] == 0.0f ? 0.0f : f[e] / l[e];
+        if (whole) f[e] = ll == 0.0f ? 0.0f : f[e] / ll;
       }
-      const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * MT;
-      if (wk == 0 && j4 == 0) {
+      const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * kRows;
+      if (warp == 0 && j4 == 0) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = wm * 16 + g + 8 * e;
+          const int row = g + 8 * e;
           if (!whole) {
             p.part_ml[(part + row) * 2] = m[e];
             p.part_ml[(part + row) * 2 + 1] = l[e];
@@ -545,91 +540,62 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
           }
         }
       }
-      if constexpr (C::WK == 1) {
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int row = wm * 16 + g + 8 * e;
-          T* o = static_cast<T*>(p.out) + tok[e] * p.o_tok + head[e] * p.o_head;
-          float* po = p.part_o + (part + row) * D;
+      for (int d0 = 0; d0 < D; d0 += 32) {
+        if (d0 > 0) __syncthreads();
 #pragma unroll
-          for (int i = 0; i < kDT; i += 2) {
-            const float a = acc[i][2 * e] * f[e], b = acc[i][2 * e + 1] * f[e];
-            const float c = acc[i + 1][2 * e] * f[e], d = acc[i + 1][2 * e + 1] * f[e];
-            // 16-bit caches: dimensions 8i + 2j, +1 of each tile; 8-bit ones: 16 dimensions over two tiles
+        for (int i = 0; i < 4; i += 2) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float* to = scratch + (warp * kRows + g + 8 * e) * 32 + i * 8;
+            const float(&x)[4] = acc[d0 / 8 + i];
+            const float(&y)[4] = acc[d0 / 8 + i + 1];
             if constexpr (C::kSmall) {
-              if (!whole)
-                *reinterpret_cast<float4*>(po + i * 8 + 4 * j4) = make_float4(a, c, b, d);
-              else if (row_ok[e])
-                *reinterpret_cast<uint2*>(o + i * 8 + 4 * j4) =
-                    make_uint2(pack2<std::is_same<T, __nv_bfloat16>::value>(a, c),
-                               pack2<std::is_same<T, __nv_bfloat16>::value>(b, d));
+              *reinterpret_cast<float4*>(to + 4 * j4) =
+                  make_float4(x[2 * e] * f[e], y[2 * e] * f[e], x[2 * e + 1] * f[e], y[2 * e + 1] * f[e]);
             } else {
-              if (!whole) {
-                *reinterpret_cast<float2*>(po + i * 8 + 2 * j4) = make_float2(a, b);
-                *reinterpret_cast<float2*>(po + i * 8 + 8 + 2 * j4) = make_float2(c, d);
-              } else if (row_ok[e]) {
-                *reinterpret_cast<uint32_t*>(o + i * 8 + 2 * j4) = pack2<C::kBf16>(a, b);
-                *reinterpret_cast<uint32_t*>(o + i * 8 + 8 + 2 * j4) = pack2<C::kBf16>(c, d);
-              }
+              *reinterpret_cast<float2*>(to + 2 * j4) = make_float2(x[2 * e] * f[e], x[2 * e + 1] * f[e]);
+              *reinterpret_cast<float2*>(to + 8 + 2 * j4) = make_float2(y[2 * e] * f[e], y[2 * e + 1] * f[e]);
             }
           }
         }
-      } else {
-        const int rts = row_tiles(p, cur.r);
-        const int h = cur.item / rts, rt = cur.item - h * rts;
+        __syncthreads();
+        const int row = tid >> 3, d = (tid & 7) * 4;  // 4 dimensions of a row each
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-        for (int d0 = 0; d0 < D; d0 += 32) {
-          __syncthreads();
-#pragma unroll
-          for (int i = 0; i < 4; i += 2) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float* to = scratch + (warp * 16 + g + 8 * e) * 32 + i * 8;
-              const float(&x)[4] = acc[d0 / 8 + i];
-              const float(&y)[4] = acc[d0 / 8 + i + 1];
-              if constexpr (C::kSmall) {
-                *reinterpret_cast<float4*>(to + 4 * j4) =
-                    make_float4(x[2 * e] * f[e], y[2 * e] * f[e], x[2 * e + 1] * f[e], y[2 * e + 1] * f[e]);
-              } else {
-                *reinterpret_cast<float2*>(to + 2 * j4) = make_float2(x[2 * e] * f[e], x[2 * e + 1] * f[e]);
-                *reinterpret_cast<float2*>(to + 8 + 2 * j4) = make_float2(y[2 * e] * f[e], y[2 * e + 1] * f[e]);
-              }
-            }
-          }
-          __syncthreads();
-          for (int i = tid; i < MT * 8; i += kThreads) {  // 4 dimensions of a row each
-            const int row = i >> 3, d = (i & 7) * 4;
-            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < C::WK; ++w) {
-              const float4 v =
-                  *reinterpret_cast<const float4*>(scratch + (((row >> 4) * C::WK + w) * 16 + (row & 15)) * 32 + d);
-              sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
-            }
-            const int r = rt * MT + row;
-            if (!whole) {
-              *reinterpret_cast<float4*>(p.part_o + (part + row) * D + d0 + d) = sum;
-            } else if (r < cur.r.n * p.group) {
-              const int i2 = r / p.group;
-              T* o = static_cast<T*>(p.out) + (cur.r.first + i2) * p.o_tok + (h * p.group + r - i2 * p.group) * p.o_head;
-              constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
-              *reinterpret_cast<uint2*>(o + d0 + d) = make_uint2(pack2<kOutBf16>(sum.x, sum.y), pack2<kOutBf16>(sum.z, sum.w));
-            }
-          }
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(scratch + (w * kRows + row) * 32 + d);
+          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        if (!whole) {
+          *reinterpret_cast<float4*>(p.part_o + (part + row) * D + d0 + d) = sum;
+        } else if (row < cur.r.n * p.group) {
+          const int i2 = row / p.group;
+          T* o = static_cast<T*>(p.out) + (cur.r.first + i2) * p.o_tok + (cur.item * p.group + row - i2 * p.group) * p.o_head;
+          constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
+          *reinterpret_cast<uint2*>(o + d0 + d) = make_uint2(pack2<kOutBf16>(sum.x, sum.y), pack2<kOutBf16>(sum.z, sum.w));
         }
       }
+      __syncthreads();
     }
     cur.next(p);
     if (++stage == C::STAGES) stage = 0;
   }
+  cp_wait<0>();
 }
 
 // ---------------------------------------------------------------- joining kernel
 // Block c joins the one row tile that begins in the main kernel's block c and
-// goes on behind it: its parts lie in slot 1 of c and slot 0 of the next blocks.
+// goes on behind it: its parts lie in slot 1 of c and slot 0 of the next
+// blocks.  A block takes 32 of its rows, four to a warp; where there are fewer
+// rows, several warps share the parts of four and join theirs at the end, so
+// that a long sequence with few rows is not a chain of loads.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p) {
-  __shared__ int red[kJoinThreads / 32 + 2];
+  constexpr int kJoinWarps = kJoinThreads / 32;
+  __shared__ int red[kJoinWarps + 2];
+  __shared__ float4 sums[kJoinWarps][4][D / 4];
+  __shared__ float2 sums_ml[kJoinWarps][4];
   const int grid = gridDim.x, c = blockIdx.x, rows = 1 << p.rows_log2;
   int total, unit, b, before, share = 0;
   locate<kJoinThreads>(
@@ -651,44 +617,68 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   const int parts = to / share - c + 1;
   const int rts = row_tiles(p, r);
   const int h = item / rts, rt = item - h * rts;
-  // D / 4 lanes hold a row, 4 dimensions each; a warp takes kAtOnce rows together so that their parts' loads overlap
+  const int first = rt * rows + blockIdx.y * 32, left = min(rows - static_cast<int>(blockIdx.y) * 32, r.n * p.group - first);
+  if (left <= 0) return;
+  int groups = 1;  // of four rows, a power of two up to the block's warps
+  while (groups * 4 < left && groups < kJoinWarps) groups *= 2;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int mine = warp % groups, k0 = warp / groups, step = kJoinWarps / groups;
+  // D / 4 lanes hold a row, 4 dimensions each; loads of four rows and two parts at a time overlap
   constexpr int kLanes = D / 4, kPerWarp = 32 / kLanes, kAtOnce = 4 / kPerWarp;
-  const int d = (threadIdx.x % kLanes) * 4;
-  const int row0 = (blockIdx.y * (kJoinThreads / 32) + threadIdx.x / 32) * 4 + (threadIdx.x % 32) / kLanes;
+  const int d = lane % kLanes, row0 = mine * 4 + lane / kLanes;
   float m[kAtOnce], l[kAtOnce];
   float4 o[kAtOnce];
 #pragma unroll
   for (int i = 0; i < kAtOnce; ++i) m[i] = -INFINITY, l[i] = 0.0f, o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (rt * rows + row0 - (threadIdx.x % 32) / kLanes >= r.n * p.group) return;
-  for (int k = 0; k < parts; ++k) {
-    float2 ml[kAtOnce];
-    float4 v[kAtOnce];
+  auto add = [](float& m0, float& l0, float4& o0, float2 ml, const float4& v) {
+    const float now = fmaxf(m0, ml.x);
+    const float a = m0 == -INFINITY ? 1.0f : exp2_fast(m0 - now);  // nothing yet: sums of 0 (or NaN)
+    const float w = ml.x == -INFINITY ? 1.0f : exp2_fast(ml.x - now);
+    l0 = l0 * a + ml.y * w;
+    o0.x = o0.x * a + v.x * w, o0.y = o0.y * a + v.y * w, o0.z = o0.z * a + v.z * w, o0.w = o0.w * a + v.w * w;
+    m0 = now;
+  };
+  for (int k = k0; k < parts; k += 2 * step) {
+    float2 ml[2][kAtOnce];
+    float4 v[2][kAtOnce];
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int kk = k + y * step, row = row0 + i * kPerWarp;
+        const bool in = row < left && kk < parts;
+        const long long at = ((static_cast<long long>(c) + kk) * 2 + (kk == 0 ? 1 : 0)) * rows + blockIdx.y * 32 + row;
+        ml[y][i] = in ? *reinterpret_cast<const float2*>(p.part_ml + at * 2) : make_float2(-INFINITY, 0.0f);
+        v[y][i] = in ? reinterpret_cast<const float4*>(p.part_o + at * D)[d] : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) add(m[i], l[i], o[i], ml[y][i], v[y][i]);
+  }
+  if (step > 1) {  // the warps that shared the rows, in the order of the first parts they took
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const long long at = ((static_cast<long long>(c) + k) * 2 + (k == 0 ? 1 : 0)) * rows + row0 + i * kPerWarp;
-      const bool in = rt * rows + row0 + i * kPerWarp < r.n * p.group;
-      ml[i] = in ? *reinterpret_cast<const float2*>(p.part_ml + at * 2) : make_float2(-INFINITY, 0.0f);
-      v[i] = in ? *reinterpret_cast<const float4*>(p.part_o + at * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+      sums[warp][lane / kLanes + i * kPerWarp][d] = o[i];
+      if (d == 0) sums_ml[warp][lane / kLanes + i * kPerWarp] = make_float2(m[i], l[i]);
     }
+    __syncthreads();
+    if (k0 > 0) return;
+    for (int w = 1; w < step; ++w)
 #pragma unroll
-    for (int i = 0; i < kAtOnce; ++i) {
-      const float now = fmaxf(m[i], ml[i].x);
-      const float a = m[i] == -INFINITY ? 1.0f : exp2_fast(m[i] - now);  // nothing yet: sums of 0 (or NaN)
-      const float w = ml[i].x == -INFINITY ? 1.0f : exp2_fast(ml[i].x - now);
-      l[i] = l[i] * a + ml[i].y * w;
-      o[i].x = o[i].x * a + v[i].x * w, o[i].y = o[i].y * a + v[i].y * w;
-      o[i].z = o[i].z * a + v[i].z * w, o[i].w = o[i].w * a + v[i].w * w;
-      m[i] = now;
-    }
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int y = lane / kLanes + i * kPerWarp;
+        add(m[i], l[i], o[i], sums_ml[mine + w * groups][y], sums[mine + w * groups][y][d]);
+      }
   }
 #pragma unroll
   for (int i = 0; i < kAtOnce; ++i) {
-    const int rr = rt * rows + row0 + i * kPerWarp;
-    if (rr >= r.n * p.group) break;
+    if (row0 + i * kPerWarp >= left) break;
+    const int rr = first + row0 + i * kPerWarp;
     const float f = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
     const int q = rr / p.group, head = h * p.group + rr - q * p.group;
     const long long t = r.first + q;
-    T* out = static_cast<T*>(p.out) + t * p.o_tok + head * p.o_head + d;
+    T* out = static_cast<T*>(p.out) + t * p.o_tok + head * p.o_head + 4 * d;
     constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
     *reinterpret_cast<uint2*>(out) =
         make_uint2(pack2<kOutBf16>(o[i].x * f, o[i].y * f), pack2<kOutBf16>(o[i].z * f, o[i].w * f));
@@ -710,11 +700,10 @@ orError_t device(Device* d) {
 }
 
 constexpr int kMaxResident = 4;  // blocks per SM the workspace is sized for
-constexpr int kFewRows = 16;     // rows per key / value head that take the kernel above
 
 // Rows of partial sums a call may leave: two parts for every block.
 unsigned long long part_rows(int sms, long long rows) {
-  if (rows <= kFewRows) return 2ull * kMaxResident * sms * 16;
+  if (rows <= kRows) return 2ull * kMaxResident * sms * kRows;
   return 2ull * sms * (rows <= 128 ? 128 : 256);
 }
 
@@ -722,22 +711,28 @@ template <typename T, typename C>
 orError_t launch(Params& p, cudaStream_t st, int sms, int* grid) {
   const void* fn = reinterpret_cast<const void*>(&attend_kernel<T, C>);
   MCPU_CUDA_TRY(ensure_dynamic_smem(fn, C::kSmem), "tree_attention");
-  int resident = 0;
-  MCPU_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, attend_kernel<T, C>, kThreads, C::kSmem),
-                "tree_attention");
-  *grid = std::max(1, std::min(resident, kMaxResident)) * sms;
-  p.rows_log2 = C::MT == 16 ? 4 : C::MT == 32 ? 5 : 6;
+  static std::atomic<int> known{0};  // blocks per SM: a property of the kernel, asked once
+  int resident = known.load(std::memory_order_relaxed);
+  if (resident == 0) {
+    MCPU_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, attend_kernel<T, C>, kThreads, C::kSmem),
+                  "tree_attention");
+    resident = std::max(1, std::min(resident, kMaxResident));
+    known.store(resident, std::memory_order_relaxed);
+  }
+  *grid = resident * sms;
+  p.rows_log2 = 4;
   p.keys_log2 = C::TN == 64 ? 6 : 7;
-  p.min_share = 1;
+  p.min_share = MINSHARE;
   attend_kernel<T, C><<<*grid, kThreads, C::kSmem, st>>>(p);
   return from_cuda(cudaGetLastError(), "tree_attention launch");
 }
 
 template <typename T, int D>
 orError_t launch_few(Params& p, int dtype, cudaStream_t st, int sms, int* grid) {
-  if (p.c.dtype == dtype) return launch<T, Cfg<T, kSame, D, 16, 64, 3>>(p, st, sms, grid);
-  if (p.c.dtype == MCPU_INT8) return launch<T, Cfg<T, kInt8, D, 16, 128, 3>>(p, st, sms, grid);
-  return launch<T, Cfg<T, kE4M3, D, 16, 128, 3>>(p, st, sms, grid);
+  constexpr int kStages = 2;
+  if (p.c.dtype == dtype) return launch<T, Cfg<T, kSame, D, kStages>>(p, st, sms, grid);
+  if (p.c.dtype == MCPU_INT8) return launch<T, Cfg<T, kInt8, D, kStages>>(p, st, sms, grid);
+  return launch<T, Cfg<T, kE4M3, D, kStages>>(p, st, sms, grid);
 }
 
 template <typename T, int D>
@@ -745,10 +740,10 @@ orError_t run(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, i
   p.part_o = static_cast<float*>(ws);
   p.part_ml = p.part_o + part_rows(sms, rows) * D;
   int grid = 0;
-  const orError_t e = rows <= kFewRows ? launch_few<T, D>(p, dtype, st, sms, &grid) : launch_tc(p, D, rows, st, sms, &grid);
+  const orError_t e = rows <= kRows ? launch_few<T, D>(p, dtype, st, sms, &grid) : launch_tc(p, D, rows, st, sms, &grid);
   if (e != orSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / (kJoinThreads / 8)));
+  cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / 32));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -847,7 +842,7 @@ extern "C" orError_t mcpu_tree_attention(
   p.mask = reinterpret_cast<const long long*>(tree_mask), p.mask_stride = mask_stride;
   p.mask_words = static_cast<int>(std::min<int64_t>(mask_words, 1 << 20));
   p.batch = static_cast<int>(batch), p.tokens = static_cast<int>(num_tokens);
-  p.kv_heads = kv, p.group = num_heads / kv;
+  p.kv_heads = kv, p.group = num_heads / kv, p.most = static_cast<int>(max_query_len);
   p.scale_log2 = scale * 1.4426950408889634f;
   const long long rows_max = max_query_len * p.group;
   cudaStream_t st = as_cuda(stream);

@@ -31,6 +31,7 @@ struct Params {
   long long mask_stride;
   int mask_words;
   int batch, tokens, kv_heads, group;
+  int most;  // new tokens of a request
   float scale_log2;
   int rows_log2, keys_log2;  // rows and keys of a unit
   int min_share;
@@ -53,7 +54,7 @@ __device__ __forceinline__ Request request(const Params& p, int b) {
   const bool fits = r.first >= 0 && r.n >= 0 && end <= p.tokens;
   const long long room = static_cast<long long>(p.table_width) * p.c.block_size;
   const bool words = p.mask == nullptr || r.n <= 64 * p.mask_words;
-  if (!fits || r.len < r.n || r.len > room || !words) {
+  if (!fits || r.len < r.n || r.len > room || !words || r.n > p.most) {
     atomicOr(&g_attn_error, 1);
     if (!fits) r.first = 0, r.n = 0;
     r.len = 0;
