@@ -32,6 +32,12 @@
 
 #include "tree_attention.cuh"
 
+#ifndef ECOST
+#define ECOST 2
+#endif
+#ifndef DMIN
+#define DMIN 2
+#endif
 #ifndef MINSHARE
 #define MINSHARE 2
 #endif
@@ -124,9 +130,9 @@ struct Place {
   bool valid;
 };
 template <typename C>
-__device__ __forceinline__ Place look(const Params& p, const Walk& w, int warp, int lane) {
+__device__ __forceinline__ Place look(const Params& p, const Pieces& w, int tile, int warp, int lane) {
   Place at{0, 0, false};
-  const int key = w.tile * C::TN + warp * C::KW + lane;
+  const int key = (w.tile0 + tile) * C::TN + warp * C::KW + lane;
   if (lane < C::KW && key < w.r.len) {
     const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
     at.slot = key - page * p.c.block_size;
@@ -138,7 +144,7 @@ __device__ __forceinline__ Place look(const Params& p, const Walk& w, int warp, 
 
 // Starts a warp's copies of its keys and values of a unit.
 template <typename C>
-__device__ __forceinline__ void copy_step(const Params& p, const Walk& w, const Place& at, uint32_t stage, int lane) {
+__device__ __forceinline__ void copy_step(const Params& p, const Pieces& w, const Place& at, uint32_t stage, int lane) {
   constexpr int kPer = C::kSmall ? 16 : 8;  // values in 16 bytes
   constexpr int kAtOnce = 32 / C::kChunks;  // rows a copy of the whole warp takes
   const int h = w.item;                     // up to 16 rows: items are key / value heads
@@ -152,13 +158,17 @@ __device__ __forceinline__ void copy_step(const Params& p, const Walk& w, const 
   const int c = lane % C::kChunks, r0 = lane / C::kChunks;
   const uint4* kb = static_cast<const uint4*>(p.c.key) + (h * p.c.key_stride[2] / kPer + c);
   const uint4* vb = static_cast<const uint4*>(p.c.value) + (h * p.c.value_stride[2] / kPer + c);
+  // shuffles first: copies and shuffles keep their order, and in turn each copy would wait for its shuffle
+  constexpr int kSteps = C::KW / kAtOnce;
+  uint32_t k[kSteps], v[kSteps];
 #pragma unroll
-  for (int i = 0; i < C::KW / kAtOnce; ++i) {
+  for (int i = 0; i < kSteps; ++i) k[i] = __shfl_sync(kFull, ko, i * kAtOnce + r0), v[i] = __shfl_sync(kFull, vo, i * kAtOnce + r0);
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
     const int row = i * kAtOnce + r0;
     const bool in = (valid >> row) & 1;
-    const uint32_t k = __shfl_sync(kFull, ko, row), v = __shfl_sync(kFull, vo, row);
-    cp_async16(stage + place<C>(row, c), kb + k, in);
-    cp_async16(stage + C::kHalf + place<C>(row, c), vb + v, in);
+    cp_async16(stage + place<C>(row, c), kb + k[i], in);
+    cp_async16(stage + C::kHalf + place<C>(row, c), vb + v[i], in);
   }
   if constexpr (C::kSmall) {
     const long long b = block, sl = at.slot;
@@ -192,7 +202,7 @@ __device__ __forceinline__ bool any_wild(const uint8_t* values) {
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, DMIN) attend_kernel(const __grid_constant__ Params p) {
   constexpr int D = C::D, KW = C::KW, KIND = C::KIND;
   constexpr int kNT = KW / 8;   // 8-key tiles of the scores
   constexpr int kDT = D / 8;    // 8-dimension tiles of the output
@@ -218,39 +228,44 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       },
       red, total, unit, b0, before);
   clear_idle_requests<kThreads>(p, D);
-  if (unit >= total) return;
-  const int end = min(unit + share, total);
+  int4 join = make_int4(0, 0, 0, 0);
+  Pieces pc, ahead;  // the piece worked on, the one copied
+  const bool busy = unit < total && pc.start(p, b0, before, unit, min(share, total - unit));
+  if (!busy) {
+    if (tid == 0) p.joins[blockIdx.x] = join;
+    return;
+  }
 
   // every warp walks the units by itself: its copies, its steps, no barrier until an item ends
-  Walk cur, ahead;
-  cur.seek(p, b0, unit - before);
-  ahead = cur;
-  int loaded = unit;
-  Place next = look<C>(p, ahead, warp, lane);
+  ahead = pc;
+  int ahead_tile = 0;
+  bool more = true;
+  Place next = look<C>(p, ahead, 0, warp, lane);
   auto load = [&](int s) {
-    if (loaded < end) {
-      copy_step<C>(p, ahead, next, stages + s * C::kStage, lane);
-      if (++loaded < end) {
-        ahead.next(p);
-        next = look<C>(p, ahead, warp, lane);
+    if (more) {
+      const Place at = next;
+      copy_step<C>(p, ahead, at, stages + s * C::kStage, lane);
+      if (++ahead_tile == ahead.nt) {
+        ahead_tile = 0;
+        more = ahead.next(p);
       }
+      if (more) next = look<C>(p, ahead, ahead_tile, warp, lane);
     }
     cp_commit();
   };
 #pragma unroll
   for (int s = 0; s < C::STAGES - 1; ++s) load(s);
 
-  uint32_t qf[D / 16][4];
+  uint4* qs = reinterpret_cast<uint4*>(scratch);  // the queries' fragments, the same for every warp
   float qscale[2];
   float acc[kDT][4];
   float m[2], l[2], vref = 0.0f;
-  bool fresh = true;
-  int first_tile = 0;
   int tok[2], qi[2], head[2];
   bool row_ok[2];
   int stage = 0;
 
-  for (int u = unit; u < end; ++u) {
+  do {
+   for (int tile = 0; tile < pc.nt; ++tile) {
     cp_wait<C::STAGES - 2>();
     __syncwarp();
     {
@@ -259,16 +274,15 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       load(s);
     }
 
-    if (fresh) {
-      fresh = false;
-      first_tile = cur.tile;
+    if (tile == 0) {
+      uint32_t qf[D / 16][4];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int row = g + 8 * e;
-        row_ok[e] = row < cur.r.n * p.group;
+        row_ok[e] = row < pc.r.n * p.group;
         qi[e] = row / p.group;
-        head[e] = cur.item * p.group + row - qi[e] * p.group;
-        tok[e] = cur.r.first + qi[e];
+        head[e] = pc.item * p.group + row - qi[e] * p.group;
+        tok[e] = pc.r.first + qi[e];
         m[e] = -INFINITY;
         l[e] = 0.0f;
         qscale[e] = p.scale_log2;
@@ -314,6 +328,10 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
             }
         }
       }
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+        if (kk % kWarps == warp) qs[kk * 32 + lane] = make_uint4(qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
+      __syncthreads();
       vref = 0.0f;
 #pragma unroll
       for (int i = 0; i < kDT; ++i)
@@ -333,17 +351,22 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     const int mi = lane >> 3, mr = lane & 7;
     if constexpr (!C::kSmall) {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint4 q4 = qs[kk * 32 + lane];
+        const uint32_t qf[4] = {q4.x, q4.y, q4.z, q4.w};
 #pragma unroll
         for (int n = 0; n < kNT; n += 2) {
           uint32_t b[4];
           ldsm4(b, ks + place<C>(n * 8 + (mi >> 1) * 8 + mr, kk * 2 + (mi & 1)));
-          mma<C::kBf16>(s[n], qf[kk], b[0], b[1]);
-          mma<C::kBf16>(s[n + 1], qf[kk], b[2], b[3]);
+          mma<C::kBf16>(s[n], qf, b[0], b[1]);
+          mma<C::kBf16>(s[n + 1], qf, b[2], b[3]);
         }
+      }
     } else {
 #pragma unroll
-      for (int kk = 0; kk < D / 16; kk += 2)
+      for (int kk = 0; kk < D / 16; kk += 2) {
+        const uint4 qa = qs[kk * 32 + lane], qb = qs[(kk + 1) * 32 + lane];
+        const uint32_t qf[2][4] = {{qa.x, qa.y, qa.z, qa.w}, {qb.x, qb.y, qb.z, qb.w}};
 #pragma unroll
         for (int n = 0; n < kNT; n += 2) {
           uint32_t b[4];
@@ -351,19 +374,20 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
 #pragma unroll
           for (int x = 0; x < 4; ++x) {
             const uint32_t w = KIND == kInt8 ? b[x] ^ 0x80808080u : b[x];
-            mma<false>(s[n + (x >> 1)], qf[kk + (x & 1)], widen<KIND, 0, 1>(w), widen<KIND, 2, 3>(w));
+            mma<false>(s[n + (x >> 1)], qf[x & 1], widen<KIND, 0, 1>(w), widen<KIND, 2, 3>(w));
           }
         }
+      }
     }
 
     // ---- scale, mask, running maximum
-    const int key0 = cur.tile * C::TN + warp * KW;
-    const bool tail = key0 + KW > cur.r.len - cur.r.n;
+    const int key0 = (pc.tile0 + tile) * C::TN + warp * KW;
+    const bool tail = key0 + KW > pc.r.len - pc.r.n;
     uint32_t view[2] = {kFull, kFull};  // the keys a row sees
     if (tail) {
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        view[e] = seen32(p, cur.r, row_ok[e] ? tok[e] : cur.r.first, row_ok[e] ? qi[e] : 0, key0) >> (2 * j4);
+        view[e] = seen32(p, pc.r, row_ok[e] ? tok[e] : pc.r.first, row_ok[e] ? qi[e] : 0, key0) >> (2 * j4);
     }
     float top[2] = {-INFINITY, -INFINITY};
     float vmax = 0.0f;
@@ -434,7 +458,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     }
 
     // ---- probabilities times values
-    if (KIND != kInt8 && tail && cur.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf)) {
+    if (KIND != kInt8 && tail && pc.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf)) {
 #pragma unroll
       for (int kk = 0; kk < kNT / 2; ++kk) {
         const int row = kk * 16 + (mi & 1) * 8 + mr;
@@ -495,13 +519,14 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
       }
     }
     __syncwarp();  // the stage is read before the next copies into it
+    if (++stage == C::STAGES) stage = 0;
+   }
 
-    // ---- end of the item, or of this block's run: join the warps, write
-    const bool last_tile = cur.tile + 1 == cur.tiles;
-    if (last_tile || u + 1 == end) {
-      fresh = true;
-      const bool whole = first_tile == 0 && last_tile;
-      const int slot = first_tile == 0 ? 1 : 0;
+    // ---- end of the piece: join the warps, write
+    {
+      const bool whole = pc.nt == pc.tiles;
+      const int slot = pc.tile0 == 0 ? 1 : 0;
+      if (!whole && pc.tile0 == 0) join = make_int4(parts_of(p, pc, share), pc.b, pc.item, 0);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(kFull, l[e], 1);
@@ -569,19 +594,18 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
         }
         if (!whole) {
           *reinterpret_cast<float4*>(p.part_o + (part + row) * D + d0 + d) = sum;
-        } else if (row < cur.r.n * p.group) {
+        } else if (row < pc.r.n * p.group) {
           const int i2 = row / p.group;
-          T* o = static_cast<T*>(p.out) + (cur.r.first + i2) * p.o_tok + (cur.item * p.group + row - i2 * p.group) * p.o_head;
+          T* o = static_cast<T*>(p.out) + (pc.r.first + i2) * p.o_tok + (pc.item * p.group + row - i2 * p.group) * p.o_head;
           constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
           *reinterpret_cast<uint2*>(o + d0 + d) = make_uint2(pack2<kOutBf16>(sum.x, sum.y), pack2<kOutBf16>(sum.z, sum.w));
         }
       }
       __syncthreads();
     }
-    cur.next(p);
-    if (++stage == C::STAGES) stage = 0;
-  }
+  } while (pc.next(p));
   cp_wait<0>();
+  if (tid == 0) p.joins[blockIdx.x] = join;
 }
 
 // ---------------------------------------------------------------- joining kernel
@@ -593,28 +617,16 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p) {
   constexpr int kJoinWarps = kJoinThreads / 32;
-  __shared__ int red[kJoinWarps + 2];
   __shared__ float4 sums[kJoinWarps][4][D / 4];
   __shared__ float2 sums_ml[kJoinWarps][4];
-  const int grid = gridDim.x, c = blockIdx.x, rows = 1 << p.rows_log2;
-  int total, unit, b, before, share = 0;
-  locate<kJoinThreads>(
-      p,
-      [&](int tot) {
-        share = share_of(p, tot, grid);
-        return static_cast<int>(min((c + 1ll) * share - 1, 2147483647ll));
-      },
-      red, total, unit, b, before);
+  const int c = blockIdx.x, rows = 1 << p.rows_log2;
   // every block waits, also those with nothing to join: what follows on the
   // stream must not overtake the main kernel
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (unit >= total - 1) return;
-  const Request r = request(p, b);
-  const int tiles = key_tiles(p, r);
-  const int item = (unit - before) / tiles;
-  const int from = before + item * tiles, to = from + tiles - 1;
-  if (from / share != c || to / share == c) return;
-  const int parts = to / share - c + 1;
+  const int4 join = p.joins[c];  // parts, request, item
+  const int parts = join.x, item = join.z;
+  if (parts == 0) return;
+  const Request r = request(p, join.y);
   const int rts = row_tiles(p, r);
   const int h = item / rts, rt = item - h * rts;
   const int first = rt * rows + blockIdx.y * 32, left = min(rows - static_cast<int>(blockIdx.y) * 32, r.n * p.group - first);
@@ -722,6 +734,7 @@ orError_t launch(Params& p, cudaStream_t st, int sms, int* grid) {
   *grid = resident * sms;
   p.rows_log2 = 4;
   p.keys_log2 = C::TN == 64 ? 6 : 7;
+  p.item_cost = ECOST;
   p.min_share = MINSHARE;
   attend_kernel<T, C><<<*grid, kThreads, C::kSmem, st>>>(p);
   return from_cuda(cudaGetLastError(), "tree_attention launch");
@@ -739,6 +752,7 @@ template <typename T, int D>
 orError_t run(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, int sms) {
   p.part_o = static_cast<float*>(ws);
   p.part_ml = p.part_o + part_rows(sms, rows) * D;
+  p.joins = reinterpret_cast<int4*>(p.part_ml + part_rows(sms, rows) * 2);
   int grid = 0;
   const orError_t e = rows <= kRows ? launch_few<T, D>(p, dtype, st, sms, &grid) : launch_tc(p, D, rows, st, sms, &grid);
   if (e != orSuccess) return e;
@@ -782,7 +796,8 @@ extern "C" orError_t mcpu_tree_attention_workspace_bytes(int64_t max_query_len, 
                  MCPU_TREE_MAX_QUERIES);
   attn::Device d{};
   if (attn::device(&d) != orSuccess) d.sms = 148;
-  *bytes = attn::part_rows(d.sms, max_query_len * (num_heads / num_kv_heads)) * (head_size + 2) * 4;
+  *bytes = attn::part_rows(d.sms, max_query_len * (num_heads / num_kv_heads)) * (head_size + 2) * 4 +
+           16ull * attn::kMaxResident * d.sms;
   return orSuccess;
 }
 
@@ -824,7 +839,7 @@ extern "C" orError_t mcpu_tree_attention(
   // unit numbers are 32-bit: the longest requests the table can hold, with tiles of 64 keys and 16 rows
   const double room = static_cast<double>(table_width) * cache->block_size;
   const double rows = static_cast<double>(max_query_len) * (num_heads / kv);
-  MCPU_ARG_CHECK(room < 2147483000.0 && batch * kv * (rows / 16 + 1) * (room / 64 + 1) < 2147483000.0,
+  MCPU_ARG_CHECK(room < 2147483000.0 && batch * kv * (rows / 16 + 1) * (room / 64 + 9) < 2147483000.0,
                  "%s: batch, heads and block_table are too large for one call", op);
   attn::Device d{};
   e = attn::device(&d);

@@ -34,10 +34,12 @@ struct Params {
   int most;  // new tokens of a request
   float scale_log2;
   int rows_log2, keys_log2;  // rows and keys of a unit
+  int item_cost;             // what beginning and ending a row tile costs, in key tiles
   int min_share;
   int bf16;                  // type of query and out: bf16, else fp16
   float* part_o;             // [grid][2][rows][D]
   float* part_ml;            // [grid][2][rows][2]
+  int4* joins;               // [grid]: the row tile that begins in a block and goes on behind it
 };
 
 // ---------------------------------------------------------------- schedule
@@ -69,8 +71,10 @@ __device__ __forceinline__ int key_tiles(const Params& p, const Request& r) {
 __device__ __forceinline__ int row_tiles(const Params& p, const Request& r) {
   return (r.n * p.group + (1 << p.rows_log2) - 1) >> p.rows_log2;
 }
+// A row tile counts as its key tiles and, in front of them, item_cost more: a
+// block that gets many short row tiles does not end after the others.
 __device__ __forceinline__ int units(const Params& p, const Request& r) {
-  return r.len == 0 ? 0 : p.kv_heads * row_tiles(p, r) * key_tiles(p, r);
+  return r.len == 0 ? 0 : p.kv_heads * row_tiles(p, r) * (key_tiles(p, r) + p.item_cost);
 }
 
 // Block-wide: total units, then the request that holds `unit` (a function of
@@ -124,36 +128,63 @@ __device__ __forceinline__ int share_of(const Params& p, int total, int grid) {
   return max((total + grid - 1) / grid, p.min_share);
 }
 
-// Position in the list of units: request, item (key / value head, row tile)
-// and key tile.
-struct Walk {
-  int b, item, tile, items, tiles;
+// A block's run of units as pieces: key tiles tile0 .. tile0 + nt - 1 of one
+// row tile (item: key / value head and row tile of request b).
+struct Pieces {
+  int b, item, items, tiles;
   Request r;
+  int tile0, nt;
+  int begin;  // unit the item begins with
+  int v, left;  // where the next piece begins in the item, units left
+
   __device__ __forceinline__ void open(const Params& p) {
     r = request(p, b);
     tiles = key_tiles(p, r);
     items = r.len == 0 ? 0 : p.kv_heads * row_tiles(p, r);
   }
-  __device__ __forceinline__ void seek(const Params& p, int b_, int offset) {
-    b = b_;
+  __device__ __forceinline__ bool start(const Params& p, int b0, int before, int unit, int count) {
+    b = b0;
     open(p);
-    item = offset / tiles;
-    tile = offset - item * tiles;
+    const int offset = unit - before, span = tiles + p.item_cost;
+    item = offset / span;
+    v = offset - item * span;
+    begin = unit - v;
+    left = count;
+    return take(p);
   }
-  __device__ __forceinline__ void skip(const Params& p, int count) {  // count <= tiles - tile
-    tile += count;
-    if (tile < tiles) return;
-    tile = 0;
-    if (++item < items) return;
-    item = 0;
-    do {
-      ++b;
-      if (b >= p.batch) return;
-      open(p);
-    } while (items == 0);
+  // The next piece with keys; false: no more.
+  __device__ __forceinline__ bool next(const Params& p) { return take(p); }
+
+ private:
+  __device__ __forceinline__ bool take(const Params& p) {
+    while (left > 0) {
+      const int span = tiles + p.item_cost;
+      if (v == span) {
+        v = 0;
+        begin += span;
+        if (++item == items) {
+          item = 0;
+          do ++b, open(p);  // units are left, so a request with some follows
+          while (items == 0);
+        }
+        continue;
+      }
+      const int count = min(span - v, left);
+      tile0 = max(v - p.item_cost, 0);
+      nt = max(v + count - p.item_cost, 0) - tile0;
+      v += count;
+      left -= count;
+      if (nt > 0) return true;
+    }
+    return false;
   }
-  __device__ __forceinline__ void next(const Params& p) { skip(p, 1); }
 };
+
+// Parts an item is in: from the block of its first key tile to that of its last.
+__device__ __forceinline__ int parts_of(const Params& p, const Pieces& pc, int share) {
+  const int first = pc.begin + p.item_cost;
+  return (first + pc.tiles - 1) / share - first / share + 1;
+}
 
 // Requests without work (no keys, or refused) still have outputs: a warp each.
 template <int NT>

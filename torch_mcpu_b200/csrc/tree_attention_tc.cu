@@ -15,9 +15,9 @@
 //             tensor-memory lane), reads the scores, keeps the running maximum
 //             and sum, writes the probabilities over the scores as 16-bit
 //             values, the left operand of the second product
-//   1 or 2    loaders.  16-bit caches: pages to shared memory by 16-byte
+//   1         loaders.  16-bit caches: pages to shared memory by 16-byte
 //             asynchronous copies into the 128-byte-swizzled layout.  8-bit
-//             ones (2 groups): rows of a raw ring widened to fp16
+//             ones: rows of a raw ring widened to fp16
 //   1         its first warp issues the products; with 8-bit caches two more
 //             fetch the rows of keys and of values, and the
 //             last looks at the scales
@@ -32,6 +32,10 @@
 #include "sm100.cuh"
 #include "tree_attention.cuh"
 
+#ifndef ECOST1
+#define ECOST1 8
+#define ECOST2 7
+#endif
 namespace mcpu {
 namespace attn {
 namespace tc {
@@ -42,10 +46,6 @@ constexpr int kSoftWarps = 8;
 constexpr int kTile = 128;        // rows and keys of a tile
 constexpr int kTmemCols = 512;
 constexpr int kScaleRing = 8;     // key tiles whose scales are kept
-#ifndef POLY
-#define POLY 0
-#endif
-constexpr int kPolyOf4 = POLY;
 constexpr float kGrow = 8.0f;     // log2 of the growth of a maximum that is tolerated
 
 template <int KIND_, bool BF16_, int D_, bool TOKEN_>
@@ -54,13 +54,12 @@ struct Cfg {
   static constexpr bool BF16 = BF16_;    // type of the products; 8-bit caches: fp16
   static constexpr bool TOKEN = TOKEN_;  // a scale for every token and head
   static constexpr bool kSmall = KIND != kSame;
-  static constexpr int kLoadWarps = kSmall ? 8 : 4;
+  static constexpr int kLoadWarps = 4;
   static constexpr int kRowsPerWarp = kTile / kLoadWarps;
   static constexpr int kWarps = kSoftWarps + kLoadWarps + 4;
   static constexpr int kThreads = 32 * kWarps;
   // registers: what the block is launched with (a multiple of 8 that fits), then each group's own share of it
-  static constexpr int kRegs = kSmall ? 96 : 128, kSoftRegs = kSmall ? 144 : 200, kLoadRegs = kSmall ? 56 : 64,
-                       kIssueRegs = kSmall ? 80 : 48;
+  static constexpr int kRegs = 128, kSoftRegs = 144, kLoadRegs = 96, kIssueRegs = 128;
   static_assert(kSoftWarps * kSoftRegs + kLoadWarps * kLoadRegs + 4 * kIssueRegs <= kWarps * kRegs, "more than launched with");
   static constexpr int kSlots = kSmall ? 3 : 4;  // key or value tiles in shared memory
   static constexpr int kSlot = kTile * D * 2;
@@ -185,28 +184,10 @@ __device__ __forceinline__ uint32_t place16(int row, int c) {
   return (c >> 3) * (kTile * 128) + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 }
 
-// ---------------------------------------------------------------- runs of key tiles
-// A block's units as pieces: a run of key tiles of one item.
-struct Pieces {
-  Walk w;
-  int left;   // units behind the current piece
-  int tile0, nt;
-  __device__ __forceinline__ void start(const Params& p, int b0, int offset, int count) {
-    w.seek(p, b0, offset);
-    left = count;
-    take();
-  }
-  __device__ __forceinline__ void take() {
-    tile0 = w.tile;
-    nt = min(w.tiles - w.tile, left);
-    left -= nt;
-  }
-  __device__ __forceinline__ bool next(const Params& p) {  // false: no more
-    if (left <= 0) return false;
-    w.skip(p, nt);
-    take();
-    return true;
-  }
+// ---------------------------------------------------------------- loads
+// A block's run: where its units begin, and how many they are.
+struct Run {
+  int b0, before, unit, count;
 };
 
 // The order in which a piece's key and value tiles are loaded, which is the
@@ -234,10 +215,10 @@ struct Place {
 __device__ __forceinline__ Place look(const Params& p, const Pieces& pc, int tile, int row) {
   Place at{0, 0, false};
   const int key = (pc.tile0 + tile) * kTile + row;
-  if (key < pc.w.r.len) {
+  if (key < pc.r.len) {
     const int page = p.block_log2 >= 0 ? key >> p.block_log2 : key / p.c.block_size;
     at.slot = key - page * p.c.block_size;
-    at.id = p.table[pc.w.b * p.table_stride + page];
+    at.id = p.table[pc.b * p.table_stride + page];
     at.valid = true;
   }
   return at;
@@ -273,7 +254,7 @@ struct Loader {
 
   // Value tiles with new tokens that some of the request's rows may not see: a lane looks through the values it wrote.
   __device__ __forceinline__ void clean_tail(const Pieces& pc, int tile, uint32_t s) const {
-    if (C::KIND == kInt8 || pc.w.r.n <= 1 || (pc.tile0 + tile + 1) * kTile <= pc.w.r.len - pc.w.r.n) return;
+    if (C::KIND == kInt8 || pc.r.n <= 1 || (pc.tile0 + tile + 1) * kTile <= pc.r.len - pc.r.n) return;
     constexpr int kChunks = C::D * (C::kSmall ? 1 : 2) / 16, kRows = 32 / kChunks, kSteps = C::kRowsPerWarp / kRows;
     constexpr uint32_t kExp = C::BF16 ? 0x7F807F80u : 0x7C007C00u;
     const int c = lane % kChunks, row0 = C::kRowsPerWarp * lw + lane / kChunks;
@@ -308,17 +289,21 @@ struct Loader {
   // oldest one under way is waited for and handed over.
   __device__ __forceinline__ void copy(const Pieces& pc, const Place& at, bool is_v, uint32_t dst) const {
     const unsigned rows_valid = __ballot_sync(kFull, at.valid);
-    const int h = pc.w.item / row_tiles(p, pc.w.r);
+    const int h = pc.item / row_tiles(p, pc.r);
     const uint32_t off = offset16(at, is_v ? p.c.value_stride : p.c.key_stride);
     constexpr int kChunks = C::D * 2 / 16, kRows = 32 / kChunks;
     const int c = lane % kChunks;
     const uint4* from = static_cast<const uint4*>(is_v ? p.c.value : p.c.key) +
                         (h * (is_v ? p.c.value_stride[2] : p.c.key_stride[2]) / 8 + c);
+    // shuffles first: copies and shuffles keep their order, and in turn each copy would wait for its shuffle
+    constexpr int kSteps = C::kRowsPerWarp / kRows;
+    uint32_t o[kSteps];
 #pragma unroll
-    for (int i = 0; i < C::kRowsPerWarp / kRows; ++i) {
+    for (int i = 0; i < kSteps; ++i) o[i] = __shfl_sync(kFull, off, i * kRows + lane / kChunks);
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
       const int row = i * kRows + lane / kChunks;
-      const uint32_t o = __shfl_sync(kFull, off, row);
-      cp_async16(dst + place16(C::kRowsPerWarp * lw + row, c), from + o, (rows_valid >> row) & 1);
+      cp_async16(dst + place16(C::kRowsPerWarp * lw + row, c), from + o[i], (rows_valid >> row) & 1);
     }
   }
   // A row's place in 16-byte units: 32 bits reach 64 GB, which the entry point makes sure of.
@@ -328,10 +313,10 @@ struct Loader {
     return static_cast<uint32_t>(block) * static_cast<uint32_t>(st[0] / kPer) +
            static_cast<uint32_t>(at.slot) * static_cast<uint32_t>(st[1] / kPer);
   }
-  __device__ __forceinline__ void run_copies(int b0, int offset, int count) {
+  __device__ __forceinline__ void run_copies(const Run& run) {
     const int lead = nq == 1 ? 2 : 1, row = C::kRowsPerWarp * lw + lane;
     Pieces a, f, k;  // tiles being started, being handed over, being looked up (two ahead)
-    a.start(p, b0, offset, count);
+    a.start(p, run.b0, run.before, run.unit, run.count);
     f = a, k = a;
     int as = 0, fs = 0, ks = 0;
     uint32_t ac = 0, fc = 0;
@@ -398,17 +383,17 @@ struct Loader {
   }
 
   // ---- 8-bit caches, fetching: one warp takes the key tiles, one the value tiles.
-  __device__ __forceinline__ void run_fetch(bool values, int b0, int offset, int count) {
+  __device__ __forceinline__ void run_fetch(bool values, const Run& run) {
     const int lead = nq == 1 ? 2 : 1;
     const int64_t* st = values ? p.c.value_stride : p.c.key_stride;
     const int64_t* ss = values ? p.c.v_scale_stride : p.c.k_scale_stride;
     Pieces pc;
-    pc.start(p, b0, offset, count);
+    pc.start(p, run.b0, run.before, run.unit, run.count);
     uint32_t n0 = 0, t0 = 0;  // tiles and key tiles before the piece
     bool ok = true;
     do {
       const int nt = pc.nt, first = min(lead, nt);
-      const int h = pc.w.item / row_tiles(p, pc.w.r);
+      const int h = pc.item / row_tiles(p, pc.r);
       constexpr int kChunks = C::D / 16, kRows = 32 / kChunks;  // rows a copy of the whole warp takes
       const int c = lane % kChunks;
       const uint4* from = static_cast<const uint4*>(values ? p.c.value : p.c.key) + (h * st[2] / 16 + c);
@@ -434,11 +419,13 @@ struct Loader {
         for (int i = 0; i < 4; ++i) {
           const unsigned valid = __ballot_sync(kFull, now[i].valid);
           const uint32_t off = offset16(now[i], st);
+          uint32_t o[32 / kRows];
+#pragma unroll
+          for (int k = 0; k < 32 / kRows; ++k) o[k] = __shfl_sync(kFull, off, k * kRows + lane / kChunks);
 #pragma unroll
           for (int k = 0; k < 32 / kRows; ++k) {
             const int row = k * kRows + lane / kChunks;
-            const uint32_t o = __shfl_sync(kFull, off, row);
-            cp_async16(dst + ((32 * i + row) * kChunks + c) * 16, from + o, (valid >> row) & 1);
+            cp_async16(dst + ((32 * i + row) * kChunks + c) * 16, from + o[k], (valid >> row) & 1);
           }
           if constexpr (C::TOKEN) {
             const long long block = kv::checked_block(now[i].id, p.c.num_blocks, &g_attn_error);
@@ -459,9 +446,9 @@ struct Loader {
   }
 
   // ---- token scales: the largest finite one of each tile's values, for the reference the probabilities are scaled by.
-  __device__ __forceinline__ void run_scales(int b0, int offset, int count) {
+  __device__ __forceinline__ void run_scales(const Run& run) {
     Pieces pc;
-    pc.start(p, b0, offset, count);
+    pc.start(p, run.b0, run.before, run.unit, run.count);
     uint32_t t = 0;
     bool ok = true;
     do {
@@ -484,12 +471,12 @@ struct Loader {
   }
 
   // ---- 8-bit caches, widening: raw rows to fp16 in the swizzled tiles.
-  __device__ __forceinline__ void run_widen(int b0, int offset, int count) {
+  __device__ __forceinline__ void run_widen(const Run& run) {
     const int lead = nq == 1 ? 2 : 1;
     constexpr int kChunks = C::D / 16, kRows = 32 / kChunks, kSteps = C::kRowsPerWarp / kRows;
     const int c = lane % kChunks, row0 = C::kRowsPerWarp * lw + lane / kChunks;
     Pieces pc;
-    pc.start(p, b0, offset, count);
+    pc.start(p, run.b0, run.before, run.unit, run.count);
     uint32_t n = 0;
     bool ok = true;
     do {
@@ -517,8 +504,11 @@ struct Loader {
             o[2 * x] = widen<C::KIND, 0, 1>(w[x]);
             o[2 * x + 1] = widen<C::KIND, 2, 3>(w[x]);
           }
-          *reinterpret_cast<uint4*>(slot + place16(row, 2 * c)) = make_uint4(o[0], o[1], o[2], o[3]);
-          *reinterpret_cast<uint4*>(slot + place16(row, 2 * c + 1)) = make_uint4(o[4], o[5], o[6], o[7]);
+          // the lanes of the second 64 dimensions store their halves the other way round: all banks at once
+          const bool late = C::D == 128 && c >= kChunks / 2;
+          const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]), hi = make_uint4(o[4], o[5], o[6], o[7]);
+          *reinterpret_cast<uint4*>(slot + place16(row, 2 * c + late)) = late ? hi : lo;
+          *reinterpret_cast<uint4*>(slot + place16(row, 2 * c + !late)) = late ? lo : hi;
         }
         if (is_v) clean_tail(pc, tile, s);
         hand_over(s);
@@ -553,29 +543,6 @@ __device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigne
   unsigned long long r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-
-// 2^x of two values on the multiply-add pipe, where the special-function unit
-// (16 results per cycle and SM) is what the softmax waits for: the whole part
-// by adding 1.5 * 2^23, 2^f on [-1/2, 1/2] by a polynomial of degree 5 fitted
-// for the least relative error (8e-8), the whole part added to the exponent.
-// x <= 2^7; below -126 the result is under 2^-125; NaN stays NaN.
-__device__ __forceinline__ float2 exp2_pair(unsigned long long x) {
-  float2 c = unpair(x);
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.x));
-  asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(c.y));
-  x = pair(c.x, c.y);
-  const unsigned long long t = add2(x, pair(12582912.0f, 12582912.0f));
-  const unsigned long long f = add2(x, mul2(add2(t, pair(-12582912.0f, -12582912.0f)), pair(-1.0f, -1.0f)));
-  unsigned long long r = pair(0.0013276472454890609f, 0.0013276472454890609f);
-  r = fma2(r, f, pair(0.009675540961325169f, 0.009675540961325169f));
-  r = fma2(r, f, pair(0.05550713092088699f, 0.05550713092088699f));
-  r = fma2(r, f, pair(0.24022120237350464f, 0.24022120237350464f));
-  r = fma2(r, f, pair(0.6931469440460205f, 0.6931469440460205f));
-  r = fma2(r, f, pair(1.0000001192092896f, 1.0000001192092896f));
-  const float2 tt = unpair(t), rr = unpair(r);
-  return make_float2(__uint_as_float(__float_as_uint(rr.x) + (__float_as_uint(tt.x) << 23)),
-                     __uint_as_float(__float_as_uint(rr.y) + (__float_as_uint(tt.y) << 23)));
 }
 
 // One thread's row of the softmax.
@@ -663,29 +630,20 @@ struct Soft {
   // Scores of one key tile to probabilities.  TAIL: some keys are not seen (a bit each in seen).
   template <bool TAIL>
   __device__ __forceinline__ void tile(const uint32_t (&seen)[4], const float* ks, const float* vs, float vmax, bool first) {
-    // 16-bit caches hold the row in registers; with 8-bit ones, whose loaders need the registers, it is read twice
-    constexpr bool kHold = !C::kSmall;
-    uint32_t s[kHold ? 4 : 2][32];
+    // The row is read twice, 64 scores at a time, in rolled loops: reading it is cheap, while the code of a whole row
+    // unrolled, beside that of the other roles, runs out of the instruction cache.
     float top = -INFINITY;
-    if constexpr (kHold) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(tmem_s + 32 * c, s[c]);
+#pragma unroll 1
+    for (int c = 0; c < 4; c += 2) {
+      uint32_t s[2][32];
+      tmem_ld32(tmem_s + 32 * c, s[0]);
+      tmem_ld32(tmem_s + 32 * c + 32, s[1]);
       tmem_ld_wait();
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        scaled<TAIL>(s[c], ks, seen[c]);
-        top = top_of(s[c], top);
+      for (int y = 0; y < 2; ++y) {
+        scaled<TAIL>(s[y], ks + 32 * (c + y), TAIL ? (c == 0 ? seen[y] : seen[2 + y]) : kFull);
+        top = top_of(s[y], top);
       }
-    } else {
-      tmem_ld32(tmem_s, s[0]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tmem_ld_wait();
-        if (c < 3) tmem_ld32(tmem_s + 32 * (c + 1), s[(c + 1) & 1]);
-        scaled<TAIL>(s[c & 1], ks + 32 * c, seen[c]);
-        top = top_of(s[c & 1], top);
-      }
-      tmem_ld32(tmem_s, s[0]);
     }
     top *= qscale;
     // the reference moves when the maximum left it by more than 2^kGrow
@@ -718,50 +676,47 @@ struct Soft {
     const float inv = C::TOKEN ? __uint_as_float(0x7F000000u - __float_as_uint(vref)) : 1.0f;
     const unsigned long long i2 = pair(inv, inv);
     unsigned long long sum0 = pair(0.0f, 0.0f), sum1 = sum0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < 4; c0 += 2) {
+      uint32_t s[2][32];
+      tmem_ld32(tmem_s + 32 * c0, s[0]);
+      tmem_ld32(tmem_s + 32 * c0 + 32, s[1]);
+      tmem_ld_wait();
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      uint32_t(&v)[32] = s[kHold ? c : c & 1];
-      uint32_t out[16];
-      if constexpr (!kHold) {
-        tmem_ld_wait();
-        if (c < 3) tmem_ld32(tmem_s + 32 * (c + 1), s[(c + 1) & 1]);
-        scaled<TAIL>(v, ks + 32 * c, seen[c]);
-      }
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t sees = TAIL ? (c0 == 0 ? seen[y] : seen[2 + y]) : kFull;
+        uint32_t(&v)[32] = s[y];
+        uint32_t out[16];
+        scaled<TAIL>(v, ks + 32 * (c0 + y), sees);
 #pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        const unsigned long long xa = fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), q2, m2);
-        const unsigned long long xb = fma2(pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), q2, m2);
-        float2 ea = unpair(xa), eb;
-        ea = make_float2(exp2_fast(ea.x), exp2_fast(ea.y));
-        if ((i / 4) % 4 < kPolyOf4) {
-          eb = exp2_pair(xb);
-        } else {
-          eb = unpair(xb);
-          eb = make_float2(exp2_fast(eb.x), exp2_fast(eb.y));
-        }
-        float e[4] = {ea.x, ea.y, eb.x, eb.y};
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          if (TAIL && !((seen[c] >> (i + x)) & 1)) e[x] = 0.0f;  // a scale of 0 makes -inf NaN
-        }
-        unsigned long long a = pair(e[0], e[1]), b = pair(e[2], e[3]);
-        sum0 = add2(sum0, a), sum1 = add2(sum1, b);
-        if constexpr (C::TOKEN) {
-          const float4 vv = *reinterpret_cast<const float4*>(vs + 32 * c + i);
-          a = mul2(a, mul2(pair(vv.x, vv.y), i2)), b = mul2(b, mul2(pair(vv.z, vv.w), i2));
-          const float2 fa = unpair(a), fb = unpair(b);
-          e[0] = fa.x, e[1] = fa.y, e[2] = fb.x, e[3] = fb.y;
+        for (int i = 0; i < 32; i += 4) {
+          const float2 xa = unpair(fma2(pair(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), q2, m2));
+          const float2 xb = unpair(fma2(pair(__uint_as_float(v[i + 2]), __uint_as_float(v[i + 3])), q2, m2));
+          float e[4] = {exp2_fast(xa.x), exp2_fast(xa.y), exp2_fast(xb.x), exp2_fast(xb.y)};
           if (TAIL) {
 #pragma unroll
             for (int x = 0; x < 4; ++x)
-              if (!((seen[c] >> (i + x)) & 1)) e[x] = 0.0f;  // an unseen scale may be anything
+              if (!((sees >> (i + x)) & 1)) e[x] = 0.0f;  // a scale of 0 makes -inf NaN
           }
+          unsigned long long a = pair(e[0], e[1]), b = pair(e[2], e[3]);
+          sum0 = add2(sum0, a), sum1 = add2(sum1, b);
+          if constexpr (C::TOKEN) {
+            const float4 vv = *reinterpret_cast<const float4*>(vs + 32 * (c0 + y) + i);
+            a = mul2(a, mul2(pair(vv.x, vv.y), i2)), b = mul2(b, mul2(pair(vv.z, vv.w), i2));
+            const float2 fa = unpair(a), fb = unpair(b);
+            e[0] = fa.x, e[1] = fa.y, e[2] = fb.x, e[3] = fb.y;
+            if (TAIL) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x)
+                if (!((sees >> (i + x)) & 1)) e[x] = 0.0f;  // an unseen scale may be anything
+            }
+          }
+          out[i / 2] = pack2<C::BF16>(e[0], e[1]);
+          out[i / 2 + 1] = pack2<C::BF16>(e[2], e[3]);
         }
-        out[i / 2] = pack2<C::BF16>(e[0], e[1]);
-        out[i / 2 + 1] = pack2<C::BF16>(e[2], e[3]);
+        // over the scores 16 c .. 16 c + 15, which have been read
+        tmem_st16(tmem_s + 16 * (c0 + y), out);
       }
-      // over the scores 16 c .. 16 c + 15, which have been read
-      tmem_st16(tmem_s + 16 * c, out);
     }
     const float2 sa = unpair(add2(sum0, sum1));
     l += sa.x + sa.y;
@@ -851,8 +806,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
         return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
       },
       red, total, unit, b0, before);
-  const int count = min(share, total - unit), offset = unit - before;
-  const bool busy = unit < total;
+  const Run run = {b0, before, unit, min(share, total - unit)};
 
   clear_idle_requests<C::kThreads>(p, D);
   tc_fence_before();
@@ -862,23 +816,27 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
   const uint32_t q_addr = base + C::kOffQ;
 
   Loader<C> ld{p, bars, base, mem, q_addr + C::q_bytes(nq), nq, C::raw_depth(nq), warp - kSoftWarps, lane, abort};
+  bool busy = unit < total;
+  if (busy) {  // a run may lie in front of its item's first key
+    Pieces any;
+    busy = any.start(p, run.b0, run.before, run.unit, run.count);
+  }
   if (!busy) {
-    // fewer units than blocks
+    if (tid == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
   } else if (warp >= kSoftWarps && warp < kSoftWarps + C::kLoadWarps) {
     // ------------------------------------------------ loaders
     regs_down<C::kLoadRegs>();
     if constexpr (C::kSmall)
-      ld.run_widen(b0, offset, count);
+      ld.run_widen(run);
     else
-      ld.run_copies(b0, offset, count);
+      ld.run_copies(run);
   } else if (warp >= kSoftWarps + C::kLoadWarps) {
     // ------------------------------------------------ products
-    regs_down<C::kIssueRegs>();
     if (warp == C::kWarps - 4) {
       // the whole warp walks the tiles, one lane issues: addresses stay in uniform registers
       const bool leader = elect_one();
       Pieces pc;
-      pc.start(p, b0, offset, count);
+      pc.start(p, run.b0, run.before, run.unit, run.count);
       const int lead = nq == 1 ? 2 : 1;
       uint32_t kv = 0, piece = 0, pp0 = 0, pp1 = 0;  // tiles taken, pieces, probabilities taken
       const uint32_t q16 = q_addr >> 4, kv16 = base >> 4;
@@ -955,9 +913,9 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       for (uint32_t n = 0; n < (1u << 22) && !mbar_try_wait(&bars->drain, 0); ++n) {
       }
     } else if (C::kSmall && warp < C::kWarps - 1) {
-      ld.run_fetch(warp == C::kWarps - 2, b0, offset, count);
+      ld.run_fetch(warp == C::kWarps - 2, run);
     } else if (C::TOKEN) {
-      ld.run_scales(b0, offset, count);
+      ld.run_scales(run);
     }
   } else if (warp < kSoftWarps) {
     // ------------------------------------------------ softmax and output
@@ -976,7 +934,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
     };
     const int lead = nq == 1 ? 2 : 1;
     Pieces pc;
-    pc.start(p, b0, offset, count);
+    pc.start(p, run.b0, run.before, run.unit, run.count);
     // the thread's row of a piece, and its queries
     struct Row {
       int h, qi, head, t;
@@ -984,22 +942,23 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       const uint8_t* q;
     };
     auto row_of = [&](const Pieces& at) {
-      const int rts = row_tiles(p, at.w.r), rows = at.w.r.n * p.group;
+      const int rts = row_tiles(p, at.r), rows = at.r.n * p.group;
       Row o;
-      o.h = at.w.item / rts;
-      const int row = ((at.w.item - o.h * rts) << p.rows_log2) + (nq == 1 ? 0 : x * kTile) + wrow;
+      o.h = at.item / rts;
+      const int row = ((at.item - o.h * rts) << p.rows_log2) + (nq == 1 ? 0 : x * kTile) + wrow;
       o.ok = row < rows;
       o.warp_ok = row - lane < rows;
       o.qi = row / p.group;
       o.head = o.h * p.group + row - o.qi * p.group;
-      o.t = at.w.r.first + o.qi;
+      o.t = at.r.first + o.qi;
       o.q = static_cast<const uint8_t*>(p.q) + (o.t * p.q_tok + o.head * p.q_head) * 2;
       return o;
     };
     bool ok = true, more = true;
+    int4 join = make_int4(0, 0, 0, 0);
     Row me = row_of(pc);
     do {
-      const Request r = pc.w.r;
+      const Request r = pc.r;
       const int h = me.h, qi = me.qi, head = me.head, t = me.t;
       const bool row_ok = me.ok, warp_ok = me.warp_ok;
       so.begin();
@@ -1063,9 +1022,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       if (!ok) break;
 
       // ---- end of the run: outputs, or partial sums where the item goes on in another block
-      const bool whole = pc.tile0 == 0 && pc.nt == pc.w.tiles;
+      const bool whole = pc.tile0 == 0 && pc.nt == pc.tiles;
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + (pc.tile0 == 0 ? 1 : 0)) << p.rows_log2;
       const bool two = nq == 1 && pc.nt > 1;  // both streams hold sums of these rows
+      if (tid == 0 && !whole && pc.tile0 == 0)
+        join = make_int4(parts_of(p, pc, share), pc.b, pc.item, 0);
       kv += 2 * pc.nt;
       t0 += pc.nt;
       more = pc.next(p);
@@ -1186,6 +1147,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
         if (!ok) break;
       }
     } while (more);
+    if (tid == 0) p.joins[blockIdx.x] = join;
   }
 
   tc_fence_before();
@@ -1226,6 +1188,7 @@ orError_t launch_tc(Params& p, int D, long long rows, cudaStream_t st, int sms, 
   const int nq = rows <= tc::kTile ? 1 : 2;
   p.rows_log2 = nq == 1 ? 7 : 8;
   p.keys_log2 = 7;
+  p.item_cost = nq == 1 ? ECOST1 : ECOST2;
   p.min_share = 1;
   *grid = sms;
   return D == 64 ? tc::pick<64>(p, nq, st, sms) : tc::pick<128>(p, nq, st, sms);
