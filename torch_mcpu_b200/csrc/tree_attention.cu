@@ -32,15 +32,6 @@
 
 #include "tree_attention.cuh"
 
-#ifndef ECOST
-#define ECOST 2
-#endif
-#ifndef DMIN
-#define DMIN 2
-#endif
-#ifndef MINSHARE
-#define MINSHARE 2
-#endif
 namespace mcpu {
 namespace attn {
 
@@ -202,7 +193,7 @@ __device__ __forceinline__ bool any_wild(const uint8_t* values) {
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(kThreads, DMIN) attend_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ Params p) {
   constexpr int D = C::D, KW = C::KW, KIND = C::KIND;
   constexpr int kNT = KW / 8;   // 8-key tiles of the scores
   constexpr int kDT = D / 8;    // 8-dimension tiles of the output
@@ -734,8 +725,8 @@ orError_t launch(Params& p, cudaStream_t st, int sms, int* grid) {
   *grid = resident * sms;
   p.rows_log2 = 4;
   p.keys_log2 = C::TN == 64 ? 6 : 7;
-  p.item_cost = ECOST;
-  p.min_share = MINSHARE;
+  p.item_cost = 2;
+  p.min_share = 2;
   attend_kernel<T, C><<<*grid, kThreads, C::kSmem, st>>>(p);
   return from_cuda(cudaGetLastError(), "tree_attention launch");
 }
