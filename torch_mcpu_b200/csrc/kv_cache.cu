@@ -52,8 +52,10 @@ struct Rows {
 
 struct Params {
   long long tokens;
-  int q_heads, kv_heads, D, R, lanes_log2, neox;
-  long long rows_per_block;
+  int q_heads, kv_heads, D, R, neox;
+  int turn_log2, lanes_log2;  // lanes of a row: where only its rotated part counts, and of a whole row
+  int turn_blocks;            // blockIdx.y below it: rows that are rotated in place; from it on: rows for the cache
+  int turn_rows, cache_rows;  // rows of a token that a block takes
   Rows q, k, v;  // q (and k without a cache) is written in place
   const long long* positions;
   const float* table;  // [max_position, R]: R/2 cosines, R/2 sines
@@ -90,36 +92,59 @@ __device__ __forceinline__ float to_odd(double v) {
   return f;
 }
 
-// Out of line: the common path keeps its registers.
+// a*c - b*s rounded once to T (as its fp32 value), in 64 bits; out of line: the
+// common path keeps its registers.
 template <typename T>
 __device__ __noinline__ float rotate_exact(float a, float c, float b, float s) {
   const double bs = static_cast<double>(b) * static_cast<double>(s);
   return up<T>(down<T>(to_odd(static_cast<double>(a) * static_cast<double>(c) - bs)));
 }
 
-// a*c - b*s (or + with s negated) rounded once to T, as its fp32 value.
+// Distance of r to the border between two neighbours of T that its bits lie
+// next to: the dropped bits replaced by 100..0.
 template <typename T>
-__device__ __forceinline__ float rotate(float a, float c, float b, float s) {
-  const float p = __fmul_rn(b, s);
-  const float r = __fmaf_rn(a, c, -p);
-  if constexpr (sizeof(T) == 4) {
-    return r;
-  } else {
-    // |r - exact| <= 2^-24 (|p| + |r|).  The border of T that r's bits fall
-    // next to: the dropped bits replaced by 100..0.
-    constexpr bool kBf16 = sizeof(T) == 2 && static_cast<int>(std::is_same<T, __nv_bfloat16>::value);
-    constexpr uint32_t kDropped = kBf16 ? 0xFFFFu : 0x1FFFu;
-    const uint32_t u = __float_as_uint(r);
-    const float border = __uint_as_float((u & ~kDropped) | ((kDropped + 1) >> 1));
-    const float mag = fabsf(p) + fabsf(r);
-    bool near = fabsf(r - border) <= mag * 1.1920929e-7f;  // 2^-23: twice the bound
-    if constexpr (kBf16)
-      near = near || fabsf(r) < 1e-30f;  // products that may have lost bits to underflow
-    else
-      near = near || fabsf(r) < 6.2e-5f;  // fp16 subnormals: their borders lie elsewhere
-    if (near) return rotate_exact<T>(a, c, b, s);
-    return up<T>(down<T>(r));
+__device__ __forceinline__ float to_border(float r) {
+  constexpr uint32_t kDropped = std::is_same<T, __nv_bfloat16>::value ? 0xFFFFu : 0x1FFFu;
+  return fabsf(r - __uint_as_float((__float_as_uint(r) & ~kDropped) | ((kDropped + 1) >> 1)));
+}
+
+// One pair in fp32, and how far its results lie from a border of T beyond
+// their error (<= 0: the rounding is not sure).  amp: 2^-23 times the largest
+// |cos|, |sin|; the error of a result is at most 2^-24 (|b s| + |result|) <=
+// amp (|a| + |b|).
+template <typename T>
+struct Pair {
+  float a, b, da, db, e;
+  __device__ __forceinline__ Pair(float x, float y, float c, float s, float amp) {
+    a = __fmaf_rn(x, c, -__fmul_rn(y, s));
+    b = __fmaf_rn(y, c, __fmul_rn(x, s));
+    if constexpr (sizeof(T) == 2) {
+      e = __fmaf_rn(fabsf(x) + fabsf(y), amp, 1e-35f);  // 1e-35: products that lost bits to underflow
+      da = to_border<T>(a), db = to_border<T>(b);
+      if constexpr (std::is_same<T, __half>::value) {  // subnormal results have their borders elsewhere
+        if (fabsf(a) < 6.2e-5f) da = 0.0f;
+        if (fabsf(b) < 6.2e-5f) db = 0.0f;
+      }
+    }
   }
+  __device__ __forceinline__ bool unsure() const { return sizeof(T) == 2 && (da <= e || db <= e); }
+};
+// Whether any of four pairs is unsure: a chain of comparisons into one
+// predicate, which the compiler does not make of the plain expression.
+template <typename T>
+__device__ __forceinline__ uint32_t any_unsure(const Pair<T>& p0, const Pair<T>& p1, const Pair<T>& p2, const Pair<T>& p3) {
+  if constexpr (sizeof(T) == 4) return 0;
+  uint32_t r;
+  asm("{\n\t.reg .pred p;\n\t"
+      "setp.le.f32 p, %1, %3;\n\tsetp.le.or.f32 p, %2, %3, p;\n\t"
+      "setp.le.or.f32 p, %4, %6, p;\n\tsetp.le.or.f32 p, %5, %6, p;\n\t"
+      "setp.le.or.f32 p, %7, %9, p;\n\tsetp.le.or.f32 p, %8, %9, p;\n\t"
+      "setp.le.or.f32 p, %10, %12, p;\n\tsetp.le.or.f32 p, %11, %12, p;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "f"(p0.da), "f"(p0.db), "f"(p0.e), "f"(p1.da), "f"(p1.db), "f"(p1.e), "f"(p2.da), "f"(p2.db), "f"(p2.e), "f"(p3.da),
+        "f"(p3.db), "f"(p3.e));
+  return r;
 }
 
 __device__ __forceinline__ float max_nan(float a, float b) {
@@ -128,63 +153,70 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// The two 8-bit forms of x / s, rounded once.  inv = 1 / s (one rounding), so
-// x * inv is within 2^-23 of x / s; usable where s is far from underflow.
-struct Scale {
-  float s, inv;
-  bool plain;  // fp32 arithmetic is safe
-  __device__ __forceinline__ explicit Scale(float v)
-      : s(v), inv(1.0f / v), plain(!(v < 1e-30f) && v < 1e30f) {}
-};
+// rn(m / top) for a row's maximum.  One multiplication, then the remainder
+// (exact in a fused multiply-add) corrects it; out of range: a division.
+__device__ __forceinline__ float scale_of(float m, float top, float inv_top) {
+  const float q = m * inv_top;
+  const float r = __fmaf_rn(__fmaf_rn(-q, top, m), inv_top, q);
+  return m > 1e-30f && m < 1e30f ? r : __fdiv_rn(m, top);
+}
 
+// rn(x / s) in 64 bits, as the fp32 value that converts to it.
 template <int KIND>
 __device__ __noinline__ float quotient_exact(float x, float s) {
+  if (s == 0.0f) return 0.0f;  // a row of zeros
+  if (!(fabsf(x) <= 3.4028235e38f) || !(s <= 3.4028235e38f)) {  // infinities, NaN: as the division has it
+    const float t = x / s;
+    return KIND == kInt8 ? fminf(fmaxf(t == t ? t : 0.0f, -127.0f), 127.0f) : t;
+  }
   const double y = static_cast<double>(x) / static_cast<double>(s);
   if (KIND == kInt8) return static_cast<float>(rint(fmin(fmax(y, -127.0), 127.0)));
   return to_odd(fmin(fmax(y, -448.0), 448.0));
 }
 
-// fp32 value whose conversion to the 8-bit type gives the rounding of x / s.
+// x * inv (inv = 1 / s within an ulp, so x / s within 4) and whether its
+// rounding to the 8-bit type is not sure.
 template <int KIND>
-__device__ __forceinline__ float quotient(float x, const Scale& sc) {
-  float t = x * sc.inv;
-  if (sc.s == 0.0f) return 0.0f;  // a row of zeros
-  bool near;
+__device__ __forceinline__ bool quotient(float x, float inv, float& t) {
+  t = x * inv;
   if constexpr (KIND == kE4M3) {
-    // above 2^-6 e4m3 keeps 3 bits of the fraction; below it is subnormal
-    const uint32_t u = __float_as_uint(t);
-    const float border = __uint_as_float((u & 0xFFF00000u) | 0x80000u);
-    near = fabsf(t - border) <= fabsf(t) * 2.3841858e-7f || (fabsf(t) < 0.015625f && t != 0.0f);
+    // above 2^-6 e4m3 keeps 3 bits of the fraction: 20 bits of fp32 are dropped; below it is subnormal
+    return ((__float_as_uint(t) + 0x80000u + 8u) & 0xFFFFFu) <= 16u || !(fabsf(t) >= 0.015625f);
   } else {
-    t = fminf(fmaxf(t == t ? t : 0.0f, -127.0f), 127.0f);
     const float q = rintf(t);
-    near = fabsf(t - q) > 0.49996f;
-    t = q;
+    const bool near = !(fabsf(t - q) < 0.49996f);  // NaN and infinity too
+    t = fminf(fmaxf(q, -127.0f), 127.0f);
+    return near;
   }
-  if ((near || !sc.plain) && x == x && fabsf(x) <= 3.4028235e38f && sc.s == sc.s && fabsf(sc.s) <= 3.4028235e38f)
-    return quotient_exact<KIND>(x, sc.s);
-  return t;
 }
 
-// 8 values -> 8 bytes.
+// 8 values -> 8 bytes, each rounded once.  plain: s is far from underflow.
 template <int KIND>
-__device__ __forceinline__ uint2 quantise8(const float (&x)[8], const Scale& sc) {
+__device__ __forceinline__ uint2 quantise8(const float (&x)[8], float s, float inv, bool plain) {
+  float t[8];
+  bool near = !plain;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) near |= quotient<KIND>(x[i], inv, t[i]);
+  if (near) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float again;
+      if (!plain || quotient<KIND>(x[i], inv, again)) t[i] = quotient_exact<KIND>(x[i], s);
+    }
+  }
   uint32_t w[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    float t[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t[i] = quotient<KIND>(x[4 * h + i], sc);
     if constexpr (KIND == kE4M3) {
       uint16_t lo, hi;  // the first source goes to the upper byte; saturates, NaN stays NaN
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(t[1]), "f"(t[0]));
-      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(t[3]), "f"(t[2]));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(t[4 * h + 1]), "f"(t[4 * h]));
+      asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(t[4 * h + 3]), "f"(t[4 * h + 2]));
       w[h] = static_cast<uint32_t>(lo) | static_cast<uint32_t>(hi) << 16;
     } else {
       // whole numbers: adding 1.5 * 2^23 leaves them in the low bits
       uint32_t b[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(t[i] + 12582912.0f);
+      for (int i = 0; i < 4; ++i) b[i] = __float_as_uint(t[4 * h + i] + 12582912.0f);
       w[h] = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
     }
   }
@@ -192,6 +224,28 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], const Scale& sc)
 }
 
 // ---------------------------------------------------------------- 8 values at a time
+// As loaded: so that a thread's next loads are under way while it works.
+template <typename T, bool VEC>
+struct Raw8 {
+  static constexpr int kWords = VEC ? sizeof(T) / 2 : 1;  // 16 bytes each
+  uint4 w[kWords];
+  T e[VEC ? 1 : 8];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (VEC) {
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = p[i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const T* t = VEC ? reinterpret_cast<const T*>(w) : e;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = up<T>(t[i]);
+  }
+};
+
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* p, float (&x)[8]) {
   if constexpr (!VEC) {
@@ -225,118 +279,175 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8]) {  // x alread
   }
 }
 
-// One block walks tokens; its threads are split into groups of 2^lanes_log2
-// lanes, one row (head) each.  gridDim.y splits a token's rows where there are
-// too few tokens to fill the GPU.
+// The 8 pairs of a thread's 16 values, rotated and rounded to T: in the half
+// layout x0[i] with x1[i], in the interleaved one neighbours.
+template <typename T>
+__device__ __forceinline__ void rotate16(float (&x0)[8], float (&x1)[8], const float (&cs)[8], const float (&sn)[8],
+                                         float amp, bool neox) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {  // four pairs at a time
+    float a[4], b[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float(&y)[8] = h ? x1 : x0;
+      a[i] = neox ? x0[4 * h + i] : y[2 * i];
+      b[i] = neox ? x1[4 * h + i] : y[2 * i + 1];
+    }
+    const float *c = cs + 4 * h, *s = sn + 4 * h;
+    const Pair<T> p0(a[0], b[0], c[0], s[0], amp), p1(a[1], b[1], c[1], s[1], amp);
+    const Pair<T> p2(a[2], b[2], c[2], s[2], amp), p3(a[3], b[3], c[3], s[3], amp);
+    float ra[4] = {p0.a, p1.a, p2.a, p3.a}, rb[4] = {p0.b, p1.b, p2.b, p3.b};
+    if (any_unsure<T>(p0, p1, p2, p3)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (!Pair<T>(a[i], b[i], c[i], s[i], amp).unsure()) continue;
+        ra[i] = rotate_exact<T>(a[i], c[i], b[i], s[i]);
+        rb[i] = rotate_exact<T>(b[i], c[i], a[i], -s[i]);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float(&y)[8] = h ? x1 : x0;
+      (neox ? x0[4 * h + i] : y[2 * i]) = ra[i];
+      (neox ? x1[4 * h + i] : y[2 * i + 1]) = rb[i];
+    }
+  }
+}
+
+// One block walks tokens; its threads are split into groups of lanes, one row
+// (head) each.  gridDim.y: blocks for the rows that are rotated in place (only
+// the rotated part of a row has lanes), then blocks for the cache's rows.
 template <typename T, int CACHE, bool ROPE, bool VEC>
-__global__ void __launch_bounds__(kThreads) rows_kernel(const __grid_constant__ Params p) {
-  const int lanes = 1 << p.lanes_log2;
-  const int g = threadIdx.x & (lanes - 1), slot_in_block = threadIdx.x >> p.lanes_log2;
-  const int groups = kThreads >> p.lanes_log2;
-  const bool active = g < p.D / 16;
+__global__ void __launch_bounds__(kThreads, 8) rows_kernel(const __grid_constant__ Params p) {
+  const bool turning = ROPE && static_cast<int>(blockIdx.y) < p.turn_blocks;
+  const int lanes_log2 = turning ? p.turn_log2 : p.lanes_log2;
+  const int lanes = 1 << lanes_log2, groups = kThreads >> lanes_log2;
+  const int g = threadIdx.x & (lanes - 1), slot_in_block = threadIdx.x >> lanes_log2;
+  const bool active = g < (turning ? p.R : p.D) / 16;
   const bool turns = ROPE && g < p.R / 16;
   // where this thread's 16 values lie in a row
   int at0 = 16 * g, at1 = 16 * g + 8;
   if (ROPE && p.neox && turns) at0 = 8 * g, at1 = 8 * g + p.R / 2;
-  const int q_rows = ROPE ? p.q_heads : 0;
-  const int rows = q_rows + p.kv_heads + (CACHE == kNoCache ? 0 : p.kv_heads);
-  const int row0 = static_cast<int>(blockIdx.y * p.rows_per_block);
-  const int row1 = min(rows, static_cast<int>(row0 + p.rows_per_block));
+  const int rows = turning ? p.q_heads + (CACHE == kNoCache ? p.kv_heads : 0) : 2 * p.kv_heads;
+  const int row0 = turning ? blockIdx.y * p.turn_rows : (blockIdx.y - p.turn_blocks) * p.cache_rows;
+  const int row1 = min(rows, row0 + (turning ? p.turn_rows : p.cache_rows));
   for (long long t = blockIdx.x; t < p.tokens; t += gridDim.x) {
-    float cs[8], sn[8];
+    float cs[8], sn[8], amp = 0.0f;
     bool rope_ok = true;
     if constexpr (ROPE) {
       const long long pos = p.positions[t];
       rope_ok = pos >= 0 && pos < p.max_position;
-      if (!rope_ok && g == 0 && slot_in_block == 0) atomicOr(&g_kv_error, 1);
+      if (!rope_ok && threadIdx.x == 0) atomicOr(&g_kv_error, 1);
       if (turns && rope_ok) {
         const float* row = p.table + pos * p.R + 8 * g;
         load8<float, true>(row, cs);
         load8<float, true>(row + p.R / 2, sn);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) amp = fmaxf(amp, fmaxf(fabsf(cs[i]), fabsf(sn[i])));
+        amp *= 1.1920929e-7f;
       }
     }
-    long long block = 0, inside = 0;
-    bool cached = false;
+    if (turning) {
+      if (!rope_ok || !active) continue;
+      auto row_at = [&](int r) {
+        const Rows& src = r < p.q_heads ? p.q : p.k;
+        return reinterpret_cast<T*>(const_cast<void*>(src.in)) + t * src.tok_stride +
+               (r < p.q_heads ? r : r - p.q_heads) * src.head_stride;
+      };
+      int r = row0 + slot_in_block;
+      if (r >= row1) continue;
+      T* x = row_at(r);
+      Raw8<T, VEC> in0, in1;
+      in0.load(x + at0);
+      in1.load(x + at1);
+      while (true) {  // the next row's loads are under way while this one is rotated
+        float x0[8], x1[8];
+        in0.get(x0);
+        in1.get(x1);
+        T* to = x;
+        const bool more = (r += groups) < row1;
+        if (more) {
+          x = row_at(r);
+          in0.load(x + at0);
+          in1.load(x + at1);
+        }
+        if (p.neox)
+          rotate16<T>(x0, x1, cs, sn, amp, true);
+        else
+          rotate16<T>(x0, x1, cs, sn, amp, false);
+        store8<T, VEC>(to + at0, x0);
+        store8<T, VEC>(to + at1, x1);
+        if (!more) break;
+      }
+      continue;
+    }
     if constexpr (CACHE != kNoCache) {
-      const long long s = p.slots[t];
-      if (s >= 0) {  // negative: a padded token, nothing is written
-        block = s / p.c.block_size;
-        inside = s - block * p.c.block_size;
-        cached = block < p.c.num_blocks && rope_ok;
-        if (block >= p.c.num_blocks && g == 0 && slot_in_block == 0) atomicOr(&g_kv_error, 1);
+      const long long at = p.slots[t];
+      if (at < 0 || !rope_ok) continue;  // negative: a padded token, nothing is written
+      const long long block = at / p.c.block_size, inside = at - block * p.c.block_size;
+      if (block >= p.c.num_blocks) {
+        if (threadIdx.x == 0) atomicOr(&g_kv_error, 1);
+        continue;
       }
-    }
-    for (int base = row0; base < row1; base += groups) {  // every lane takes every turn: the maxima are shuffled
-      const int r = base + slot_in_block;
-      const bool is_q = r < q_rows;
-      const bool is_k = !is_q && r < q_rows + p.kv_heads;
-      const bool here = r < row1 && active && (is_q ? rope_ok : CACHE == kNoCache ? rope_ok : cached);
-      const int h = is_q ? r : is_k ? r - q_rows : r - q_rows - p.kv_heads;
-      float x0[8], x1[8];
-      const Rows& src = is_q ? p.q : is_k ? p.k : p.v;
-      T* in = reinterpret_cast<T*>(const_cast<void*>(src.in)) + t * src.tok_stride + h * src.head_stride;
-      if (here) {
-        load8<T, VEC>(in + at0, x0);
-        load8<T, VEC>(in + at1, x1);
-        if (ROPE && turns && (is_q || is_k)) {
-          if (p.neox) {
+      Raw8<T, VEC> in0, in1;
+      auto fetch = [&](int r) {
+        if (r >= row1 || !active) return;
+        const Rows& src = r < p.kv_heads ? p.k : p.v;
+        const T* in = static_cast<const T*>(src.in) + t * src.tok_stride + (r < p.kv_heads ? r : r - p.kv_heads) * src.head_stride;
+        in0.load(in + at0);
+        in1.load(in + at1);
+      };
+      fetch(row0 + slot_in_block);
+      for (int base = row0; base < row1; base += groups) {  // every lane takes every turn: the maxima are shuffled
+        const int r = base + slot_in_block;
+        const bool is_k = r < p.kv_heads;
+        const bool here = r < row1 && active;
+        const int h = is_k ? r : r - p.kv_heads;
+        const int64_t* st = is_k ? p.c.key_stride : p.c.value_stride;
+        const long long to = block * st[0] + inside * st[1] + h * st[2];
+        float x0[8], x1[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const float a = x0[i], b = x1[i];
-              x0[i] = rotate<T>(a, cs[i], b, sn[i]);
-              x1[i] = rotate<T>(b, cs[i], a, -sn[i]);
-            }
-          } else {
+        for (int i = 0; i < 8; ++i) x0[i] = x1[i] = 0.0f;
+        if (here) {
+          in0.get(x0);
+          in1.get(x1);
+          fetch(r + groups);
+          if (ROPE && turns && is_k) {
+            if (p.neox)
+              rotate16<T>(x0, x1, cs, sn, amp, true);
+            else
+              rotate16<T>(x0, x1, cs, sn, amp, false);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float a = x0[2 * i], b = x0[2 * i + 1];
-              x0[2 * i] = rotate<T>(a, cs[i], b, sn[i]);
-              x0[2 * i + 1] = rotate<T>(b, cs[i], a, -sn[i]);
-              a = x1[2 * i], b = x1[2 * i + 1];
-              x1[2 * i] = rotate<T>(a, cs[4 + i], b, sn[4 + i]);
-              x1[2 * i + 1] = rotate<T>(b, cs[4 + i], a, -sn[4 + i]);
-            }
+            for (int i = 0; i < 8; ++i) x0[i] = up<T>(down<T>(x0[i])), x1[i] = up<T>(down<T>(x1[i]));
           }
         }
-      }
-      if (CACHE == kNoCache || is_q) {
-        if (here && turns) {
-          store8<T, VEC>(in + at0, x0);
-          store8<T, VEC>(in + at1, x1);
-        }
-      }
-      if constexpr (CACHE == kSame) {
-        if (here && !is_q) {
-          const int64_t* st = is_k ? p.c.key_stride : p.c.value_stride;
-          T* out = static_cast<T*>(is_k ? p.c.key : p.c.value) + block * st[0] + inside * st[1] + h * st[2];
-          store8<T, true>(out + at0, x0);
-          store8<T, true>(out + at1, x1);
-        }
-      }
-      if constexpr (CACHE == kE4M3 || CACHE == kInt8) {
-        if (__any_sync(kFull, here && !is_q)) {
-          const bool is_kv = here && !is_q;
+        if constexpr (CACHE == kSame) {
+          if (here) {
+            T* out = static_cast<T*>(is_k ? p.c.key : p.c.value) + to;
+            store8<T, true>(out + at0, x0);
+            store8<T, true>(out + at1, x1);
+          }
+        } else {
           const int64_t* ss = is_k ? p.c.k_scale_stride : p.c.v_scale_stride;
           float* scale = (is_k ? p.c.k_scale : p.c.v_scale) + block * ss[0] + inside * ss[1] + h * ss[2];
-          float s = 0.0f;
+          float s = 1.0f;
           if (p.c.scale_mode == MCPU_KV_SCALE_TOKEN) {
             float m = 0.0f;
-            if (is_kv) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) m = max_nan(m, max_nan(fabsf(x0[i]), fabsf(x1[i])));
-            }
+            for (int i = 0; i < 8; ++i) m = max_nan(m, max_nan(fabsf(x0[i]), fabsf(x1[i])));
             for (int o = lanes >> 1; o > 0; o >>= 1) m = max_nan(m, __shfl_xor_sync(kFull, m, o));
-            s = __fdiv_rn(m, CACHE == kE4M3 ? 448.0f : 127.0f);
-            if (is_kv && g == 0) *scale = s;
-          } else if (is_kv) {
+            s = CACHE == kE4M3 ? scale_of(m, 448.0f, 1.0f / 448.0f) : scale_of(m, 127.0f, 1.0f / 127.0f);
+            if (here && g == 0) *scale = s;
+          } else if (here) {
             s = *scale;
           }
-          if (is_kv) {
-            const Scale sc(s);
-            const int64_t* st = is_k ? p.c.key_stride : p.c.value_stride;
-            uint8_t* out = static_cast<uint8_t*>(is_k ? p.c.key : p.c.value) + block * st[0] + inside * st[1] + h * st[2];
-            *reinterpret_cast<uint2*>(out + at0) = quantise8<CACHE>(x0, sc);
-            *reinterpret_cast<uint2*>(out + at1) = quantise8<CACHE>(x1, sc);
+          if (here) {
+            float inv;
+            asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+            const bool plain = s > 1e-30f && s < 1e30f;
+            uint8_t* out = static_cast<uint8_t*>(is_k ? p.c.key : p.c.value) + to;
+            *reinterpret_cast<uint2*>(out + at0) = quantise8<CACHE>(x0, s, inv, plain);
+            *reinterpret_cast<uint2*>(out + at1) = quantise8<CACHE>(x1, s, inv, plain);
           }
         }
       }
@@ -367,8 +478,10 @@ __global__ void __launch_bounds__(kThreads) pairs_kernel(const __grid_constant__
       T* pb = x + (p.neox ? d + half : 2 * d + 1);
       const float a = up<T>(*pa), b = up<T>(*pb);
       const float c = p.table[pos * p.R + d], s = p.table[pos * p.R + half + d];
-      *pa = down<T>(rotate<T>(a, c, b, s));
-      *pb = down<T>(rotate<T>(b, c, a, -s));
+      const Pair<T> r2(a, b, c, s, 1.1920929e-7f * fmaxf(fabsf(c), fabsf(s)));
+      const bool again = r2.unsure();
+      *pa = down<T>(again ? rotate_exact<T>(a, c, b, s) : r2.a);
+      *pb = down<T>(again ? rotate_exact<T>(b, c, a, -s) : r2.b);
     }
   }
 }
@@ -502,20 +615,27 @@ bool aligned(const Rows& r, int elem) {
 
 template <typename T, int CACHE, bool ROPE>
 orError_t launch_rows(Params& p, cudaStream_t st, const char* what) {
-  const int lanes_needed = p.D / 16;
-  p.lanes_log2 = 0;
-  while ((1 << p.lanes_log2) < lanes_needed) ++p.lanes_log2;
-  const int groups = kThreads >> p.lanes_log2;
-  const int rows = (ROPE ? p.q_heads : 0) + p.kv_heads + (CACHE == kNoCache ? 0 : p.kv_heads);
-  // Few tokens: one turn of the row loop per block, so a token's rows are in
-  // flight together; many: a block keeps a token's cosines for all its rows.
-  const long long fill = 16LL * sm_count();
-  long long parts = (rows + groups - 1) / groups;
-  if (p.tokens * parts > fill) parts = std::max<long long>(1, fill / p.tokens);
-  p.rows_per_block = (rows + parts - 1) / parts;
-  p.rows_per_block = (p.rows_per_block + groups - 1) / groups * groups;
-  const dim3 grid(static_cast<unsigned>(std::min<long long>(p.tokens, fill)),
-                  static_cast<unsigned>((rows + p.rows_per_block - 1) / p.rows_per_block));
+  auto log2_lanes = [](int values) {
+    int n = 0;
+    while ((16 << n) < values) ++n;
+    return n;
+  };
+  p.lanes_log2 = log2_lanes(p.D);
+  p.turn_log2 = log2_lanes(p.R);
+  // Few tokens: a block takes one turn of its threads, so that a token's rows are in flight together; many: a block keeps a
+  // token's cosines for as many rows as still leave blocks enough.
+  const long long fill = 8LL * sm_count();
+  auto split = [&](int rows, int groups, int& per) {
+    long long parts = (rows + groups - 1) / groups;
+    if (p.tokens * parts > fill) parts = std::max<long long>(1, fill / p.tokens);
+    per = static_cast<int>((rows + parts - 1) / parts);
+    per = (per + groups - 1) / groups * groups;
+    return (rows + per - 1) / per;
+  };
+  const int turn = !ROPE ? 0 : p.q_heads + (CACHE == kNoCache ? p.kv_heads : 0);
+  p.turn_blocks = turn ? split(turn, kThreads >> p.turn_log2, p.turn_rows) : 0;
+  const int cache_blocks = CACHE == kNoCache ? 0 : split(2 * p.kv_heads, kThreads >> p.lanes_log2, p.cache_rows);
+  const dim3 grid(static_cast<unsigned>(std::min<long long>(p.tokens, fill)), static_cast<unsigned>(p.turn_blocks + cache_blocks));
   const int elem = sizeof(T);
   bool vec = aligned(p.k, elem);
   if (ROPE) vec = vec && aligned(p.q, elem);

@@ -172,6 +172,7 @@ inline void rotary_embedding(const Api& api, const at::Tensor& positions, const 
   if (key) {
     k = heads_of(*key, head_size, op, "key");
     TORCH_CHECK(k.tokens == q.tokens, op, ": key has ", k.tokens, " tokens, query ", q.tokens);
+    TORCH_CHECK(key->numel() == 0 || key->data_ptr() != query.data_ptr(), op, ": query and key are written and must not overlap");
     disjoint<2>({Dim{k.token_stride, k.tokens}, Dim{k.head_stride, k.heads}}, part, op, "key");
   }
   ok(api,
