@@ -38,7 +38,7 @@ namespace attn {
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = 16;  // rows of a tile: a matrix instruction's
-constexpr int kJoinThreads = 256;  // 32 rows a block
+constexpr int kJoinThreads = 128;  // 16 rows a block
 
 // ---------------------------------------------------------------- instructions
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
@@ -193,7 +193,7 @@ __device__ __forceinline__ bool any_wild(const uint8_t* values) {
 }
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_constant__ Params p) {
+__global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p) {
   constexpr int D = C::D, KW = C::KW, KIND = C::KIND;
   constexpr int kNT = KW / 8;   // 8-key tiles of the scores
   constexpr int kDT = D / 8;    // 8-dimension tiles of the output
@@ -517,7 +517,7 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
     {
       const bool whole = pc.nt == pc.tiles;
       const int slot = pc.tile0 == 0 ? 1 : 0;
-      if (!whole && pc.tile0 == 0) join = make_int4(parts_of(p, pc, share), pc.b, pc.item, 0);
+      if (!whole && pc.tile0 == 0) join = make_int4(parts_of(p, pc, share), pc.r.first, pc.r.n, pc.item);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(kFull, l[e], 1);
@@ -602,11 +602,11 @@ __global__ void __launch_bounds__(kThreads, 2) attend_kernel(const __grid_consta
 // ---------------------------------------------------------------- joining kernel
 // Block c joins the one row tile that begins in the main kernel's block c and
 // goes on behind it: its parts lie in slot 1 of c and slot 0 of the next
-// blocks.  A block takes 32 of its rows, four to a warp; where there are fewer
+// blocks.  A block takes 16 of its rows, four to a warp; where there are fewer
 // rows, several warps share the parts of four and join theirs at the end, so
 // that a long sequence with few rows is not a chain of loads.
 template <typename T, int D>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(kJoinThreads, 8) join_kernel(const __grid_constant__ Params p) {
   constexpr int kJoinWarps = kJoinThreads / 32;
   __shared__ float4 sums[kJoinWarps][4][D / 4];
   __shared__ float2 sums_ml[kJoinWarps][4];
@@ -614,13 +614,13 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
   // every block waits, also those with nothing to join: what follows on the
   // stream must not overtake the main kernel
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 join = p.joins[c];  // parts, request, item
-  const int parts = join.x, item = join.z;
+  const int4 join = p.joins[c];
+  const int parts = join.x, item = join.w;
   if (parts == 0) return;
-  const Request r = request(p, join.y);
+  const Request r = {join.y, join.z, 0};
   const int rts = row_tiles(p, r);
   const int h = item / rts, rt = item - h * rts;
-  const int first = rt * rows + blockIdx.y * 32, left = min(rows - static_cast<int>(blockIdx.y) * 32, r.n * p.group - first);
+  const int first = rt * rows + blockIdx.y * (kJoinThreads / 8), left = min(rows - static_cast<int>(blockIdx.y) * (kJoinThreads / 8), r.n * p.group - first);
   if (left <= 0) return;
   int groups = 1;  // of four rows, a power of two up to the block's warps
   while (groups * 4 < left && groups < kJoinWarps) groups *= 2;
@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
       for (int i = 0; i < kAtOnce; ++i) {
         const int kk = k + y * step, row = row0 + i * kPerWarp;
         const bool in = row < left && kk < parts;
-        const long long at = ((static_cast<long long>(c) + kk) * 2 + (kk == 0 ? 1 : 0)) * rows + blockIdx.y * 32 + row;
+        const long long at = ((static_cast<long long>(c) + kk) * 2 + (kk == 0 ? 1 : 0)) * rows + blockIdx.y * (kJoinThreads / 8) + row;
         ml[y][i] = in ? *reinterpret_cast<const float2*>(p.part_ml + at * 2) : make_float2(-INFINITY, 0.0f);
         v[y][i] = in ? reinterpret_cast<const float4*>(p.part_o + at * D)[d] : make_float4(0.f, 0.f, 0.f, 0.f);
       }
@@ -726,7 +726,7 @@ orError_t launch(Params& p, cudaStream_t st, int sms, int* grid) {
   p.rows_log2 = 4;
   p.keys_log2 = C::TN == 64 ? 6 : 7;
   p.item_cost = 2;
-  p.min_share = 2;
+  p.min_share = 1;
   attend_kernel<T, C><<<*grid, kThreads, C::kSmem, st>>>(p);
   return from_cuda(cudaGetLastError(), "tree_attention launch");
 }
@@ -748,7 +748,7 @@ orError_t run(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, i
   const orError_t e = rows <= kRows ? launch_few<T, D>(p, dtype, st, sms, &grid) : launch_tc(p, D, rows, st, sms, &grid);
   if (e != orSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / 32));
+  cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / (kJoinThreads / 8)));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = st;
   cudaLaunchAttribute attr;

@@ -39,7 +39,8 @@ struct Params {
   int bf16;                  // type of query and out: bf16, else fp16
   float* part_o;             // [grid][2][rows][D]
   float* part_ml;            // [grid][2][rows][2]
-  int4* joins;               // [grid]: the row tile that begins in a block and goes on behind it
+  int4* joins;               // [grid]: of the row tile that begins in a block and goes on behind it: its parts (0: there
+                             // is none), its request's first token and new tokens, its item
 };
 
 // ---------------------------------------------------------------- schedule

@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + (pc.tile0 == 0 ? 1 : 0)) << p.rows_log2;
       const bool two = nq == 1 && pc.nt > 1;  // both streams hold sums of these rows
       if (tid == 0 && !whole && pc.tile0 == 0)
-        join = make_int4(parts_of(p, pc, share), pc.b, pc.item, 0);
+        join = make_int4(parts_of(p, pc, share), pc.r.first, pc.r.n, pc.item);
       kv += 2 * pc.nt;
       t0 += pc.nt;
       more = pc.next(p);
