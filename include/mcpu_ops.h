@@ -525,8 +525,10 @@ OPENREG_EXPORT orError_t mcpu_gather_cache(const mcpuKvCache* cache, const int32
  * slots behind seq_lens hold (NaN included) does not matter.  Tokens outside
  * every request are left as they are.  A request that does not fit (lengths
  * negative or falling, seq_lens[b] < n or beyond the block table, more tokens
- * than the mask has bits) gives zeros, one with a page outside the cache
+ * than max_query_len) gives zeros, or leaves its tokens as they are where
+ * cu_query_lens falls or passes num_tokens; one with a page outside the cache
  * reads block 0 instead; both set mcpu_device_error.
+ * The key and the value cache span at most 64 GB each.
  * workspace: mcpu_tree_attention_workspace_bytes bytes, 16-byte aligned, of
  * any content; calls that may run at the same time have one each.
  */
@@ -542,7 +544,7 @@ OPENREG_EXPORT orError_t mcpu_tree_attention_workspace_bytes(int64_t max_query_l
                                                              int head_size, uint64_t* bytes);
 
 /* *flag = 1 if a kernel on the current device (tensor-core GEMM, TMA-fed
- * router or bulk-copy-fed rms_norm) gave up on a bounded wait, or a gather /
+ * router, tree attention or bulk-copy-fed rms_norm) gave up on a bounded wait, or a gather /
  * scatter met an index out of range, since the last reset; that launch left
  * its output incomplete.  No counterpart in the reference, whose host
  * worker threads report hangs through orStreamSynchronize's timeout. */

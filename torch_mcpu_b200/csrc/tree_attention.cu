@@ -26,6 +26,15 @@
 // 8-bit caches are multiplied as fp16, which holds e4m3 and int8 values
 // exactly: the scales of the keys go onto the scores, those of the values onto
 // the probabilities.
+//
+// Which kernel.  Rows that share a key / value head = queries of the longest
+// request x query heads per key / value head.  Up to 8 and up to 16 rows: the
+// kernels of this file, which read each key once at the cost of one matrix
+// instruction a 16-key tile; the 8-row one is the faster where it applies (100
+// requests of up to 6000 tokens, 32 / 8 heads of 128: e4m3 152 us against 161,
+// int8 148 against 163, bf16 219 against 228).  More rows: tensor memory,
+// tree_attention_tc.cu, whose 128-row tile costs the same however many rows
+// of it are used, but which is the only one that keeps up with more than 16.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -89,10 +98,34 @@ __device__ __forceinline__ void mma_seen(float (&acc)[4], const uint32_t (&p)[4]
   }
 }
 
+// An 8 x 8 matrix of 16-bit values, transposed across the warp.
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// mma_seen with the values as the left operand.
+template <bool BF16>
+__device__ __forceinline__ void mma_seen_values(float (&acc)[4], const uint32_t (&v)[4], const uint32_t (&p)[2],
+                                                const uint32_t (&seen)[2]) {
+  uint32_t c[4], plus[4], minus[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) split_finite<BF16>(v[x], c[x], plus[x], minus[x]);
+  mma<BF16>(acc, c, p[0], p[1]);
+  float up[4] = {0.f, 0.f, 0.f, 0.f}, down[4] = {0.f, 0.f, 0.f, 0.f};
+  mma<BF16>(up, plus, seen[0], seen[1]);
+  mma<BF16>(down, minus, seen[0], seen[1]);
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    if (up[x] > 0.0f) acc[x] += INFINITY;
+    if (down[x] > 0.0f) acc[x] -= INFINITY;
+  }
+}
+
 // ---------------------------------------------------------------- main kernel
-template <typename T, int KIND_, int D_, int STAGES_>
+template <typename T, int KIND_, int D_, int STAGES_, int ROWS_>
 struct Cfg {
-  static constexpr int KIND = KIND_, D = D_, STAGES = STAGES_;
+  static constexpr int KIND = KIND_, D = D_, STAGES = STAGES_, ROWS = ROWS_;
   static constexpr bool kSmall = KIND != kSame;
   static constexpr bool kBf16 = !kSmall && std::is_same<T, __nv_bfloat16>::value;  // type of the products
   static constexpr int kRow = D * (kSmall ? 1 : 2);                                // bytes of a key row
@@ -101,8 +134,8 @@ struct Cfg {
   static constexpr int TN = kWarps * KW;                                           // keys of a unit
   static constexpr int kHalf = KW * kRow;                                          // keys, or values, of a step
   static constexpr int kStage = 2 * kHalf + (kSmall ? 2 * KW * 4 : 0);
-  static constexpr int kScratch = kWarps * kRows * 32 * 4;  // joining the warps' sums, 32 dimensions a turn
-  static constexpr int kSmem = kWarps * STAGES * kStage + kScratch + kWarps * kRows * 16;
+  static constexpr int kScratch = kWarps * ROWS * (ROWS == 8 ? 36 : 32) * 4;  // joining the warps' sums, 32 dimensions a turn
+  static constexpr int kSmem = kWarps * STAGES * kStage + kScratch + kWarps * ROWS * 16;
 };
 
 // Byte offset of 16-byte chunk c of a row: rows shifted against one another so
@@ -192,6 +225,14 @@ __device__ __forceinline__ bool any_wild(const uint8_t* values) {
   return __any_sync(kFull, wild != 0);
 }
 
+// Up to 16 rows.  Each warp runs through its own keys of a block's units with
+// copies of its own (a step is 16 keys, or 32 of 8 bits), so nothing in the loop waits for another warp;
+// the warps are joined at the end of a piece.  Bound by the chain of
+// instructions a warp works through per step (widening 8-bit values, softmax)
+// with two blocks of four warps on an SM: 224 registers and two blocks beat
+// 168 and three (264 us against 276; 128 requests of all lengths up to 8192, 32 / 8 heads
+// of 128, e4m3), two stages equal three, and one block-wide pipeline with
+// barriers took 580.
 template <typename T, typename C>
 __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p) {
   constexpr int D = C::D, KW = C::KW, KIND = C::KIND;
@@ -599,12 +640,397 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
   if (tid == 0) p.joins[blockIdx.x] = join;
 }
 
+// The same for up to 8 rows, which is what a single token mostly has, with the
+// operands the other way round: 16 keys (or dimensions) against 8 rows, so that
+// no half of a matrix instruction, and no half of the exponentials, is spent on
+// rows that are not there.  Fewer sums per thread leave room for three blocks on
+// an SM (with two: 267 us; with three: 259; 128 requests of all lengths up to
+// 8192, 32 / 8 heads of 128, e4m3 with a scale per token, 1.26 GB: 4.8 TB/s).
+// Issue slots are 48 % used, DRAM 54 %: what is left is the latency of each
+// warp's chain.  A single request of some hundred tokens takes 12 us, 5 of them
+// the joining kernel.
+template <typename T, typename C>
+__global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_constant__ Params p) {
+  constexpr int D = C::D, KW = C::KW, KIND = C::KIND;
+  constexpr int kMT = KW / 16;  // 16-key tiles of the scores
+  constexpr int kDT = D / 16;   // 16-dimension tiles of the output
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int red[kWarps + 2];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, j4 = lane & 3;
+  uint8_t* mine = smem + warp * (C::STAGES * C::kStage);  // the warp's own stages
+  const uint32_t stages = smem_u32(mine);
+  float* scratch = reinterpret_cast<float*>(smem + kWarps * C::STAGES * C::kStage);
+  float4* warp_ml = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(scratch) + C::kScratch);
+
+  // the joining kernel may start; it waits for this one to end before it reads
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  int total, unit, b0, before;
+  int share = 0;
+  locate<kThreads>(
+      p,
+      [&](int tot) {
+        share = share_of(p, tot, gridDim.x);
+        return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
+      },
+      red, total, unit, b0, before);
+  clear_idle_requests<kThreads>(p, D);
+  int4 join = make_int4(0, 0, 0, 0);
+  Pieces pc, ahead;  // the piece worked on, the one copied
+  const bool busy = unit < total && pc.start(p, b0, before, unit, min(share, total - unit));
+  if (!busy) {
+    if (tid == 0) p.joins[blockIdx.x] = join;
+    return;
+  }
+
+  // every warp walks the units by itself: its copies, its steps, no barrier until an item ends
+  ahead = pc;
+  int ahead_tile = 0;
+  bool more = true;
+  Place next = look<C>(p, ahead, 0, warp, lane);
+  auto load = [&](int s) {
+    if (more) {
+      const Place at = next;
+      copy_step<C>(p, ahead, at, stages + s * C::kStage, lane);
+      if (++ahead_tile == ahead.nt) {
+        ahead_tile = 0;
+        more = ahead.next(p);
+      }
+      if (more) next = look<C>(p, ahead, ahead_tile, warp, lane);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < C::STAGES - 1; ++s) load(s);
+
+  uint32_t qf[D / 16][2];  // the queries, right operand of the first product
+  float qscale[2];         // of the thread's two rows, 2 j and 2 j + 1
+  float acc[kDT][4];
+  float m[2], l[2], vref = 0.0f;
+  int tok[2], qi[2], head[2];
+  bool row_ok[2];
+  int stage = 0;
+
+  do {
+   for (int tile = 0; tile < pc.nt; ++tile) {
+    cp_wait<C::STAGES - 2>();
+    __syncwarp();
+    {
+      int s = stage + C::STAGES - 1;
+      if (s >= C::STAGES) s -= C::STAGES;
+      load(s);
+    }
+
+    if (tile == 0) {
+      const int rows = pc.r.n * p.group;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int row = 2 * j4 + e;
+        row_ok[e] = row < rows;
+        qi[e] = row / p.group;
+        head[e] = pc.item * p.group + row - qi[e] * p.group;
+        tok[e] = pc.r.first + qi[e];
+        m[e] = -INFINITY;
+        l[e] = 0.0f;
+      }
+      float mine_scale = p.scale_log2;
+      {
+        const int i = g / p.group;
+        const bool ok = g < rows;
+        const T* q = static_cast<const T*>(p.q) + (pc.r.first + i) * p.q_tok + (pc.item * p.group + g - i * p.group) * p.q_head;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          qf[kk][0] = qf[kk][1] = 0;
+          if (ok) {
+            if constexpr (C::kSmall) {  // dimensions 4j..4j+3, the order the 8-bit keys come in
+              const uint2 q4 = *reinterpret_cast<const uint2*>(q + kk * 16 + 4 * j4);
+              qf[kk][0] = q4.x, qf[kk][1] = q4.y;
+            } else {
+              qf[kk][0] = *reinterpret_cast<const uint32_t*>(q + kk * 16 + 2 * j4);
+              qf[kk][1] = *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8 + 2 * j4);
+            }
+          }
+        }
+        if constexpr (C::kSmall && std::is_same<T, __nv_bfloat16>::value) {
+          // bf16 queries as fp16: scaled by a power of two to a maximum in [1, 2), which is exact for all values
+          // that count beside the row's largest
+          float top = 0.0f;
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              top = fmaxf(top, fmaxf(fabsf(__uint_as_float(qf[kk][x] << 16)), fabsf(__uint_as_float(qf[kk][x] & 0xFFFF0000u))));
+          top = fmaxf(top, __shfl_xor_sync(kFull, top, 1));
+          top = fmaxf(top, __shfl_xor_sync(kFull, top, 2));
+          const uint32_t ex = min(max(__float_as_uint(top) & 0x7F800000u, 0x0A000000u), 0x75000000u);
+          const float down = __uint_as_float(0x7F000000u - ex);
+          mine_scale *= __uint_as_float(ex);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+              qf[kk][x] = pack2<false>(__uint_as_float(qf[kk][x] << 16) * down, __uint_as_float(qf[kk][x] & 0xFFFF0000u) * down);
+        }
+      }
+      // the scale of row g lies with lanes 4 g ..; this thread's results are of rows 2 j and 2 j + 1
+      qscale[0] = __shfl_sync(kFull, mine_scale, 8 * j4);
+      qscale[1] = __shfl_sync(kFull, mine_scale, 8 * j4 + 4);
+      vref = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[i][x] = 0.0f;
+    }
+
+    // ---- scores of the warp's KW keys (g and g + 8 of each tile of 16) and the rows 2 j, 2 j + 1
+    const uint32_t ks = stages + stage * C::kStage, vs = ks + C::kHalf;
+    const float* scale_k = reinterpret_cast<const float*>(mine + stage * C::kStage + 2 * C::kHalf);
+    const float* scale_v = scale_k + KW;
+    float s[kMT][4];
+#pragma unroll
+    for (int i = 0; i < kMT; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) s[i][x] = 0.0f;
+    const int mi = lane >> 3, mr = lane & 7;
+    if constexpr (!C::kSmall) {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int t = 0; t < kMT; ++t) {
+          uint32_t a[4];  // keys 0-7, 8-15 of dimensions 0-7, then of 8-15
+          ldsm4(a, ks + place<C>(t * 16 + (mi & 1) * 8 + mr, kk * 2 + (mi >> 1)));
+          mma<C::kBf16>(s[t], a, qf[kk][0], qf[kk][1]);
+        }
+    } else {
+#pragma unroll
+      for (int kk = 0; kk < D / 16; kk += 2)
+#pragma unroll
+        for (int t = 0; t < kMT; ++t) {
+          uint32_t b[4];  // keys 0-7, 8-15 of 16 dimensions, then of the next 16
+          ldsm4(b, ks + place<C>(t * 16 + (mi & 1) * 8 + mr, kk + (mi >> 1)));
+#pragma unroll
+          for (int x = 0; x < 4; ++x)
+            if (KIND == kInt8) b[x] ^= 0x80808080u;
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t a[4] = {widen<KIND, 0, 1>(b[2 * y]), widen<KIND, 0, 1>(b[2 * y + 1]), widen<KIND, 2, 3>(b[2 * y]),
+                                   widen<KIND, 2, 3>(b[2 * y + 1])};
+            mma<false>(s[t], a, qf[kk + y][0], qf[kk + y][1]);
+          }
+        }
+    }
+
+    // ---- scale, mask, running maximum: element x of tile t is key 16 t + g + 8 (x >> 1), row 2 j + (x & 1)
+    const int key0 = (pc.tile0 + tile) * C::TN + warp * KW;
+    const bool tail = key0 + KW > pc.r.len - pc.r.n;
+    uint32_t view[2] = {kFull, kFull};  // the keys a row sees
+    if (tail) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) view[e] = seen32(p, pc.r, row_ok[e] ? tok[e] : pc.r.first, row_ok[e] ? qi[e] : 0, key0);
+    }
+    float top[2] = {-INFINITY, -INFINITY};
+    float vmax = 0.0f, sv[kMT][2];
+#pragma unroll
+    for (int t = 0; t < kMT; ++t) {
+      float sk[2] = {1.0f, 1.0f};
+      if constexpr (C::kSmall) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          sk[y] = scale_k[t * 16 + g + 8 * y];
+          sv[t][y] = scale_v[t * 16 + g + 8 * y];
+          vmax = fmaxf(vmax, sv[t][y] < 1e30f ? sv[t][y] : 0.0f);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        s[t][x] *= qscale[x & 1] * sk[x >> 1];
+        if (tail && !((view[x & 1] >> (16 * t + g + 8 * (x >> 1))) & 1)) s[t][x] = -INFINITY;
+        top[x & 1] = fmaxf(top[x & 1], s[t][x]);
+      }
+    }
+    // over the keys: lanes of one j
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      top[0] = fmaxf(top[0], __shfl_xor_sync(kFull, top[0], o));
+      top[1] = fmaxf(top[1], __shfl_xor_sync(kFull, top[1], o));
+      if constexpr (C::kSmall) vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, o));
+    }
+    float shrink = 1.0f;  // of the sums, when the reference scale of the values moves
+    if constexpr (C::kSmall) {
+      if (vmax > 64.0f * vref) {
+        const float to = __uint_as_float(max(__float_as_uint(vmax) & 0x7F800000u, 0x0A000000u));
+        shrink = vref / to;
+        vref = to;
+      }
+    }
+    if (__any_sync(kFull, top[0] > m[0] || top[1] > m[1]) || shrink != 1.0f) {
+      float alpha[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float now = fmaxf(m[e], top[e]);
+        alpha[e] = now == -INFINITY ? 1.0f : exp2_fast(m[e] - now);
+        l[e] *= alpha[e];
+        alpha[e] *= shrink;
+        m[e] = now;
+      }
+#pragma unroll
+      for (int i = 0; i < kDT; ++i)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) acc[i][x] *= alpha[x & 1];
+    }
+    const float inv_vref = C::kSmall ? __uint_as_float(0x7F000000u - __float_as_uint(vref)) : 1.0f;
+    const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+    // probabilities, keys x rows, turned into the right operand (rows x keys) 8 x 8 at a time
+    uint32_t pf[kMT][2];
+#pragma unroll
+    for (int t = 0; t < kMT; ++t)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float pr[2];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          pr[x] = exp2_fast(s[t][2 * y + x] - sub[x]);
+          l[x] += pr[x];
+          if constexpr (C::kSmall) pr[x] = pr[x] == 0.0f && tail ? 0.0f : pr[x] * (sv[t][y] * inv_vref);
+        }
+        pf[t][y] = turned(pack2<C::kBf16>(pr[0], pr[1]));
+      }
+
+    // ---- values (16 dimensions x 16 keys) times probabilities
+    const bool wild = KIND != kInt8 && tail && pc.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf);
+    uint32_t ones[kMT][2];
+    if (wild) {
+#pragma unroll
+      for (int t = 0; t < kMT; ++t)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int key = 16 * t + g + 8 * y;
+          ones[t][y] = turned((((view[0] >> key) & 1u) | ((view[1] >> key) & 1u) << 16) * (C::kBf16 ? 0x3F80u : 0x3C00u));
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < kMT; ++t)
+#pragma unroll
+      for (int d = 0; d < kDT; d += C::kSmall ? 2 : 1) {
+        uint32_t a[2][4];
+        if constexpr (!C::kSmall) {  // keys 0-7 of dimensions 0-7, 8-15, then keys 8-15
+          ldsm4t(a[0], vs + place<C>(t * 16 + (mi >> 1) * 8 + mr, 2 * d + (mi & 1)));
+        } else {
+          uint32_t b[4];  // keys 0-7, 8-15 of 16 dimensions, then of the next 16: even dimensions first, odd ones behind
+          ldsm4t(b, vs + place<C>(t * 16 + (mi & 1) * 8 + mr, d + (mi >> 1)));
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t lo = KIND == kInt8 ? b[2 * y] ^ 0x80808080u : b[2 * y];
+            const uint32_t hi = KIND == kInt8 ? b[2 * y + 1] ^ 0x80808080u : b[2 * y + 1];
+            a[y][0] = widen<KIND, 0, 2>(lo), a[y][1] = widen<KIND, 1, 3>(lo);
+            a[y][2] = widen<KIND, 0, 2>(hi), a[y][3] = widen<KIND, 1, 3>(hi);
+          }
+        }
+#pragma unroll
+        for (int y = 0; y < (C::kSmall ? 2 : 1); ++y) {
+          if (wild)
+            mma_seen_values<C::kBf16>(acc[d + y], a[y], pf[t], ones[t]);
+          else
+            mma<C::kBf16>(acc[d + y], a[y], pf[t][0], pf[t][1]);
+        }
+      }
+    __syncwarp();  // the stage is read before the next copies into it
+    if (++stage == C::STAGES) stage = 0;
+   }
+
+    // ---- end of the piece: join the warps, write
+    {
+      const bool whole = pc.nt == pc.tiles;
+      const int slot = pc.tile0 == 0 ? 1 : 0;
+      if (!whole && pc.tile0 == 0) join = make_int4(parts_of(p, pc, share), pc.r.first, pc.r.n, pc.item);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[e] += __shfl_xor_sync(kFull, l[e], o);
+        if (g == 0) warp_ml[warp * 8 + 2 * j4 + e] = make_float4(m[e], l[e], 0.0f, 0.0f);
+      }
+      __syncthreads();
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, warp_ml[w * 8 + 2 * j4 + e].x);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 o = warp_ml[w * 8 + 2 * j4 + e];
+          ll += o.x == -INFINITY ? o.y : exp2_fast(o.x - mm) * o.y;
+        }
+        f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
+        m[e] = mm;
+        l[e] = ll;
+        if (C::kSmall) f[e] *= vref;
+        if (whole) f[e] = ll == 0.0f ? 0.0f : f[e] / ll;
+      }
+      const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * 8;
+      if (warp == 0 && g == 0) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = 2 * j4 + e;
+          if (!whole) {
+            p.part_ml[(part + row) * 2] = m[e];
+            p.part_ml[(part + row) * 2 + 1] = l[e];
+          } else if (row_ok[e] && p.lse) {
+            p.lse[static_cast<long long>(tok[e]) * p.kv_heads * p.group + head[e]] =
+                l[e] == 0.0f ? -INFINITY : (m[e] + log2f(l[e])) * 0.69314718055994531f;
+          }
+        }
+      }
+#pragma unroll
+      for (int d0 = 0; d0 < D; d0 += 32) {
+        if (d0 > 0) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float(&x)[4] = acc[d0 / 16 + i];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float* to = scratch + (warp * 8 + 2 * j4 + e) * 36 + i * 16;  // 36: rows apart in the banks
+            if constexpr (C::kSmall) {
+              *reinterpret_cast<float2*>(to + 2 * g) = make_float2(x[e] * f[e], x[2 + e] * f[e]);
+            } else {
+              to[g] = x[e] * f[e];
+              to[g + 8] = x[2 + e] * f[e];
+            }
+          }
+        }
+        __syncthreads();
+        const int row = tid >> 3, d = (tid & 7) * 4;  // 4 dimensions of a row each
+        if (row >= 8) continue;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float4 v = *reinterpret_cast<const float4*>(scratch + (w * 8 + row) * 36 + d);
+          sum.x += v.x, sum.y += v.y, sum.z += v.z, sum.w += v.w;
+        }
+        if (!whole) {
+          *reinterpret_cast<float4*>(p.part_o + (part + row) * D + d0 + d) = sum;
+        } else if (row < pc.r.n * p.group) {
+          const int i2 = row / p.group;
+          T* o = static_cast<T*>(p.out) + (pc.r.first + i2) * p.o_tok + (pc.item * p.group + row - i2 * p.group) * p.o_head;
+          constexpr bool kOutBf16 = std::is_same<T, __nv_bfloat16>::value;
+          *reinterpret_cast<uint2*>(o + d0 + d) = make_uint2(pack2<kOutBf16>(sum.x, sum.y), pack2<kOutBf16>(sum.z, sum.w));
+        }
+      }
+      __syncthreads();
+    }
+  } while (pc.next(p));
+  cp_wait<0>();
+  if (tid == 0) p.joins[blockIdx.x] = join;
+}
+
 // ---------------------------------------------------------------- joining kernel
 // Block c joins the one row tile that begins in the main kernel's block c and
 // goes on behind it: its parts lie in slot 1 of c and slot 0 of the next
 // blocks.  A block takes 16 of its rows, four to a warp; where there are fewer
 // rows, several warps share the parts of four and join theirs at the end, so
-// that a long sequence with few rows is not a chain of loads.
+// that a long sequence with few rows is not a chain of loads.  Bound by latency
+// (the wait on the main kernel, then two dependent loads): about 5 us.
 template <typename T, int D>
 __global__ void __launch_bounds__(kJoinThreads, 8) join_kernel(const __grid_constant__ Params p) {
   constexpr int kJoinWarps = kJoinThreads / 32;
@@ -712,31 +1138,36 @@ unsigned long long part_rows(int sms, long long rows) {
 
 template <typename T, typename C>
 orError_t launch(Params& p, cudaStream_t st, int sms, int* grid) {
-  const void* fn = reinterpret_cast<const void*>(&attend_kernel<T, C>);
+  void (*kernel)(Params);
+  if constexpr (C::ROWS == 8)
+    kernel = &attend8_kernel<T, C>;
+  else
+    kernel = &attend_kernel<T, C>;
+  const void* fn = reinterpret_cast<const void*>(kernel);
   MCPU_CUDA_TRY(ensure_dynamic_smem(fn, C::kSmem), "tree_attention");
   static std::atomic<int> known{0};  // blocks per SM: a property of the kernel, asked once
   int resident = known.load(std::memory_order_relaxed);
   if (resident == 0) {
-    MCPU_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, attend_kernel<T, C>, kThreads, C::kSmem),
+    MCPU_CUDA_TRY(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&resident, kernel, kThreads, C::kSmem),
                   "tree_attention");
     resident = std::max(1, std::min(resident, kMaxResident));
     known.store(resident, std::memory_order_relaxed);
   }
   *grid = resident * sms;
-  p.rows_log2 = 4;
+  p.rows_log2 = C::ROWS == 8 ? 3 : 4;
   p.keys_log2 = C::TN == 64 ? 6 : 7;
-  p.item_cost = 2;
-  p.min_share = 1;
-  attend_kernel<T, C><<<*grid, kThreads, C::kSmem, st>>>(p);
+  p.item_cost = 2;  // measured: 0 293 us, 2 276 us, 5 275 us for a decoding batch of all lengths
+  p.min_share = 1;  // units a block takes at least; 2 and 4 cost a single request 0.6 and 1.9 us
+  kernel<<<*grid, kThreads, C::kSmem, st>>>(p);
   return from_cuda(cudaGetLastError(), "tree_attention launch");
 }
 
-template <typename T, int D>
+template <typename T, int D, int ROWS>
 orError_t launch_few(Params& p, int dtype, cudaStream_t st, int sms, int* grid) {
   constexpr int kStages = 2;
-  if (p.c.dtype == dtype) return launch<T, Cfg<T, kSame, D, kStages>>(p, st, sms, grid);
-  if (p.c.dtype == MCPU_INT8) return launch<T, Cfg<T, kInt8, D, kStages>>(p, st, sms, grid);
-  return launch<T, Cfg<T, kE4M3, D, kStages>>(p, st, sms, grid);
+  if (p.c.dtype == dtype) return launch<T, Cfg<T, kSame, D, kStages, ROWS>>(p, st, sms, grid);
+  if (p.c.dtype == MCPU_INT8) return launch<T, Cfg<T, kInt8, D, kStages, ROWS>>(p, st, sms, grid);
+  return launch<T, Cfg<T, kE4M3, D, kStages, ROWS>>(p, st, sms, grid);
 }
 
 template <typename T, int D>
@@ -745,7 +1176,9 @@ orError_t run(Params& p, int dtype, long long rows, void* ws, cudaStream_t st, i
   p.part_ml = p.part_o + part_rows(sms, rows) * D;
   p.joins = reinterpret_cast<int4*>(p.part_ml + part_rows(sms, rows) * 2);
   int grid = 0;
-  const orError_t e = rows <= kRows ? launch_few<T, D>(p, dtype, st, sms, &grid) : launch_tc(p, D, rows, st, sms, &grid);
+  const orError_t e = rows <= 8      ? launch_few<T, D, 8>(p, dtype, st, sms, &grid)
+                       : rows <= kRows ? launch_few<T, D, kRows>(p, dtype, st, sms, &grid)
+                                       : launch_tc(p, D, rows, st, sms, &grid);
   if (e != orSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid, std::max(1, (1 << p.rows_log2) / (kJoinThreads / 8)));

@@ -26,6 +26,18 @@
 // The output is scaled down only when a row's maximum grew by more than 2^8
 // since the reference was set; until then probabilities up to 256 are summed,
 // which fp16 and bf16 hold and fp32 sums take without loss.
+//
+// Measured: 16 requests of up to 8192 tokens with trees of 61, 64 / 8 heads of
+// 128, bf16 (133 GFLOP) 212 us, 630 TFLOP/s; 6 requests of up to 32768 with
+// trees of 13, 32 / 8 heads, fp16 over int8 (279 MB) 132 us, 2.1 TB/s.  The
+// tensor pipe is 36 % and the exponentials' 31 % busy: each stream's chain
+// (scores, softmax, product) is what a pair of tiles waits for, about 3500
+// cycles against 2048 of exponentials, and a piece's beginning and end cost as
+// much as four tiles.  With 8 bits the widening of the rows adds to it.
+// Tried and slower: sixteen softmax warps (234 us), softmax loops unrolled over
+// the whole row (308 us, the code outgrew the instruction cache), part of the
+// exponentials by polynomial (equal), bulk copies of 128-byte rows (34 cycles
+// each to issue).
 #include <algorithm>
 #include <type_traits>
 

@@ -112,6 +112,8 @@ inline mcpuKvCache cache_of(const at::Tensor& key_cache, const at::Tensor& value
   TORCH_CHECK((ks[3] == 1 && vs[3] == 1) || sz[3] <= 1, op, ": cache rows must be contiguous");
   TORCH_CHECK(sz[1] < (1LL << 31) && sz[2] < (1LL << 31) && sz[3] < (1LL << 31), op, ": bad cache sizes");
   if (writes) {
+    TORCH_CHECK(key_cache.numel() == 0 || key_cache.data_ptr() != value_cache.data_ptr(), op,
+                ": key_cache and value_cache are written and must not overlap");
     using Dim = std::pair<int64_t, int64_t>;
     disjoint<3>({Dim{ks[0], sz[0]}, Dim{ks[1], sz[1]}, Dim{ks[2], sz[2]}}, sz[3], op, "key_cache");
     disjoint<3>({Dim{vs[0], sz[0]}, Dim{vs[1], sz[1]}, Dim{vs[2], sz[2]}}, sz[3], op, "value_cache");
@@ -136,6 +138,8 @@ inline mcpuKvCache cache_of(const at::Tensor& key_cache, const at::Tensor& value
     c.scale_mode = MCPU_KV_SCALE_TOKEN;
     for (int i = 0; i < 3; ++i) c.k_scale_stride[i] = k_scale->stride(i), c.v_scale_stride[i] = v_scale->stride(i);
     if (writes) {
+      TORCH_CHECK(k_scale->numel() == 0 || k_scale->data_ptr() != v_scale->data_ptr(), op,
+                  ": k_scale and v_scale are written and must not overlap");
       using Dim = std::pair<int64_t, int64_t>;
       const int64_t *k3 = c.k_scale_stride, *v3 = c.v_scale_stride;
       disjoint<3>({Dim{k3[0], sz[0]}, Dim{k3[1], sz[1]}, Dim{k3[2], sz[2]}}, 1, op, "k_scale");
@@ -251,6 +255,8 @@ inline void gather_cache(const Api& api, const at::Tensor& key_cache, const at::
   TORCH_CHECK(key_out.dim() == 3 && key_out.size(1) == c.kv_heads && key_out.size(2) == c.head_size &&
                   key_out.is_contiguous() && value_out.is_contiguous(),
               op, ": outputs must be contiguous [tokens, ", c.kv_heads, ", ", c.head_size, "] tensors");
+  TORCH_CHECK(key_out.numel() == 0 || key_out.data_ptr() != value_out.data_ptr(), op,
+              ": key_out and value_out are written and must not overlap");
   check_block_table(block_table, op);
   const int64_t batch = block_table.size(0), width = block_table.size(1);
   check_int32(cu_seq_lens, batch + 1, op, "cu_seq_lens");
