@@ -617,3 +617,107 @@ def test_two_graphs_and_a_stream_at_once():
         torch.cuda.synchronize()
         for a, b in zip(want, outs + [third]):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------ borders between the kernels, long caches, refusals
+@pytest.mark.parametrize("dtype", HALF)
+@pytest.mark.parametrize("kind,scales", [("same", "none"), (torch.float8_e4m3fn, "token"), (torch.int8, "head")])
+@pytest.mark.parametrize("size", [64, 128])
+@pytest.mark.parametrize("most", [7, 8, 9, 15, 16, 17, 128, 129])
+def test_attention_at_the_row_borders(dtype, kind, scales, size, most):
+    """The largest request fills a kernel's rows, or is one row short of them or beyond; trees and chains."""
+    counts = [most, 1, max(1, most - 1)]
+    x = make(12, [most + 200, 77, most + 3], counts, 2, 2, size, 32, dtype, kind, scales)
+    q, kc, vc, ks, vs, bt, sl, cu = x
+    for mask in (None, random_tree(5, counts)):
+        got, lse = ops.tree_attention(q, kc, vc, bt, sl, cu, most, size ** -0.5, tree_mask=mask, k_scale=ks, v_scale=vs, return_lse=True)
+        check(*x, size ** -0.5, mask, got, lse)
+
+
+@pytest.mark.parametrize("kind,scales", [("same", "none"), (torch.float8_e4m3fn, "token"), (torch.int8, "token"),
+                                         (torch.float8_e4m3fn, "tensor")])
+def test_attention_garbage_with_few_rows(kind, scales):
+    """NaN and infinities where nothing is seen, up to 8 rows a key / value head."""
+    test_attention_garbage_where_nothing_is_seen(kind, scales, 1, [6, 3])
+
+
+@pytest.mark.parametrize("dtype", HALF)
+def test_attention_infinite_value_of_a_draft_with_few_rows(dtype):
+    for heads, counts, sign in ((1, [6], -1), (2, [4], 1)):
+        x = make(4, [90], counts, heads, 1, 128, 16, dtype, "same", "none")
+        q, kc, vc, ks, vs, bt, sl, cu = x
+        mask = torch.tensor([[1], [3], [1], [9], [19], [41]][: counts[0]], device="cuda")  # [3]: draft 1
+        clean = ops.tree_attention(q, kc, vc, bt, sl, cu, counts[0], 0.125, tree_mask=mask)
+        pos = 90 - counts[0] + 1
+        vc[int(bt[0, pos // 16]), pos % 16, 0, 77] = sign * math.inf
+        got = ops.tree_attention(q, kc, vc, bt, sl, cu, counts[0], 0.125, tree_mask=mask)
+        seen_by = ((mask[:, 0] >> 1) & 1).bool()
+        assert seen_by.any() and not seen_by.all()
+        want = clean.clone()
+        want[..., 77][seen_by] = sign * math.inf
+        assert torch.equal(got, want)
+
+
+def test_attention_more_tokens_than_announced():
+    """A request with more than max_query_len tokens gives zeros and the flag; the others are served."""
+    for most, counts in ((1, [1, 3, 1]), (2, [2, 5, 1]), (40, [40, 41, 3])):
+        x = make(6, [80, 90, 70], counts, 4, 2, 64, 16, torch.bfloat16, "same", "none")
+        q, kc, vc, ks, vs, bt, sl, cu = x
+        ops.device_error(reset=True)
+        got, lse = ops.tree_attention(q, kc, vc, bt, sl, cu, most, 0.125, return_lse=True)
+        assert ops.device_error(reset=True) == 1
+        a, b = counts[0], counts[0] + counts[1]
+        assert (got[a:b] == 0).all() and (lse[a:b] == -math.inf).all()
+        served = [0, 2]
+        cu2 = torch.tensor([0, a, a + counts[2]], dtype=torch.int32, device="cuda")
+        rest = [torch.cat([t[:a], t[b:]]) for t in (q, got, lse)]
+        check(rest[0], kc, vc, ks, vs, bt[served], sl[served], cu2, 0.125, None, rest[1], rest[2])
+
+
+def test_caches_beyond_32_bit_offsets():
+    """Pages past 2^32 elements: written, read back and attended as in a small cache."""
+    blocks, block, kv, size = 263000, 16, 8, 128  # 4.3e9 values each
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    g = gen(3)
+    big = [torch.zeros(blocks, block, kv, size, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2)]
+    small = [torch.zeros(8, block, kv, size, dtype=torch.float8_e4m3fn, device="cuda") for _ in range(2)]
+    far = torch.tensor([[blocks - 1, 3, blocks - 2, 262200, 262145, 0]], dtype=torch.int32, device="cuda")
+    near = torch.tensor([[7, 3, 2, 4, 5, 0]], dtype=torch.int32, device="cuda")
+    n = 6 * block - 5
+    k, v = (randn(g, n, kv, size, dtype=torch.bfloat16) for _ in range(2))
+    at = torch.arange(n, device="cuda")
+    cu = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    results = []
+    for (kc, vc), table_ in ((big, far), (small, near)):
+        ks, vs = (torch.zeros(kc.shape[:3], device="cuda") for _ in range(2))
+        slots = table_[0, at // block].long() * block + at % block
+        ops.reshape_and_cache(k, v, kc, vc, slots, ks, vs)
+        out = [torch.empty_like(k) for _ in range(2)]
+        ops.gather_cache(kc, vc, table_, cu, out[0], out[1], ks, vs)
+        for tokens, heads in ((1, 32), (4, 32), (20, 64)):
+            q = randn(gen(tokens), tokens, heads, size, dtype=torch.bfloat16)
+            out.append(ops.tree_attention(q, kc, vc, table_, cu[1:], torch.tensor([0, tokens], dtype=torch.int32, device="cuda"),
+                                          tokens, size ** -0.5, k_scale=ks, v_scale=vs))
+        results.append(out)
+        del ks, vs
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    assert results[0][2].abs().max() > 0
+
+
+def test_written_tensors_must_not_be_one():
+    g = gen(1)
+    k, v = (randn(g, 3, 2, 64, dtype=torch.float16) for _ in range(2))
+    kc, vc, ks, vs = new_cache(4, 16, 2, 64, torch.int8, torch.float16, "token", g)
+    slots = torch.arange(3, device="cuda")
+    with pytest.raises(RuntimeError, match="key_cache and value_cache are written"):
+        ops.reshape_and_cache(k, v, kc, kc, slots, ks, vs)
+    with pytest.raises(RuntimeError, match="k_scale and v_scale are written"):
+        ops.reshape_and_cache(k, v, kc, vc, slots, ks, ks)
+    with pytest.raises(RuntimeError, match="query and key are written"):
+        ops.rotary_embedding(slots, k, k, 64, table(8, 64), True)
+    bt = torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    with pytest.raises(RuntimeError, match="key_out and value_out are written"):
+        ops.gather_cache(kc, vc, bt, cu, k, k, ks, vs)
