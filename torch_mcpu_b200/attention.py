@@ -143,7 +143,8 @@ def rotary_reshape_and_cache(positions: torch.Tensor, query: torch.Tensor | None
                              k_scale: torch.Tensor | None = None, v_scale: torch.Tensor | None = None) -> None:
     """rotary_embedding and reshape_and_cache in one launch: query is rotated
     in place, the rotated key goes to the cache only (key is left as it is).
-    Results are those of the two calls, bit for bit."""
+    rotary_dim is a multiple of 16 here.  Results are those of the two calls,
+    bit for bit."""
     if cos_sin_cache is None:
         _fail("rotary_reshape_and_cache", "cos_sin_cache is needed")
     (_ops or _native()).write(positions, query, key, value, cos_sin_cache, is_neox, key_cache, value_cache, slot_mapping,
@@ -182,6 +183,7 @@ def tree_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: to
     Returns the output (`out` where given), with return_lse also the float32
     [tokens, heads] logarithms of the softmax sums.  A token that sees nothing
     gives zeros and -inf; tokens outside every request are left as they are
-    (undefined in an output made by the call)."""
+    (undefined in an output made by the call).  out overlaps no other tensor
+    of the call."""
     return (_ops or _native()).tree_attention(query, key_cache, value_cache, block_table, seq_lens, cu_query_lens,
                                               max_query_len, scale, tree_mask, k_scale, v_scale, out, return_lse)
