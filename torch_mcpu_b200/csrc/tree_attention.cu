@@ -31,8 +31,8 @@
 // request x query heads per key / value head.  Up to 8 and up to 16 rows: the
 // kernels of this file, which read each key once at the cost of one matrix
 // instruction a 16-key tile; the 8-row one is the faster where it applies (100
-// requests of up to 6000 tokens, 32 / 8 heads of 128: e4m3 152 us against 161,
-// int8 148 against 163, bf16 219 against 228).  More rows: tensor memory,
+// requests of up to 6000 tokens, 32 / 8 heads of 128: e4m3 148 us against 161,
+// int8 151 against 163, bf16 217 against 228).  More rows: tensor memory,
 // tree_attention_tc.cu, whose 128-row tile costs the same however many rows
 // of it are used, but which is the only one that keeps up with more than 16.
 #include <algorithm>
@@ -644,9 +644,9 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
 // operands the other way round: 16 keys (or dimensions) against 8 rows, so that
 // no half of a matrix instruction, and no half of the exponentials, is spent on
 // rows that are not there.  Fewer sums per thread leave room for three blocks on
-// an SM (with two: 267 us; with three: 259; 128 requests of all lengths up to
-// 8192, 32 / 8 heads of 128, e4m3 with a scale per token, 1.26 GB: 4.8 TB/s).
-// Issue slots are 48 % used, DRAM 54 %: what is left is the latency of each
+// an SM (with two: 267 us; with three: 258; 128 requests of all lengths up to
+// 8192, 32 / 8 heads of 128, e4m3 with a scale per token, 1.26 GB: 4.9 TB/s).
+// Issue slots are 50 % used, DRAM 60 %: what is left is the latency of each
 // warp's chain.  A single request of some hundred tokens takes 12 us, 5 of them
 // the joining kernel.
 template <typename T, typename C>
@@ -839,7 +839,6 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
         for (int y = 0; y < 2; ++y) {
           sk[y] = scale_k[t * 16 + g + 8 * y];
           sv[t][y] = scale_v[t * 16 + g + 8 * y];
-          vmax = fmaxf(vmax, sv[t][y] < 1e30f ? sv[t][y] : 0.0f);
         }
       }
 #pragma unroll
@@ -854,7 +853,10 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
     for (int o = 4; o < 32; o <<= 1) {
       top[0] = fmaxf(top[0], __shfl_xor_sync(kFull, top[0], o));
       top[1] = fmaxf(top[1], __shfl_xor_sync(kFull, top[1], o));
-      if constexpr (C::kSmall) vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, o));
+    }
+    if constexpr (C::kSmall) {  // a lane a key; not negative, so ordered as whole numbers are
+      const float v = scale_v[lane];
+      vmax = __uint_as_float(__reduce_max_sync(kFull, v > 0.0f && v < 1e30f ? __float_as_uint(v) : 0u));
     }
     float shrink = 1.0f;  // of the sums, when the reference scale of the values moves
     if constexpr (C::kSmall) {
@@ -898,43 +900,49 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
       }
 
     // ---- values (16 dimensions x 16 keys) times probabilities
-    const bool wild = KIND != kInt8 && tail && pc.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf);
-    uint32_t ones[kMT][2];
-    if (wild) {
+    auto products = [&](auto some_wild) {
+      uint32_t ones[kMT][2];
+      if constexpr (some_wild.value) {
+#pragma unroll
+        for (int t = 0; t < kMT; ++t)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int key = 16 * t + g + 8 * y;
+            ones[t][y] = turned((((view[0] >> key) & 1u) | ((view[1] >> key) & 1u) << 16) * (C::kBf16 ? 0x3F80u : 0x3C00u));
+          }
+      }
 #pragma unroll
       for (int t = 0; t < kMT; ++t)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int key = 16 * t + g + 8 * y;
-          ones[t][y] = turned((((view[0] >> key) & 1u) | ((view[1] >> key) & 1u) << 16) * (C::kBf16 ? 0x3F80u : 0x3C00u));
-        }
-    }
+        for (int d = 0; d < kDT; d += C::kSmall ? 2 : 1) {
+          uint32_t a[2][4];
+          if constexpr (!C::kSmall) {  // keys 0-7 of dimensions 0-7, 8-15, then keys 8-15
+            ldsm4t(a[0], vs + place<C>(t * 16 + (mi >> 1) * 8 + mr, 2 * d + (mi & 1)));
+          } else {
+            uint32_t b[4];  // keys 0-7, 8-15 of 16 dimensions, then of the next 16: even dimensions first, odd ones behind
+            ldsm4t(b, vs + place<C>(t * 16 + (mi & 1) * 8 + mr, d + (mi >> 1)));
 #pragma unroll
-    for (int t = 0; t < kMT; ++t)
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t lo = KIND == kInt8 ? b[2 * y] ^ 0x80808080u : b[2 * y];
+              const uint32_t hi = KIND == kInt8 ? b[2 * y + 1] ^ 0x80808080u : b[2 * y + 1];
+              a[y][0] = widen<KIND, 0, 2>(lo), a[y][1] = widen<KIND, 1, 3>(lo);
+              a[y][2] = widen<KIND, 0, 2>(hi), a[y][3] = widen<KIND, 1, 3>(hi);
+            }
+          }
 #pragma unroll
-      for (int d = 0; d < kDT; d += C::kSmall ? 2 : 1) {
-        uint32_t a[2][4];
-        if constexpr (!C::kSmall) {  // keys 0-7 of dimensions 0-7, 8-15, then keys 8-15
-          ldsm4t(a[0], vs + place<C>(t * 16 + (mi >> 1) * 8 + mr, 2 * d + (mi & 1)));
-        } else {
-          uint32_t b[4];  // keys 0-7, 8-15 of 16 dimensions, then of the next 16: even dimensions first, odd ones behind
-          ldsm4t(b, vs + place<C>(t * 16 + (mi & 1) * 8 + mr, d + (mi >> 1)));
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const uint32_t lo = KIND == kInt8 ? b[2 * y] ^ 0x80808080u : b[2 * y];
-            const uint32_t hi = KIND == kInt8 ? b[2 * y + 1] ^ 0x80808080u : b[2 * y + 1];
-            a[y][0] = widen<KIND, 0, 2>(lo), a[y][1] = widen<KIND, 1, 3>(lo);
-            a[y][2] = widen<KIND, 0, 2>(hi), a[y][3] = widen<KIND, 1, 3>(hi);
+          for (int y = 0; y < (C::kSmall ? 2 : 1); ++y) {
+            if constexpr (some_wild.value)
+              mma_seen_values<C::kBf16>(acc[d + y], a[y], pf[t], ones[t]);
+            else
+              mma<C::kBf16>(acc[d + y], a[y], pf[t][0], pf[t][1]);
           }
         }
-#pragma unroll
-        for (int y = 0; y < (C::kSmall ? 2 : 1); ++y) {
-          if (wild)
-            mma_seen_values<C::kBf16>(acc[d + y], a[y], pf[t], ones[t]);
-          else
-            mma<C::kBf16>(acc[d + y], a[y], pf[t][0], pf[t][1]);
-        }
-      }
+    };
+    // one branch for all products: the rare ones stay out of the way of the instruction fetch
+    if (KIND != kInt8 && tail && pc.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf))
+      products(std::true_type());
+    else
+      products(std::false_type());
     __syncwarp();  // the stage is read before the next copies into it
     if (++stage == C::STAGES) stage = 0;
    }
