@@ -721,3 +721,61 @@ def test_written_tensors_must_not_be_one():
     cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
     with pytest.raises(RuntimeError, match="key_out and value_out are written"):
         ops.gather_cache(kc, vc, bt, cu, k, k, ks, vs)
+
+
+def test_tensors_that_require_a_gradient_are_refused():
+    x = make(6, [50], [2], 4, 2, 64, 16, torch.bfloat16, "same", "none")
+    q, kc, vc, ks, vs, bt, sl, cu = x
+    want = ops.tree_attention(q, kc, vc, bt, sl, cu, 2, 0.125)
+    k = torch.zeros(2, 2, 64, dtype=q.dtype, device="cuda", requires_grad=True)
+    pos = torch.arange(2, device="cuda")
+    q.requires_grad_()
+    calls = [lambda: ops.tree_attention(q, kc, vc, bt, sl, cu, 2, 0.125),
+             lambda: ops.rotary_embedding(pos, q, None, 64, table(8, 64), True),
+             lambda: ops.reshape_and_cache(k, k.detach(), kc, vc, pos),
+             lambda: ops.rotary_reshape_and_cache(pos, q, k.detach(), k.detach(), table(8, 64), True, kc, vc, pos)]
+    for call in calls:
+        with pytest.raises(RuntimeError, match="requires a gradient"):
+            call()
+    with torch.no_grad():
+        assert torch.equal(calls[0](), want)
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured: nothing has been loaded or configured before."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from torch_mcpu_b200 import ops
+for n in (1, 3, 40):  # a kernel each
+    q = torch.randn(n, 16, 128, device="cuda").half()
+    k = torch.randn(n, 4, 128, device="cuda").half()
+    kc, vc = (torch.randn(8, 16, 4, 128, device="cuda").to(torch.float8_e4m3fn) for _ in range(2))
+    ks, vs = (torch.rand(8, 16, 4, device="cuda") + 0.5 for _ in range(2))
+    bt = torch.arange(8, dtype=torch.int32, device="cuda")[None]
+    sl, cu, cs = (torch.tensor(v, dtype=torch.int32, device="cuda") for v in ([100], [0, n], [0, 100]))
+    table = ops.rotary_cos_sin_cache(128, 128, device="cuda")
+    pos = torch.arange(n, device="cuda")
+    back = [torch.empty(100, 4, 128, device="cuda").half() for _ in range(2)]
+    q0 = q.clone()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.rotary_reshape_and_cache(pos, q, k, k, table, True, kc, vc, pos, ks, vs)
+        o = ops.tree_attention(q, kc, vc, bt, sl, cu, n, 0.1, k_scale=ks, v_scale=vs)
+        ops.gather_cache(kc, vc, bt, cs, back[0], back[1], ks, vs)
+    graph.replay()
+    torch.cuda.synchronize()
+    got = [o.clone(), back[0].clone(), back[1].clone(), q.clone()]
+    ops.rotary_reshape_and_cache(pos, q0, k, k, table, True, kc, vc, pos, ks, vs)
+    o = ops.tree_attention(q0, kc, vc, bt, sl, cu, n, 0.1, k_scale=ks, v_scale=vs)
+    ops.gather_cache(kc, vc, bt, cs, back[0], back[1], ks, vs)
+    assert all(torch.equal(a, b) for a, b in zip(got, [o, *back, q0])) and ops.device_error() == 0
+print("same")
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and done.stdout.strip() == "same", done.stderr[-2000:]

@@ -4,7 +4,8 @@ read-back, and attention over it for single tokens and drafted trees.
 
 Like torch_mcpu_b200.ops (which re-exports every function here), each call
 checks its arguments, enqueues on torch's current stream of the tensors'
-device and returns; there is no CPU fallback.
+device and returns; there is no CPU fallback.  The operators have no
+gradients: tensors that require one are refused while gradients are recorded.
 """
 
 from __future__ import annotations
@@ -111,8 +112,7 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
 
 def rotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor | None, head_size: int,
                      cos_sin_cache: torch.Tensor, is_neox: bool = True) -> None:
-    """vLLM's rotary_embedding (vllm/_custom_ops.py, rotary_embedding), in
-    place: the first rotary_dim = cos_sin_cache.size(1) dimensions of every
+    """Rotary positions with vLLM's argument order, in place: the first rotary_dim = cos_sin_cache.size(1) dimensions of every
     head of query and key ([tokens, heads * head_size] or [tokens, heads,
     head_size], float32, bfloat16 or float16; views of a larger tensor are
     fine) are rotated by their position's angles.  is_neox: pairs (i, i +
@@ -126,7 +126,7 @@ def reshape_and_cache(key: torch.Tensor, value: torch.Tensor, key_cache: torch.T
     """Writes the rows of key and value [tokens, kv_heads, head_size] into
     their slots (slot_mapping[t] = block * block_size + place; negative: not
     written; no slot twice) of a paged cache [num_blocks, block_size,
-    kv_heads, head_size] (vLLM's reshape_and_cache_flash layout; strided views
+    kv_heads, head_size] (vLLM's layout; strided views
     such as a [num_blocks, kv_heads, block_size, head_size] tensor permuted
     are fine).
 

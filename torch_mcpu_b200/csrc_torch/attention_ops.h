@@ -5,6 +5,7 @@
 #pragma once
 
 #include <ATen/ATen.h>
+#include <c10/core/GradMode.h>
 
 #include <algorithm>
 #include <array>
@@ -44,6 +45,15 @@ inline void same_device(const at::Tensor& t, const at::Tensor& first, const char
 }
 inline void same_device(const Opt& t, const at::Tensor& first, const char* op, const char* name) {
   if (t) same_device(*t, first, op, name);
+}
+
+// Operators of serving: they have no gradient to give, and what is rotated in place would falsify others'.
+inline void no_gradient(const at::Tensor& t, const char* op, const char* name) {
+  TORCH_CHECK(!t.requires_grad() || !c10::GradMode::is_enabled(), op, ": ", name,
+              " requires a gradient, which this operator does not have; call it under torch.no_grad()");
+}
+inline void no_gradient(const Opt& t, const char* op, const char* name) {
+  if (t) no_gradient(*t, op, name);
 }
 
 // [tokens, heads * head_size] or [tokens, heads, head_size] with contiguous heads.
@@ -163,6 +173,8 @@ inline void rotary_embedding(const Api& api, const at::Tensor& positions, const 
   same_device(positions, query, op, "positions");
   same_device(key, query, op, "key");
   same_device(table, query, op, "cos_sin_cache");
+  no_gradient(query, op, "query");
+  no_gradient(key, op, "key");
   const auto type = query.scalar_type();
   TORCH_CHECK((type == at::kFloat || type == at::kBFloat16 || type == at::kHalf) && (!key || key->scalar_type() == type), op,
               ": query and key must both be float32, bfloat16 or float16");
@@ -203,6 +215,9 @@ inline void write(const Api& api, const Opt& positions, const Opt& query, const 
   same_device(slot_mapping, key, op, "slot_mapping");
   same_device(k_scale, key, op, "k_scale");
   same_device(v_scale, key, op, "v_scale");
+  no_gradient(query, op, "query");
+  no_gradient(key, op, "key");
+  no_gradient(value, op, "value");
   const auto type = key.scalar_type();
   TORCH_CHECK(value.scalar_type() == type && (!query || query->scalar_type() == type), op,
               ": query, key and value must have one type");
@@ -284,6 +299,8 @@ inline std::tuple<at::Tensor, at::Tensor> tree_attention(
   same_device(k_scale, query, op, "k_scale");
   same_device(v_scale, query, op, "v_scale");
   same_device(out_given, query, op, "out");
+  no_gradient(query, op, "query");
+  no_gradient(out_given, op, "out");
   const auto type = query.scalar_type();
   const mcpuKvCache c = cache_of(key_cache, value_cache, k_scale, v_scale, type, false, op);
   TORCH_CHECK(query.dim() == 3 && query.size(2) == c.head_size && query.stride(2) == 1, op,

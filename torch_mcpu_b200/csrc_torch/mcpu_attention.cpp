@@ -1,6 +1,5 @@
-// The attention path on the mcpu device: schemas with vLLM's argument order
-// (vllm/_custom_ops.py: rotary_embedding, reshape_and_cache_flash,
-// gather_and_maybe_dequant_cache), bodies in attention_ops.h.
+// The attention path on the mcpu device: schemas with vLLM's argument order,
+// bodies in attention_ops.h.
 #include <torch/library.h>
 
 #include "attention_ops.h"
