@@ -25,7 +25,7 @@
 //
 // 8-bit caches are multiplied as fp16, which holds e4m3 and int8 values
 // exactly: the scales of the keys go onto the scores, those of the values onto
-// the probabilities.
+// the probabilities, relative to a reference of each row (kLift).
 //
 // Which kernel.  Rows that share a key / value head = queries of the longest
 // request x query heads per key / value head.  Up to 8 and up to 16 rows: the
@@ -225,6 +225,36 @@ __device__ __forceinline__ bool any_wild(const uint8_t* values) {
   return __any_sync(kFull, wild != 0);
 }
 
+// A row's maximum m moves to top: its sum l, the lift that goes with it, and
+// by what its output sums are scaled.  With scales (SMALL) those keep to their
+// reference, 2^(m - lift), and the lift rises with m up to its limit.
+template <bool SMALL>
+__device__ __forceinline__ float grow(float top, float& m, float& l, float& lift) {
+  const float now = fmaxf(m, SMALL ? ceilf(top) : top);
+  const float alpha = now == -INFINITY ? 1.0f : exp2_fast(m - now);
+  float by = alpha;
+  if constexpr (SMALL) {
+    by = 1.0f;
+    if (now > m) {
+      lift += now - m;
+      if (lift > kLift) by = exp2_fast(kLift - lift), lift = kLift;
+    }
+  }
+  l *= alpha;
+  m = now;
+  return by;
+}
+// The lift falls where the products' largest, w, would pass the room: by what
+// the output sums are scaled.  An infinite scale lowers it once, to its least.
+__device__ __forceinline__ float lower(float w, float& lift, float& up) {
+  const float to = lift_for(w);
+  if (!(w * up > kRoom) || to >= lift) return 1.0f;
+  const float by = exp2_fast(to - lift);
+  lift = to;
+  up = exp2_whole(to);
+  return by;
+}
+
 // Up to 16 rows.  Each warp runs through its own keys of a block's units with
 // copies of its own (a step is 16 keys, or 32 of 8 bits), so nothing in the loop waits for another warp;
 // the warps are joined at the end of a piece.  Bound by the chain of
@@ -291,7 +321,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
   uint4* qs = reinterpret_cast<uint4*>(scratch);  // the queries' fragments, the same for every warp
   float qscale[2];
   float acc[kDT][4];
-  float m[2], l[2], vref = 0.0f;
+  float m[2], l[2], lift[2];
   int tok[2], qi[2], head[2];
   bool row_ok[2];
   int stage = 0;
@@ -317,6 +347,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
         tok[e] = pc.r.first + qi[e];
         m[e] = -INFINITY;
         l[e] = 0.0f;
+        lift[e] = kLift;
         qscale[e] = p.scale_log2;
         const T* q = static_cast<const T*>(p.q) + tok[e] * p.q_tok + head[e] * p.q_head;
 #pragma unroll
@@ -364,7 +395,6 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
       for (int kk = 0; kk < D / 16; ++kk)
         if (kk % kWarps == warp) qs[kk * 32 + lane] = make_uint4(qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
       __syncthreads();
-      vref = 0.0f;
 #pragma unroll
       for (int i = 0; i < kDT; ++i)
 #pragma unroll
@@ -422,15 +452,10 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
         view[e] = seen32(p, pc.r, row_ok[e] ? tok[e] : pc.r.first, row_ok[e] ? qi[e] : 0, key0) >> (2 * j4);
     }
     float top[2] = {-INFINITY, -INFINITY};
-    float vmax = 0.0f;
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
       float2 sk = make_float2(1.0f, 1.0f);
-      if constexpr (C::kSmall) {
-        sk = *reinterpret_cast<const float2*>(scale_k + n * 8 + 2 * j4);
-        const float2 sv = *reinterpret_cast<const float2*>(scale_v + n * 8 + 2 * j4);
-        vmax = fmaxf(vmax, fmaxf(sv.x < 1e30f ? sv.x : 0.0f, sv.y < 1e30f ? sv.y : 0.0f));
-      }
+      if constexpr (C::kSmall) sk = *reinterpret_cast<const float2*>(scale_k + n * 8 + 2 * j4);
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         s[n][x] *= qscale[x >> 1] * ((x & 1) ? sk.y : sk.x);
@@ -443,50 +468,59 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
       top[e] = fmaxf(top[e], __shfl_xor_sync(kFull, top[e], 1));
       top[e] = fmaxf(top[e], __shfl_xor_sync(kFull, top[e], 2));
     }
-    float shrink = 1.0f;  // of the sums, when the reference scale of the values moves
-    if constexpr (C::kSmall) {
-      vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, 1));
-      vmax = fmaxf(vmax, __shfl_xor_sync(kFull, vmax, 2));
-      if (vmax > 64.0f * vref) {
-        const float to = __uint_as_float(max(__float_as_uint(vmax) & 0x7F800000u, 0x0A000000u));
-        shrink = vref / to;
-        vref = to;
-      }
-    }
-    if (__any_sync(kFull, top[0] > m[0] || top[1] > m[1]) || shrink != 1.0f) {
-      float alpha[2];
+    if (__any_sync(kFull, top[0] > m[0] || top[1] > m[1])) {
+      float by[2];  // of the sums
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const float now = fmaxf(m[e], top[e]);
-        alpha[e] = now == -INFINITY ? 1.0f : exp2_fast(m[e] - now);
-        l[e] *= alpha[e];
-        alpha[e] *= shrink;
-        m[e] = now;
+        by[e] = grow<C::kSmall>(top[e], m[e], l[e], lift[e]);
       }
+      if (!C::kSmall || __any_sync(kFull, by[0] != 1.0f || by[1] != 1.0f)) {
 #pragma unroll
-      for (int i = 0; i < kDT; ++i)
+        for (int i = 0; i < kDT; ++i)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[i][x] *= alpha[x >> 1];
+          for (int x = 0; x < 4; ++x) acc[i][x] *= by[x >> 1];
+      }
     }
-    const float inv_vref = C::kSmall ? __uint_as_float(0x7F000000u - __float_as_uint(vref)) : 1.0f;
     const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
-    uint32_t pf[kNT / 2][4];
+    float wtop[2] = {0.0f, 0.0f};  // products with the values' scales
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
-      float pr[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
-        pr[x] = exp2_fast(s[n][x] - sub[x >> 1]);
-        l[x >> 1] += pr[x];
+        s[n][x] = exp2_fast(s[n][x] - sub[x >> 1]);
+        l[x >> 1] += s[n][x];
       }
       if constexpr (C::kSmall) {
         const float2 sv = *reinterpret_cast<const float2*>(scale_v + n * 8 + 2 * j4);
-        const float f[2] = {sv.x * inv_vref, sv.y * inv_vref};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) pr[x] = pr[x] == 0.0f && tail ? 0.0f : pr[x] * f[x & 1];
+        for (int x = 0; x < 4; ++x) {
+          s[n][x] = s[n][x] == 0.0f && tail ? 0.0f : s[n][x] * ((x & 1) ? sv.y : sv.x);
+          wtop[x >> 1] = fmaxf(wtop[x >> 1], s[n][x]);
+        }
       }
-      pf[n >> 1][(n & 1) * 2] = pack2<C::kBf16>(pr[0], pr[1]);
-      pf[n >> 1][(n & 1) * 2 + 1] = pack2<C::kBf16>(pr[2], pr[3]);
+    }
+    float up[2] = {1.0f, 1.0f};
+    if constexpr (C::kSmall) {
+      up[0] = exp2_whole(lift[0]), up[1] = exp2_whole(lift[1]);
+      if (__any_sync(kFull, wtop[0] * up[0] > kRoom || wtop[1] * up[1] > kRoom)) {
+        float by[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          wtop[e] = fmaxf(wtop[e], __shfl_xor_sync(kFull, wtop[e], 1));
+          wtop[e] = fmaxf(wtop[e], __shfl_xor_sync(kFull, wtop[e], 2));
+          by[e] = lower(wtop[e], lift[e], up[e]);
+        }
+#pragma unroll
+        for (int i = 0; i < kDT; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[i][x] *= by[x >> 1];
+      }
+    }
+    uint32_t pf[kNT / 2][4];
+#pragma unroll
+    for (int n = 0; n < kNT; ++n) {
+      pf[n >> 1][(n & 1) * 2] = pack2<C::kBf16>(s[n][0] * up[0], s[n][1] * up[0]);
+      pf[n >> 1][(n & 1) * 2 + 1] = pack2<C::kBf16>(s[n][2] * up[1], s[n][3] * up[1]);
     }
 
     // ---- probabilities times values
@@ -580,7 +614,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
         f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
         m[e] = mm;
         l[e] = ll;
-        if (C::kSmall) f[e] *= vref;
+        if (C::kSmall) f[e] *= exp2_whole(-lift[e]);
         if (whole) f[e] = ll == 0.0f ? 0.0f : f[e] / ll;
       }
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * kRows;
@@ -707,7 +741,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
   uint32_t qf[D / 16][2];  // the queries, right operand of the first product
   float qscale[2];         // of the thread's two rows, 2 j and 2 j + 1
   float acc[kDT][4];
-  float m[2], l[2], vref = 0.0f;
+  float m[2], l[2], lift[2];
   int tok[2], qi[2], head[2];
   bool row_ok[2];
   int stage = 0;
@@ -733,6 +767,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
         tok[e] = pc.r.first + qi[e];
         m[e] = -INFINITY;
         l[e] = 0.0f;
+        lift[e] = kLift;
       }
       float mine_scale = p.scale_log2;
       {
@@ -776,7 +811,6 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
       // the scale of row g lies with lanes 4 g ..; this thread's results are of rows 2 j and 2 j + 1
       qscale[0] = __shfl_sync(kFull, mine_scale, 8 * j4);
       qscale[1] = __shfl_sync(kFull, mine_scale, 8 * j4 + 4);
-      vref = 0.0f;
 #pragma unroll
       for (int i = 0; i < kDT; ++i)
 #pragma unroll
@@ -830,16 +864,12 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
       for (int e = 0; e < 2; ++e) view[e] = seen32(p, pc.r, row_ok[e] ? tok[e] : pc.r.first, row_ok[e] ? qi[e] : 0, key0);
     }
     float top[2] = {-INFINITY, -INFINITY};
-    float vmax = 0.0f, sv[kMT][2];
 #pragma unroll
     for (int t = 0; t < kMT; ++t) {
       float sk[2] = {1.0f, 1.0f};
       if constexpr (C::kSmall) {
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          sk[y] = scale_k[t * 16 + g + 8 * y];
-          sv[t][y] = scale_v[t * 16 + g + 8 * y];
-        }
+        for (int y = 0; y < 2; ++y) sk[y] = scale_k[t * 16 + g + 8 * y];
       }
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
@@ -854,50 +884,59 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
       top[0] = fmaxf(top[0], __shfl_xor_sync(kFull, top[0], o));
       top[1] = fmaxf(top[1], __shfl_xor_sync(kFull, top[1], o));
     }
-    if constexpr (C::kSmall) {  // a lane a key; not negative, so ordered as whole numbers are
-      const float v = scale_v[lane];
-      vmax = __uint_as_float(__reduce_max_sync(kFull, v > 0.0f && v < 1e30f ? __float_as_uint(v) : 0u));
-    }
-    float shrink = 1.0f;  // of the sums, when the reference scale of the values moves
-    if constexpr (C::kSmall) {
-      if (vmax > 64.0f * vref) {
-        const float to = __uint_as_float(max(__float_as_uint(vmax) & 0x7F800000u, 0x0A000000u));
-        shrink = vref / to;
-        vref = to;
+    if (__any_sync(kFull, top[0] > m[0] || top[1] > m[1])) {
+      float by[2];  // of the sums
+#pragma unroll
+      for (int e = 0; e < 2; ++e) by[e] = grow<C::kSmall>(top[e], m[e], l[e], lift[e]);
+      if (!C::kSmall || __any_sync(kFull, by[0] != 1.0f || by[1] != 1.0f)) {
+#pragma unroll
+        for (int i = 0; i < kDT; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[i][x] *= by[x & 1];
       }
     }
-    if (__any_sync(kFull, top[0] > m[0] || top[1] > m[1]) || shrink != 1.0f) {
-      float alpha[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float now = fmaxf(m[e], top[e]);
-        alpha[e] = now == -INFINITY ? 1.0f : exp2_fast(m[e] - now);
-        l[e] *= alpha[e];
-        alpha[e] *= shrink;
-        m[e] = now;
-      }
-#pragma unroll
-      for (int i = 0; i < kDT; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) acc[i][x] *= alpha[x & 1];
-    }
-    const float inv_vref = C::kSmall ? __uint_as_float(0x7F000000u - __float_as_uint(vref)) : 1.0f;
     const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+    float wtop[2] = {0.0f, 0.0f};  // products with the values' scales
+#pragma unroll
+    for (int t = 0; t < kMT; ++t)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        float sv = 1.0f;
+        if constexpr (C::kSmall) sv = scale_v[t * 16 + g + 8 * y];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          float& w = s[t][2 * y + x];
+          w = exp2_fast(w - sub[x]);
+          l[x] += w;
+          if constexpr (C::kSmall) {
+            w = w == 0.0f && tail ? 0.0f : w * sv;
+            wtop[x] = fmaxf(wtop[x], w);
+          }
+        }
+      }
+    float up[2] = {1.0f, 1.0f};
+    if constexpr (C::kSmall) {
+      up[0] = exp2_whole(lift[0]), up[1] = exp2_whole(lift[1]);
+      if (__any_sync(kFull, wtop[0] * up[0] > kRoom || wtop[1] * up[1] > kRoom)) {
+        float by[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) wtop[e] = fmaxf(wtop[e], __shfl_xor_sync(kFull, wtop[e], o));
+          by[e] = lower(wtop[e], lift[e], up[e]);
+        }
+#pragma unroll
+        for (int i = 0; i < kDT; ++i)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) acc[i][x] *= by[x & 1];
+      }
+    }
     // probabilities, keys x rows, turned into the right operand (rows x keys) 8 x 8 at a time
     uint32_t pf[kMT][2];
 #pragma unroll
     for (int t = 0; t < kMT; ++t)
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float pr[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          pr[x] = exp2_fast(s[t][2 * y + x] - sub[x]);
-          l[x] += pr[x];
-          if constexpr (C::kSmall) pr[x] = pr[x] == 0.0f && tail ? 0.0f : pr[x] * (sv[t][y] * inv_vref);
-        }
-        pf[t][y] = turned(pack2<C::kBf16>(pr[0], pr[1]));
-      }
+      for (int y = 0; y < 2; ++y) pf[t][y] = turned(pack2<C::kBf16>(s[t][2 * y] * up[0], s[t][2 * y + 1] * up[1]));
 
     // ---- values (16 dimensions x 16 keys) times probabilities
     auto products = [&](auto some_wild) {
@@ -973,7 +1012,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
         f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
         m[e] = mm;
         l[e] = ll;
-        if (C::kSmall) f[e] *= vref;
+        if (C::kSmall) f[e] *= exp2_whole(-lift[e]);
         if (whole) f[e] = ll == 0.0f ? 0.0f : f[e] / ll;
       }
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * 8;

@@ -230,6 +230,26 @@ __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2^-22 rela
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Products of probabilities and value scales, w_j = p_j s_j, are multiplied as
+// fp16, relative to a reference of each row: w_j 2^lift.  The lift brings the
+// largest product so far of the keys the row sees to 2^7 .. 2^8; it falls, with
+// the sums scaled down, when a product would pass 2^15, and rises with the
+// row's maximum, whose growth makes the earlier products smaller.  So only what
+// lies below 2^-21 of the largest product is held with fewer bits than fp16
+// has, at most 2^-32 of it off, however far apart the scales are and whatever
+// those of unseen keys are.  (From 2^10 the lift falls more often: 145 us
+// instead of 137 for the small trees of tree_attention_tc.cu.)  A reference
+// taken from the scales alone, the largest of a step, lost whole outputs beside
+// one key of a large scale and no probability.  Lifts, and the maxima they go
+// with, are whole numbers: the scaling is exact.
+constexpr float kLift = 100.0f;    // the highest; where no product above 0 has been seen
+constexpr float kRoom = 32768.0f;  // of 65504
+__device__ __forceinline__ float exp2_whole(float e) {  // -126 .. 127
+  return __int_as_float((static_cast<int>(e) + 127) << 23);
+}
+__device__ __forceinline__ float lift_for(float w) {
+  return fminf(kLift, 7.0f - static_cast<float>(static_cast<int>(__float_as_uint(w) >> 23) - 127));
+}
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   if constexpr (BF16) {

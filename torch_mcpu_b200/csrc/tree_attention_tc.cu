@@ -19,8 +19,7 @@
 //             asynchronous copies into the 128-byte-swizzled layout.  8-bit
 //             ones: rows of a raw ring widened to fp16
 //   1         its first warp issues the products; with 8-bit caches two more
-//             fetch the rows of keys and of values, and the
-//             last looks at the scales
+//             fetch the rows of keys and of values, with their scales
 // Tensor memory: scores of the two streams (2 x 128 columns), outputs (2 x D).
 //
 // The output is scaled down only when a row's maximum grew by more than 2^8
@@ -29,7 +28,7 @@
 //
 // Measured: 16 requests of up to 8192 tokens with trees of 61, 64 / 8 heads of
 // 128, bf16 (133 GFLOP) 212 us, 630 TFLOP/s; 6 requests of up to 32768 with
-// trees of 13, 32 / 8 heads, fp16 over int8 (279 MB) 132 us, 2.1 TB/s.  The
+// trees of 13, 32 / 8 heads, fp16 over int8 (279 MB) 137 us, 2.0 TB/s.  The
 // tensor pipe is 36 % and the exponentials' 31 % busy: each stream's chain
 // (scores, softmax, product) is what a pair of tiles waits for, about 3500
 // cycles against 2048 of exponentials, and a piece's beginning and end cost as
@@ -78,7 +77,7 @@ struct Cfg {
   static constexpr int kOffWild = kSlots * kSlot;
   static constexpr int kOffRowWild = kOffWild + kSlots * kWild;
   static constexpr int kOffScale = kOffRowWild + (KIND == kInt8 ? 0 : 2 * kTile * 32);
-  static constexpr int kOffMl = kOffScale + (TOKEN ? kScaleRing * (2 * kTile * 4 + 16) : 0);
+  static constexpr int kOffMl = kOffScale + (TOKEN ? kScaleRing * 2 * kTile * 4 : 0);
   static constexpr int kOffBars = kOffMl + 2 * kTile * 16;
   static constexpr int kOffQ = (kOffBars + 768 + 1023) / 1024 * 1024;
   static constexpr int raw_depth(int nq) { return !kSmall ? 0 : nq == 1 ? 4 : 2; }
@@ -87,7 +86,7 @@ struct Cfg {
 };
 
 struct Bars {
-  uint64_t kv_full[4], kv_empty[4], raw_full[4], raw_empty[4], sc_full[kScaleRing], sc_top[kScaleRing], q_full, s_full[2], p_full[2], o_done[2], both, drain;
+  uint64_t kv_full[4], kv_empty[4], raw_full[4], raw_empty[4], sc_full[kScaleRing], q_full, s_full[2], p_full[2], o_done[2], both, drain;
   uint32_t tmem;
   int abort;
   int wild[4][8];
@@ -453,31 +452,6 @@ struct Loader {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
   }
 
-  // ---- token scales: the largest finite one of each tile's values, for the reference the probabilities are scaled by.
-  __device__ __forceinline__ void run_scales(const Run& run) {
-    Pieces pc;
-    pc.start(p, run.b0, run.before, run.unit, run.count);
-    uint32_t t = 0;
-    bool ok = true;
-    do {
-      for (int j = 0; j < pc.nt && ok; ++j, ++t) {
-        const int ring = t & (kScaleRing - 1);
-        ok = wait(&bars->sc_full[ring], (t / kScaleRing) & 1, abort);
-        if (!ok) break;
-        const float4 s4 = *reinterpret_cast<const float4*>(mem + C::kOffScale + ((ring * 2 + 1) * kTile + 4 * lane) * 4);
-        const float v[4] = {s4.x, s4.y, s4.z, s4.w};
-        unsigned top = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(v[i] > 0.0f && v[i] < 1e30f ? v[i] : 0.0f));
-        top = __reduce_max_sync(kFull, top);
-        if (lane == 0) {
-          *reinterpret_cast<uint32_t*>(mem + C::kOffScale + kScaleRing * 2 * kTile * 4 + ring * 4) = top;
-          mbar_arrive(&bars->sc_top[ring]);
-        }
-      }
-    } while (ok && pc.next(p));
-  }
-
   // ---- 8-bit caches, widening: raw rows to fp16 in the swizzled tiles.
   __device__ __forceinline__ void run_widen(const Run& run) {
     const int lead = nq == 1 ? 2 : 1;
@@ -561,7 +535,7 @@ struct Soft {
   uint8_t* mem;
   uint32_t tmem_s, tmem_o;  // this warp's lanes of the stream's scores and outputs
   volatile int* abort;
-  float m, l, vref, qscale;  // reference maximum and sum; reference scale of the values
+  float m, l, lift, qscale;  // reference maximum and sum; lift of the products with the values' scales
   bool wild;
 
   // Chunks [c0, c1) of 8 dimensions of a row of queries into shared memory.  bf16 queries of an 8-bit cache become fp16 after a power of two brings the row's
@@ -602,7 +576,7 @@ struct Soft {
   }
 
   __device__ __forceinline__ void begin() {
-    m = -INFINITY, l = 0.0f, vref = 0.0f;
+    m = -INFINITY, l = 0.0f, lift = kLift;
     wild = false;
   }
 
@@ -638,9 +612,38 @@ struct Soft {
     return fmaxf(t0, t1);
   }
 
+  // The row's output sums times `by`.
+  __device__ __forceinline__ void scale_outputs(float by) const {
+#pragma unroll 1
+    for (int c = 0; c < C::D / 16; ++c) {
+      uint32_t o[16];
+      tmem_ld16(tmem_o + 16 * c, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * by);
+      tmem_st16(tmem_o + 16 * c, o);
+    }
+  }
+  // What the first chunks of 32 scores have become, times `by`.
+  __device__ __forceinline__ void scale_written(int chunks, float by) const {
+    tmem_st_wait();
+#pragma unroll 1
+    for (int c = 0; c < chunks; ++c) {
+      uint32_t o[16];
+      tmem_ld16(tmem_s + 16 * c, o);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&o[i]));
+        o[i] = pack2<false>(f.x * by, f.y * by);
+      }
+      tmem_st16(tmem_s + 16 * c, o);
+    }
+  }
+
   // Scores of one key tile to probabilities.  TAIL: some keys are not seen (a bit each in seen).
   template <bool TAIL>
-  __device__ __forceinline__ void tile(const uint32_t (&seen)[4], const float* ks, const float* vs, float vmax, bool first) {
+  __device__ __forceinline__ void tile(const uint32_t (&seen)[4], const float* ks, const float* vs, bool first) {
     // The row is read twice, 32 scores at a time, in rolled loops: reading it is cheap, while the code of a whole row
     // unrolled, beside that of the other roles, overran the instruction cache (full trees 308 us; 64 at a time 224 us, 32
     // 220 us; half of the exponentials by a polynomial on the multiply-add pipe 234 us).
@@ -655,38 +658,31 @@ struct Soft {
     }
     top *= qscale;
     // the reference moves when the maximum left it by more than 2^kGrow
-    float alpha = 1.0f;
+    float alpha = 1.0f, by = 1.0f;  // of the sum, of the outputs
     if (top > m + kGrow || m == -INFINITY) {
-      alpha = m == -INFINITY ? 1.0f : exp2_fast(m - top);
-      m = fmaxf(top, m);
+      const float now = fmaxf(C::TOKEN ? ceilf(top) : top, m);
+      if (m != -INFINITY) {
+        alpha = exp2_fast(m - now);
+        if constexpr (C::TOKEN) {
+          lift += now - m;
+          if (lift > kLift) by = exp2_fast(kLift - lift), lift = kLift;
+        }
+      }
+      m = now;
     }
     l *= alpha;
-    if constexpr (C::TOKEN) {
-      if (vmax > 64.0f * vref) {
-        const float to = __uint_as_float(max(__float_as_uint(vmax) & 0x7F800000u, 0x0A000000u));
-        alpha *= vref == 0.0f ? 1.0f : vref / to;  // nothing but zeros so far
-        vref = to;
-      }
-    }
-    if (!first && __any_sync(kFull, alpha != 1.0f)) {
-#pragma unroll 1
-      for (int c = 0; c < C::D / 16; ++c) {
-        uint32_t o[16];
-        tmem_ld16(tmem_o + 16 * c, o);
-        tmem_ld_wait();
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-        tmem_st16(tmem_o + 16 * c, o);
-      }
-    }
+    if constexpr (!C::TOKEN) by = alpha;
+    if (!first && __any_sync(kFull, by != 1.0f)) scale_outputs(by);
     const float sub = m == -INFINITY ? 0.0f : m;
     const unsigned long long q2 = pair(qscale, qscale), m2 = pair(-sub, -sub);
-    const float inv = C::TOKEN ? __uint_as_float(0x7F000000u - __float_as_uint(vref)) : 1.0f;
-    const unsigned long long i2 = pair(inv, inv);
+    float up = C::TOKEN ? exp2_whole(lift) : 1.0f;
     unsigned long long sum0 = pair(0.0f, 0.0f), sum1 = sum0;
 #pragma unroll 1
     for (int c = 0; c < 4; ++c) {
       const uint32_t sees = TAIL ? pick(seen, c) : kFull;
+      const unsigned long long u2 = pair(up, up);
+      unsigned long long part0 = pair(0.0f, 0.0f), part1 = part0;  // sums of the chunk, with scales
+      float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
       uint32_t v[32], out[16];
       tmem_ld32(tmem_s + 32 * c, v);
       tmem_ld_wait();
@@ -702,20 +698,44 @@ struct Soft {
             if (!((sees >> (i + x)) & 1)) e[x] = 0.0f;  // a scale of 0 makes -inf NaN
         }
         unsigned long long a = pair(e[0], e[1]), b = pair(e[2], e[3]);
-        sum0 = add2(sum0, a), sum1 = add2(sum1, b);
+        if constexpr (C::TOKEN)
+          part0 = add2(part0, a), part1 = add2(part1, b);
+        else
+          sum0 = add2(sum0, a), sum1 = add2(sum1, b);
         if constexpr (C::TOKEN) {
           const float4 vv = *reinterpret_cast<const float4*>(vs + 32 * c + i);
-          a = mul2(a, mul2(pair(vv.x, vv.y), i2)), b = mul2(b, mul2(pair(vv.z, vv.w), i2));
-          const float2 fa = unpair(a), fb = unpair(b);
-          e[0] = fa.x, e[1] = fa.y, e[2] = fb.x, e[3] = fb.y;
-          if (TAIL) {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-              if (!((sees >> (i + x)) & 1)) e[x] = 0.0f;  // an unseen scale may be anything
+          a = mul2(a, pair(vv.x, vv.y)), b = mul2(b, pair(vv.z, vv.w));
+          float2 fa = unpair(a), fb = unpair(b);
+          if (TAIL) {  // an unseen scale may be anything
+            if (!((sees >> i) & 1)) fa.x = 0.0f;
+            if (!((sees >> (i + 1)) & 1)) fa.y = 0.0f;
+            if (!((sees >> (i + 2)) & 1)) fb.x = 0.0f;
+            if (!((sees >> (i + 3)) & 1)) fb.y = 0.0f;
           }
+          w[i / 4 % 2] = fmaxf(fmaxf(w[i / 4 % 2], fa.x), fa.y), w[2 + i / 4 % 2] = fmaxf(fmaxf(w[2 + i / 4 % 2], fb.x), fb.y);
+          fa = unpair(mul2(pair(fa.x, fa.y), u2)), fb = unpair(mul2(pair(fb.x, fb.y), u2));
+          e[0] = fa.x, e[1] = fa.y, e[2] = fb.x, e[3] = fb.y;
         }
         out[i / 2] = pack2<C::BF16>(e[0], e[1]);
         out[i / 2 + 1] = pack2<C::BF16>(e[2], e[3]);
+      }
+      if constexpr (C::TOKEN) {
+        const float wtop = fmaxf(fmaxf(w[0], w[1]), fmaxf(w[2], w[3]));
+        if (__any_sync(kFull, wtop * up > kRoom)) {
+          // rare: the lift falls for these scores, which are still there, for what was written of the tile, and for the
+          // outputs; in all rows at once, where it would fall soon
+          const float to = lift_for(wtop);
+          if (__any_sync(kFull, to < lift)) {  // an infinite scale lowers the lift once, to its least
+            const float by = to < lift ? exp2_fast(to - lift) : 1.0f;
+            lift = fminf(lift, to);
+            up = exp2_whole(lift);
+            scale_written(c, by);
+            if (!first) scale_outputs(by);
+            --c;
+            continue;
+          }
+        }
+        sum0 = add2(sum0, part0), sum1 = add2(sum1, part1);
       }
       // over the scores 16 c .. 16 c + 15, which have been read
       tmem_st16(tmem_s + 16 * c, out);
@@ -781,10 +801,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       mbar_init(&bars->raw_full[i], 32);
       mbar_init(&bars->raw_empty[i], C::kLoadWarps);
     }
-    for (int i = 0; i < kScaleRing; ++i) {
-      mbar_init(&bars->sc_full[i], 32);
-      mbar_init(&bars->sc_top[i], 1);
-    }
+    for (int i = 0; i < kScaleRing; ++i) mbar_init(&bars->sc_full[i], 32);
     mbar_init(&bars->q_full, kSoftWarps);
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bars->s_full[i], 1);
@@ -916,8 +933,6 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       }
     } else if (C::kSmall && warp < C::kWarps - 1) {
       ld.run_fetch(warp == C::kWarps - 2, run);
-    } else if (C::TOKEN) {
-      ld.run_scales(run);
     }
   } else if (warp < kSoftWarps) {
     // ------------------------------------------------ softmax and output
@@ -925,9 +940,8 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
     const int x = warp >> 2, wrow = (warp & 3) * 32 + lane;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     Soft<C> so{p, bars, mem, tmem + lanes + x * kTile, tmem + lanes + 2 * kTile + x * D, abort};
-    float4* ml = reinterpret_cast<float4*>(mem + C::kOffMl);  // a row's maximum, sum, scale of values, note
+    float4* ml = reinterpret_cast<float4*>(mem + C::kOffMl);  // a row's maximum, sum, 2^-lift, note
     const float* scales = reinterpret_cast<const float*>(mem + C::kOffScale);
-    const float* vtop = scales + kScaleRing * 2 * kTile;
     uint32_t kv = 0, t0 = 0, sp = 0, op0 = 0, op1 = 0, meets = 0;
     auto meet = [&]() {  // the two streams' warps
       __syncwarp();
@@ -984,15 +998,13 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
           const int key0 = (pc.tile0 + j) * kTile;
           const bool tail = key0 + kTile > r.len - r.n;
           const float *ks = nullptr, *vs = nullptr;
-          float vmax = 0.0f;
           uint32_t seen[4] = {kFull, kFull, kFull, kFull};
           int slot = 0;
           if constexpr (C::TOKEN) {
             const int ring = (t0 + j) & (kScaleRing - 1);
-            ok = wait(&bars->sc_top[ring], ((t0 + j) / kScaleRing) & 1, abort);
+            ok = wait(&bars->sc_full[ring], ((t0 + j) / kScaleRing) & 1, abort);
             if (!ok) break;
             ks = scales + ring * 2 * kTile, vs = ks + kTile;
-            vmax = vtop[ring];
           }
           if (C::KIND != kInt8 && tail && r.n > 1) {
             // the value tile's notes are needed: its place in the order of loads
@@ -1010,10 +1022,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
               for (int i = 0; i < C::kLoadWarps; ++i) any |= bars->wild[slot][i];
               if (any) so.note_wild(seen, slot, x * kTile + wrow);
             }
-            so.template tile<true>(seen, ks, vs, vmax, first);
-          } else {
-            so.template tile<false>(seen, ks, vs, vmax, first);
           }
+          if (tail)
+            so.template tile<true>(seen, ks, vs, first);
+          else
+            so.template tile<false>(seen, ks, vs, first);
           first = false;
           tmem_st_wait();
         }
@@ -1051,11 +1064,11 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       int c0 = 0, c1 = D / 32;
       uint32_t o0 = so.tmem_o, o1 = so.tmem_o;
       bool noted0 = so.wild, noted1 = false;
-      const float vscale = C::kSmall ? (C::TOKEN ? so.vref : p.c.v_scale[h * p.c.v_scale_stride[2]]) : 1.0f;
+      const float vscale = C::kSmall ? (C::TOKEN ? exp2_whole(-so.lift) : p.c.v_scale[h * p.c.v_scale_stride[2]]) : 1.0f;
       f0 = vscale;
       if (nq == 1) {
         // each stream's warps write half of the dimensions, joining both streams' sums
-        ml[x * kTile + wrow] = make_float4(so.m, so.l, so.vref, so.wild ? 1.0f : 0.0f);
+        ml[x * kTile + wrow] = make_float4(so.m, so.l, C::TOKEN ? vscale : 0.0f, so.wild ? 1.0f : 0.0f);
         ok = meet();
         if (!ok) break;
         const float4 a = ml[wrow], b = two ? ml[kTile + wrow] : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
