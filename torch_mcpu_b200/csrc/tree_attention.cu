@@ -524,7 +524,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
     }
 
     // ---- probabilities times values
-    if (KIND != kInt8 && tail && pc.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf)) {
+    if (KIND != kInt8 && tail && some_unseen(p, pc.r) && any_wild<C>(mine + stage * C::kStage + C::kHalf)) {
 #pragma unroll
       for (int kk = 0; kk < kNT / 2; ++kk) {
         const int row = kk * 16 + (mi & 1) * 8 + mr;
@@ -978,7 +978,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
         }
     };
     // one branch for all products: the rare ones stay out of the way of the instruction fetch
-    if (KIND != kInt8 && tail && pc.r.n > 1 && any_wild<C>(mine + stage * C::kStage + C::kHalf))
+    if (KIND != kInt8 && tail && some_unseen(p, pc.r) && any_wild<C>(mine + stage * C::kStage + C::kHalf))
       products(std::true_type());
     else
       products(std::false_type());

@@ -224,6 +224,10 @@ __device__ __forceinline__ uint32_t seen32(const Params& p, const Request& r, in
   return seen & bits;
 }
 
+// Whether some of a request's rows may not see some of its new tokens: without
+// a mask a single one sees itself, with one it need not.
+__device__ __forceinline__ bool some_unseen(const Params& p, const Request& r) { return r.n > 1 || p.mask != nullptr; }
+
 // ---------------------------------------------------------------- arithmetic
 __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2^-22 relative, 0 for -inf
   float y;

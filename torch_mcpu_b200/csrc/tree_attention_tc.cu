@@ -261,7 +261,7 @@ struct Loader {
 
   // Value tiles with new tokens that some of the request's rows may not see: a lane looks through the values it wrote.
   __device__ __forceinline__ void clean_tail(const Pieces& pc, int tile, uint32_t s) const {
-    if (C::KIND == kInt8 || pc.r.n <= 1 || (pc.tile0 + tile + 1) * kTile <= pc.r.len - pc.r.n) return;
+    if (C::KIND == kInt8 || !some_unseen(p, pc.r) || (pc.tile0 + tile + 1) * kTile <= pc.r.len - pc.r.n) return;
     constexpr int kChunks = C::D * (C::kSmall ? 1 : 2) / 16, kRows = 32 / kChunks, kSteps = C::kRowsPerWarp / kRows;
     constexpr uint32_t kExp = C::BF16 ? 0x7F807F80u : 0x7C007C00u;
     const int c = lane % kChunks, row0 = C::kRowsPerWarp * lw + lane / kChunks;
@@ -1006,7 +1006,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
             if (!ok) break;
             ks = scales + ring * 2 * kTile, vs = ks + kTile;
           }
-          if (C::KIND != kInt8 && tail && r.n > 1) {
+          if (C::KIND != kInt8 && tail && some_unseen(p, r)) {
             // the value tile's notes are needed: its place in the order of loads
             const uint32_t n = kv + (j + lead < pc.nt ? lead + 2 * j : pc.nt + j);
             slot = n % C::kSlots;
@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
           if (tail) {
 #pragma unroll
             for (int c = 0; c < 4; ++c) seen[c] = row_ok ? seen32(p, r, t, qi, key0 + 32 * c) : kFull;
-            if (C::KIND != kInt8 && r.n > 1) {
+            if (C::KIND != kInt8 && some_unseen(p, r)) {
               int any = 0;
 #pragma unroll
               for (int i = 0; i < C::kLoadWarps; ++i) any |= bars->wild[slot][i];
