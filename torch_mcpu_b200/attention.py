@@ -47,6 +47,19 @@ def _fail(op: str, why: str):
     raise RuntimeError(f"{op}: {why}")
 
 
+# Keys of a configuration's scaling that each kind reads, beside its name; those of _SAID say what the call says already, or
+# nothing about the table
+_SCALINGS = {
+    "default": (),
+    "linear": ("factor", "original_max_position_embeddings"),
+    "dynamic": ("factor", "original_max_position_embeddings"),
+    "llama3": ("factor", "original_max_position_embeddings", "low_freq_factor", "high_freq_factor"),
+    "yarn": ("factor", "original_max_position_embeddings", "beta_fast", "beta_slow", "attention_factor", "mscale",
+             "mscale_all_dim", "truncate"),
+}
+_SAID = ("rope_type", "type", "rope_theta", "partial_rotary_factor", "finetuned")
+
+
 def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000.0, scaling: dict | None = None,
                          device=None) -> torch.Tensor:
     """The float32 [max_position, rotary_dim] table of rotary_embedding: row p
@@ -62,15 +75,30 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
       "llama3"   f_i where its wavelength is below o / "high_freq_factor",
                  f_i / s above o / "low_freq_factor", blended between
       "yarn"     blended over the dimensions that turn between "beta_fast"
-                 (32) and "beta_slow" (1) times in o positions; cos and sin
-                 times "attention_factor" (0.1 ln s + 1)."""
+                 (32) and "beta_slow" (1) times in o positions, from whole
+                 dimensions unless "truncate" is false; cos and sin times
+                 "attention_factor", else, with m(c) = 0.1 c ln s + 1 for
+                 s > 1, m("mscale") / m("mscale_all_dim") where both are
+                 given, else m(1)
+    Keys whose value is None count as not given; "rope_theta" must be base, and
+    "partial_rotary_factor" is what rotary_dim says.  Other keys are refused:
+    they would make another table."""
     op = "rotary_cos_sin_cache"
     if rotary_dim <= 0 or rotary_dim % 2 or max_position <= 0 or base <= 0:
         _fail(op, "max_position and base must be positive, rotary_dim even and positive")
-    scaling = dict(scaling or {})
+    scaling = {k: v for k, v in (scaling or {}).items() if v is not None}
     kind = scaling.get("rope_type", scaling.get("type", "default"))
-    if kind not in ("default", "linear", "dynamic", "llama3", "yarn"):
+    if kind not in _SCALINGS:
         _fail(op, f"unknown rope_type {kind!r}")
+    if scaling.get("type", kind) != kind:
+        _fail(op, f"rope_type is {kind!r}, type {scaling['type']!r}")
+    unknown = [k for k in scaling if k not in _SCALINGS[kind] and k not in _SAID]
+    if unknown:
+        _fail(op, f"{kind} scaling does not know {', '.join(map(str, unknown))}")
+    if float(scaling.get("rope_theta", base)) != float(base):
+        _fail(op, f"rope_theta is {scaling['rope_theta']}, base {base}")
+    if ("mscale" in scaling) != ("mscale_all_dim" in scaling):
+        _fail(op, "mscale and mscale_all_dim are given together: what one alone means differs between models")
     factor = float(scaling.get("factor", 1.0))
     if factor <= 0:
         _fail(op, "factor must be positive")
@@ -100,11 +128,17 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
         def dim_of(turns: float) -> float:
             return rotary_dim * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        lo = max(math.floor(dim_of(float(scaling.get("beta_fast", 32)))), 0)
-        hi = min(math.ceil(dim_of(float(scaling.get("beta_slow", 1)))), rotary_dim - 1)
+        lo, hi = dim_of(float(scaling.get("beta_fast", 32))), dim_of(float(scaling.get("beta_slow", 1)))
+        if scaling.get("truncate", True):
+            lo, hi = math.floor(lo), math.ceil(hi)
+        lo, hi = max(lo, 0), min(hi, rotary_dim - 1)
         ramp = ((torch.arange(rotary_dim // 2, dtype=torch.float64) - lo) / max(hi - lo, 0.001)).clamp(0, 1)
         inv = inv / factor * ramp + inv * (1 - ramp)
-        amp = float(scaling.get("attention_factor") or (0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0))
+        def grown(c: float) -> float:
+            return 0.1 * c * math.log(factor) + 1.0 if factor > 1 else 1.0
+
+        amp = float(scaling.get("attention_factor", 0)) or grown(float(scaling.get("mscale", 1))) / grown(
+            float(scaling.get("mscale_all_dim", 0)))
     angle = torch.arange(max_position, dtype=torch.float64)[:, None] * inv[None]
     table = torch.cat([angle.cos() * amp, angle.sin() * amp], dim=1).float()
     return table if device is None else table.to(device)
