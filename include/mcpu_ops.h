@@ -521,11 +521,11 @@ OPENREG_EXPORT orError_t mcpu_gather_cache(const mcpuKvCache* cache, const int32
  * h / (num_heads / kv_heads).
  *   out = softmax(scale * q . k) v over the keys seen, rounded once;
  *   lse (fp32 [num_tokens, num_heads], or NULL) = log sum exp of the scores.
- * Errors of out: its own rounding; the probabilities' (over 8-bit caches their
- * products with the value scales, w) rounding to the products' type, fp16 over
- * 8-bit caches, where what lies below 2^-21 of a query's largest w is off by
- * at most 2^-32 of that, whatever the scales of its keys; probabilities below
- * 2^-126 of the largest count as 0.
+ * Errors of out: its own rounding; the rounding of the probabilities (over
+ * 8-bit caches, of their products with the value scales) to the type of the
+ * second product, which is bf16 for bf16 caches, else fp16, where what lies
+ * below 2^-21 of a query's largest is off by at most 2^-32 of that, whatever
+ * the scales of its keys; probabilities below 2^-126 of the largest count as 0.
  * A query that sees no key gives zeros and -inf; what unseen keys, values and
  * slots behind seq_lens hold (NaN included) does not matter.  Tokens outside
  * every request are left as they are.  A request that does not fit (lengths

@@ -171,3 +171,28 @@ def test_scale_of_a_draft_matters_to_its_rows_alone(kind, counts, heads):
         results.append(ops.tree_attention(q, kc, vc, bt, sl, cu, max(counts), 0.125, tree_mask=mask, k_scale=ks, v_scale=vs))
     for r in results[1:]:
         assert torch.equal(r[~seen_by], results[0][~seen_by])
+
+
+@pytest.mark.parametrize("kind,scales", [("same", "none"), (torch.float8_e4m3fn, "tensor"), (torch.int8, "head"), (torch.int8, "token")])
+@pytest.mark.parametrize("shape", list(SHAPES))
+def test_many_faint_probabilities(kind, scales, shape):
+    """One key takes next to all of the probability and has values of 0; the others, 2^-26 each, make the output: their
+    products count although they lie below the normal range of fp16 beside the largest."""
+    lens, counts, heads = SHAPES[shape]
+    size, kv = 64, 4 if "many" in shape else 2
+    x = make(13, lens, counts, heads, kv, size, 16, torch.float16, kind, scales)
+    q, kc, vc, ks, vs, bt, sl, cu = x
+    held = kc.dtype
+    q[:] = 0
+    q[..., 0] = 4.0
+    kc.copy_(torch.zeros(kc.shape, device="cuda").to(held))
+    vc.copy_((vc.float().abs() + 0.25).to(held))
+    top = 36.0 if kind == "same" else ref.LARGEST[kind]
+    if ks is not None:
+        ks[:] = 36.0 / top
+    for b, n in enumerate(lens):
+        p, s = place_of(x, b, n // 2 if counts[b] < n // 2 else 0)
+        kc[int(p), s, :, 0] = torch.tensor(top, device="cuda").to(held)  # its score: 4 * 36 / 8 = 18 above the others
+        vc[int(p), s] = torch.zeros(kv, size, device="cuda").to(held)
+    got, lse = ops.tree_attention(q, kc, vc, bt, sl, cu, max(counts), 0.125, k_scale=ks, v_scale=vs, return_lse=True)
+    check(x, 0.125, None, got, lse)

@@ -128,6 +128,7 @@ struct Cfg {
   static constexpr int KIND = KIND_, D = D_, STAGES = STAGES_, ROWS = ROWS_;
   static constexpr bool kSmall = KIND != kSame;
   static constexpr bool kBf16 = !kSmall && std::is_same<T, __nv_bfloat16>::value;  // type of the products
+  static constexpr float kBias = kSmall || kBf16 ? 0.0f : 15.0f;                   // probabilities are held times 2^kBias
   static constexpr int kRow = D * (kSmall ? 1 : 2);                                // bytes of a key row
   static constexpr int kChunks = kRow / 16;
   static constexpr int KW = kSmall ? 32 : 16;                                      // keys of a warp's step
@@ -481,7 +482,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
           for (int x = 0; x < 4; ++x) acc[i][x] *= by[x >> 1];
       }
     }
-    const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+    const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0] - C::kBias, m[1] == -INFINITY ? 0.0f : m[1] - C::kBias};
     float wtop[2] = {0.0f, 0.0f};  // products with the values' scales
 #pragma unroll
     for (int n = 0; n < kNT; ++n) {
@@ -597,6 +598,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
       for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(kFull, l[e], 1);
         l[e] += __shfl_xor_sync(kFull, l[e], 2);
+        l[e] *= exp2_whole(-C::kBias);
         if (j4 == 0) warp_ml[warp * kRows + g + 8 * e] = make_float4(m[e], l[e], 0.0f, 0.0f);
       }
       __syncthreads();
@@ -614,7 +616,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
         f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
         m[e] = mm;
         l[e] = ll;
-        if (C::kSmall) f[e] *= exp2_whole(-lift[e]);
+        f[e] *= C::kSmall ? exp2_whole(-lift[e]) : exp2_whole(-C::kBias);
         if (whole) f[e] = ll == 0.0f ? 0.0f : f[e] / ll;
       }
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * kRows;
@@ -895,7 +897,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
           for (int x = 0; x < 4; ++x) acc[i][x] *= by[x & 1];
       }
     }
-    const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0], m[1] == -INFINITY ? 0.0f : m[1]};
+    const float sub[2] = {m[0] == -INFINITY ? 0.0f : m[0] - C::kBias, m[1] == -INFINITY ? 0.0f : m[1] - C::kBias};
     float wtop[2] = {0.0f, 0.0f};  // products with the values' scales
 #pragma unroll
     for (int t = 0; t < kMT; ++t)
@@ -995,6 +997,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
       for (int e = 0; e < 2; ++e) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[e] += __shfl_xor_sync(kFull, l[e], o);
+        l[e] *= exp2_whole(-C::kBias);
         if (g == 0) warp_ml[warp * 8 + 2 * j4 + e] = make_float4(m[e], l[e], 0.0f, 0.0f);
       }
       __syncthreads();
@@ -1012,7 +1015,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
         f[e] = m[e] == -INFINITY ? 1.0f : exp2_fast(m[e] - mm);
         m[e] = mm;
         l[e] = ll;
-        if (C::kSmall) f[e] *= exp2_whole(-lift[e]);
+        f[e] *= C::kSmall ? exp2_whole(-lift[e]) : exp2_whole(-C::kBias);
         if (whole) f[e] = ll == 0.0f ? 0.0f : f[e] / ll;
       }
       const long long part = (static_cast<long long>(blockIdx.x) * 2 + slot) * 8;

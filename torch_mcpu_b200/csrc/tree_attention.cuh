@@ -234,6 +234,13 @@ __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2^-22 rela
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// Probabilities that are multiplied as fp16 are held times 2^15 (times 2^7 where
+// the maximum they refer to may be 2^8 too low), which is taken off the sums at
+// the end: those down to 2^-29 (2^-21) of the largest keep fp16's precision,
+// and what lies below is off by at most 2^-40 (2^-32) of it.  Held as they are,
+// those below 2^-25 were gone from the outputs though not from the sum that
+// these are divided by.
+//
 // Products of probabilities and value scales, w_j = p_j s_j, are multiplied as
 // fp16, relative to a reference of each row: w_j 2^lift.  The lift brings the
 // largest product so far of the keys the row sees to 2^7 .. 2^8; it falls, with

@@ -61,6 +61,7 @@ struct Cfg {
   static constexpr bool BF16 = BF16_;    // type of the products; 8-bit caches: fp16
   static constexpr bool TOKEN = TOKEN_;  // a scale for every token and head
   static constexpr bool kSmall = KIND != kSame;
+  static constexpr float kBias = TOKEN || BF16 ? 0.0f : 7.0f;  // probabilities are held times 2^kBias
   static constexpr int kLoadWarps = 4;
   static constexpr int kRowsPerWarp = kTile / kLoadWarps;
   static constexpr int kWarps = kSoftWarps + kLoadWarps + 4;
@@ -673,7 +674,7 @@ struct Soft {
     l *= alpha;
     if constexpr (!C::TOKEN) by = alpha;
     if (!first && __any_sync(kFull, by != 1.0f)) scale_outputs(by);
-    const float sub = m == -INFINITY ? 0.0f : m;
+    const float sub = m == -INFINITY ? 0.0f : m - C::kBias;
     const unsigned long long q2 = pair(qscale, qscale), m2 = pair(-sub, -sub);
     float up = C::TOKEN ? exp2_whole(lift) : 1.0f;
     unsigned long long sum0 = pair(0.0f, 0.0f), sum1 = sum0;
@@ -1060,11 +1061,14 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
       }
       if (!ok) break;
       tc_fence_after();
+      so.l *= exp2_whole(-C::kBias);
       float f0, f1 = 0.0f, m = so.m, l = so.l;
       int c0 = 0, c1 = D / 32;
       uint32_t o0 = so.tmem_o, o1 = so.tmem_o;
       bool noted0 = so.wild, noted1 = false;
-      const float vscale = C::kSmall ? (C::TOKEN ? exp2_whole(-so.lift) : p.c.v_scale[h * p.c.v_scale_stride[2]]) : 1.0f;
+      const float vscale = C::TOKEN    ? exp2_whole(-so.lift)
+                           : C::kSmall ? p.c.v_scale[h * p.c.v_scale_stride[2]] * exp2_whole(-C::kBias)
+                                       : exp2_whole(-C::kBias);
       f0 = vscale;
       if (nq == 1) {
         // each stream's warps write half of the dimensions, joining both streams' sums
