@@ -450,10 +450,11 @@ OPENREG_EXPORT orError_t mcpu_vllm_bad_words(void* logits, int dtype, int64_t nu
  * mcpu_rotary_embedding: for each token t, with row = cos_sin_cache[
  *   positions[t]] (fp32, rotary_dim/2 cosines then rotary_dim/2 sines), every
  *   head's pairs (a, b) -- (x[i], x[i + rotary_dim/2]) when is_neox, else
- *   (x[2i], x[2i+1]) -- become (a cos - b sin, b cos + a sin), rounded once,
- *   in place; dimensions from rotary_dim on are not touched.  Heads lie at
- *   token and head strides (elements), dimensions contiguous; query and key
- *   do not overlap; num_kv_heads may be 0.  fp32, bf16 or fp16.  A position
+ *   (x[2i], x[2i+1]) -- become (a cos - b sin, b cos + a sin), in place: bf16
+ *   and fp16 from 64 bits, rounded once; fp32 in fp32, a cos - b sin off by at
+ *   most 2^-24 (|b sin| + |result|).  Dimensions from rotary_dim on are not
+ *   touched.  Heads lie at token and head strides (elements), dimensions
+ *   contiguous; query and key do not overlap; num_kv_heads may be 0.  A position
  *   outside [0, max_position) leaves the token and sets mcpu_device_error.
  *
  * mcpu_rotary_reshape_and_cache: query rotated in place; the rotated key

@@ -49,3 +49,28 @@ def test_read_back_of_rows_that_are_not_finite():
     ops.gather_cache(cache, cache, bt, cu, *out, scale, scale)
     for o in out:
         assert o[0, 0, 0].isinf() and o[0, 0, 3].isnan() and o[1].isnan().all() and torch.isfinite(o[2:]).all()
+
+
+@pytest.mark.parametrize("neox", [True, False])
+@pytest.mark.parametrize("tokens,heads,size,part", [(200, 5, 128, 128), (33, 3, 192, 64), (17, 2, 80, 20)])
+def test_rotation_in_32_bits(neox, tokens, heads, size, part):
+    """fma(a, c, -rn(b s)): half a step of b s and half a step of the result, also where the result all but vanishes."""
+    g = gen(tokens)
+    x = torch.randn(tokens, heads, size, generator=g, device="cuda")
+    x[:, 0] *= 1e-3
+    pos = torch.randint(0, 4000, (tokens,), generator=g, device="cuda")
+    tab = ops.rotary_cos_sin_cache(4000, part, device="cuda")
+    half = part // 2
+    row = tab[pos]
+    a, b = (slice(0, half), slice(half, part)) if neox else (slice(0, part, 2), slice(1, part, 2))
+    x[:, 1, a], x[:, 1, b] = row[:, half:], row[:, :half] * (1 + 2.0 ** -14)  # pairs next to (sin, cos)
+    want = ref.rotated(x, pos, tab, neox)
+    sin = row[:, None, half:].double().abs()
+    second = torch.zeros_like(want)
+    second[..., a], second[..., b] = x[..., b].double().abs() * sin, x[..., a].double().abs() * sin
+    rest = x[..., part:].clone()
+    ops.rotary_embedding(pos, x, None, size, tab, neox)
+    # a rounding of a value is off by 2^-24 of it; the result's is taken of what it is before, 2^-24 of the product away
+    bound = 2.0 ** -24 * (second + want.abs()) * (1 + 2.0 ** -23) + 2.0 ** -48 * second
+    assert ((x.double() - want).abs()[..., :part] <= bound[..., :part]).all()
+    assert torch.equal(x[..., part:], rest)

@@ -150,7 +150,9 @@ def rotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: torch.Te
     head of query and key ([tokens, heads * head_size] or [tokens, heads,
     head_size], float32, bfloat16 or float16; views of a larger tensor are
     fine) are rotated by their position's angles.  is_neox: pairs (i, i +
-    rotary_dim / 2), else (2i, 2i + 1).  Results are rounded once."""
+    rotary_dim / 2), else (2i, 2i + 1).  bfloat16 and float16 results are
+    64-bit ones rounded once; float32 ones, a cos - b sin, are off by at most
+    2^-24 (|b sin| + |result|)."""
     (_ops or _native()).rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox)
 
 
