@@ -55,6 +55,13 @@ inline void no_gradient(const at::Tensor& t, const char* op, const char* name) {
 inline void no_gradient(const Opt& t, const char* op, const char* name) {
   if (t) no_gradient(*t, op, name);
 }
+inline void no_gradient(const at::Tensor& key_cache, const at::Tensor& value_cache, const Opt& k_scale, const Opt& v_scale,
+                        const char* op) {
+  no_gradient(key_cache, op, "key_cache");
+  no_gradient(value_cache, op, "value_cache");
+  no_gradient(k_scale, op, "k_scale");
+  no_gradient(v_scale, op, "v_scale");
+}
 
 // [tokens, heads * head_size] or [tokens, heads, head_size] with contiguous heads.
 struct Heads {
@@ -175,6 +182,7 @@ inline void rotary_embedding(const Api& api, const at::Tensor& positions, const 
   same_device(table, query, op, "cos_sin_cache");
   no_gradient(query, op, "query");
   no_gradient(key, op, "key");
+  no_gradient(table, op, "cos_sin_cache");
   const auto type = query.scalar_type();
   TORCH_CHECK((type == at::kFloat || type == at::kBFloat16 || type == at::kHalf) && (!key || key->scalar_type() == type), op,
               ": query and key must both be float32, bfloat16 or float16");
@@ -218,6 +226,8 @@ inline void write(const Api& api, const Opt& positions, const Opt& query, const 
   no_gradient(query, op, "query");
   no_gradient(key, op, "key");
   no_gradient(value, op, "value");
+  no_gradient(table, op, "cos_sin_cache");
+  no_gradient(key_cache, value_cache, k_scale, v_scale, op);
   const auto type = key.scalar_type();
   TORCH_CHECK(value.scalar_type() == type && (!query || query->scalar_type() == type), op,
               ": query, key and value must have one type");
@@ -264,6 +274,9 @@ inline void gather_cache(const Api& api, const at::Tensor& key_cache, const at::
   same_device(k_scale, key_cache, op, "k_scale");
   same_device(v_scale, key_cache, op, "v_scale");
   same_device(seq_starts, key_cache, op, "seq_starts");
+  no_gradient(key_cache, value_cache, k_scale, v_scale, op);
+  no_gradient(key_out, op, "key_out");
+  no_gradient(value_out, op, "value_out");
   TORCH_CHECK(value_out.scalar_type() == key_out.scalar_type() && value_out.sizes() == key_out.sizes(), op,
               ": key_out and value_out must have one shape and type");
   const mcpuKvCache c = cache_of(key_cache, value_cache, k_scale, v_scale, key_out.scalar_type(), false, op);
@@ -301,6 +314,7 @@ inline std::tuple<at::Tensor, at::Tensor> tree_attention(
   same_device(out_given, query, op, "out");
   no_gradient(query, op, "query");
   no_gradient(out_given, op, "out");
+  no_gradient(key_cache, value_cache, k_scale, v_scale, op);
   const auto type = query.scalar_type();
   const mcpuKvCache c = cache_of(key_cache, value_cache, k_scale, v_scale, type, false, op);
   TORCH_CHECK(query.dim() == 3 && query.size(2) == c.head_size && query.stride(2) == 1, op,
