@@ -50,3 +50,44 @@ def test_every_tensor_that_requires_a_gradient_is_refused():
                 call({**tensors, name: leaf})
             with torch.inference_mode():
                 call({**tensors, name: leaf})
+
+
+def test_written_tensors_count_as_changed():
+    """A tensor that autograd has saved and a call has written since is noticed by the backward pass."""
+    for call, tensors, written in calls():
+        for name in written:
+            x = tensors[name]
+            weight = torch.ones(x.shape, device="cuda", requires_grad=True)
+            if x.dtype != torch.float32:
+                weight = torch.ones(x.shape, dtype=x.dtype, device="cuda", requires_grad=True)
+            y = (weight * x).sum()
+            call(tensors)
+            with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+                y.backward()
+        for name, x in tensors.items():
+            before = x._version
+            call(tensors)
+            assert (x._version > before) == (name in written), name
+
+
+def test_tensors_of_inference_mode_are_taken():
+    with torch.inference_mode():
+        for call, tensors, _ in calls():
+            call(tensors)
+    for call, tensors, _ in calls():
+        with torch.inference_mode():
+            call({n: x.clone() for n, x in tensors.items()})
+
+
+def test_written_mcpu_tensors_count_as_changed():
+    import torch_mcpu_b200.device  # noqa: F401
+
+    q, k, tab = (x.cpu().to("mcpu") for x in calls()[0][1].values())
+    pos = torch.arange(3).to("mcpu")
+    for x in (q, k, tab):
+        assert not x.requires_grad
+    before = [x._version for x in (q, k, tab)]
+    torch.ops.mcpu.rotary_embedding(pos, q, k, 64, tab, True)
+    assert [x._version > b for x, b in zip((q, k, tab), before)] == [True, True, False]
+    with pytest.raises(RuntimeError, match="requires a gradient"):
+        torch.ops.mcpu.rotary_embedding(pos, q, k, 64, tab.clone().requires_grad_(), True)

@@ -63,6 +63,12 @@ inline void no_gradient(const at::Tensor& key_cache, const at::Tensor& value_cac
   no_gradient(v_scale, op, "v_scale");
 }
 
+// A tensor the call has written: autograd, where it has saved it for another operator, is to know.  Tensors of inference
+// mode count no versions.
+inline void written(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // [tokens, heads * head_size] or [tokens, heads, head_size] with contiguous heads.
 struct Heads {
   int64_t tokens = 0, heads = 0, token_stride = 0, head_stride = 0;
@@ -206,6 +212,8 @@ inline void rotary_embedding(const Api& api, const at::Tensor& positions, const 
                 type == at::kFloat ? MCPU_FLOAT32 : type == at::kHalf ? MCPU_FLOAT16 : MCPU_BFLOAT16,
                 api.stream(query.device().index())),
      op);
+  written(query);
+  if (key) written(*key);
 }
 
 // table without a value: the write alone.
@@ -259,6 +267,13 @@ inline void write(const Api& api, const Opt& positions, const Opt& query, const 
                table ? table->const_data_ptr<float>() : nullptr, table ? table->size(0) : 0, is_neox, half_code(type, op),
                slot_mapping.const_data_ptr<int64_t>(), &c, api.stream(key.device().index())),
      op);
+  if (table && query) written(*query);
+  written(key_cache);
+  written(value_cache);
+  if (c.scale_mode == MCPU_KV_SCALE_TOKEN) {
+    written(*k_scale);
+    written(*v_scale);
+  }
 }
 
 inline void gather_cache(const Api& api, const at::Tensor& key_cache, const at::Tensor& value_cache,
@@ -295,6 +310,8 @@ inline void gather_cache(const Api& api, const at::Tensor& key_cache, const at::
                 key_out.data_ptr(), value_out.data_ptr(), key_out.size(0), half_code(key_out.scalar_type(), op),
                 api.stream(key_cache.device().index())),
      op);
+  written(key_out);
+  written(value_out);
 }
 
 inline std::tuple<at::Tensor, at::Tensor> tree_attention(
@@ -357,6 +374,7 @@ inline std::tuple<at::Tensor, at::Tensor> tree_attention(
                 tree_mask ? tree_mask->const_data_ptr<int64_t>() : nullptr, mask_stride, words, static_cast<float>(scale),
                 work.data_ptr(), need, api.stream(query.device().index())),
      op);
+  if (out_given) written(out);
   return {out, lse};
 }
 
