@@ -91,3 +91,80 @@ def test_written_mcpu_tensors_count_as_changed():
     assert [x._version > b for x, b in zip((q, k, tab), before)] == [True, True, False]
     with pytest.raises(RuntimeError, match="requires a gradient"):
         torch.ops.mcpu.rotary_embedding(pos, q, k, 64, tab.clone().requires_grad_(), True)
+
+
+def test_written_tensors_that_overlap_with_an_offset_are_refused():
+    g = gen(4)
+    half = torch.bfloat16
+    pos = torch.arange(3, device="cuda")
+    bt = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    tab = table(8, 64)
+    packed = randn(g, 3, 8, 64, dtype=half)
+    k, v = randn(g, 3, 2, 64, dtype=half), randn(g, 3, 2, 64, dtype=half)
+    pages = randn(g, 9, 16, 2, 64, dtype=half)
+    ks = torch.zeros(9, 16, 2, device="cuda")
+    kc8, vc8 = (torch.zeros(4, 16, 2, 64, dtype=torch.int8, device="cuda") for _ in range(2))
+    rows = randn(g, 8, 2, 64, dtype=half)
+    for call, why in (
+            (lambda: ops.rotary_embedding(pos, packed[:, :4], packed[:, 3:5], 64, tab), "query and key are written"),
+            (lambda: ops.rotary_embedding(pos, packed[:, 2:6], packed[:, 1:3], 64, tab), "query and key are written"),
+            (lambda: ops.rotary_embedding(pos[:2], packed[:2, :4], packed[1:, 2:4], 64, tab), "query and key are written"),
+            (lambda: ops.rotary_embedding(pos, packed.view(3, 512)[:, :256], packed.view(3, 512)[:, 248:504], 64, tab),
+             "query and key are written"),
+            (lambda: ops.reshape_and_cache(k, v, pages[:4], pages[3:7], pos), "key_cache and value_cache are written"),
+            (lambda: ops.reshape_and_cache(k, v, pages[:8:2], pages[2::2], pos), "key_cache and value_cache are written"),
+            (lambda: ops.reshape_and_cache(k, v, pages.view(-1)[:8192].view(4, 16, 2, 64), pages.view(-1)[2048 - 64:][:8192].view(4, 16, 2, 64), pos),
+             "key_cache and value_cache are written"),
+            (lambda: ops.reshape_and_cache(k, v, kc8, vc8, pos, ks[:4], ks[2:6]), "k_scale and v_scale are written"),
+            (lambda: ops.rotary_reshape_and_cache(pos, packed[:, :4], packed[:, 3:5], v, tab, True, pages[:4], pages[4:8], pos),
+             "query is written"),
+            (lambda: ops.rotary_reshape_and_cache(pos, packed[:, :4], k, packed[:, 2:4], tab, True, pages[:4], pages[4:8], pos),
+             "query is written"),
+            (lambda: ops.gather_cache(pages[:4], pages[4:8], bt, cu, rows[:3], rows[2:5]), "key_out and value_out are written"),
+            (lambda: ops.tree_attention(rows[:3], pages[:4], pages[4:8], bt, cu[1:], cu, 3, 0.1, out=rows[1:4]), "out is written")):
+        before = [x.clone() for x in (packed, pages, ks, rows)]
+        with pytest.raises(RuntimeError, match=why):
+            call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(before, (packed, pages, ks, rows)))
+
+
+def test_interleaved_tensors_are_taken():
+    """Views of one tensor that share no element, in the layouts that programs have."""
+    g = gen(5)
+    half = torch.bfloat16
+    pos = torch.arange(3, device="cuda")
+    bt = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    cu = torch.tensor([0, 3], dtype=torch.int32, device="cuda")
+    tab = table(8, 64)
+    packed = randn(g, 3, 8, 64, dtype=half)
+    flat = packed.view(3, 512)
+    by_group = randn(g, 3, 2, 4, 64, dtype=half)  # key heads, then its two query heads, key and value
+    want = packed.clone()
+    ops.rotary_embedding(pos, want, None, 64, tab)
+    for q, k in ((packed[:, :4], packed[:, 4:6]), (packed[:, 2:], packed[:, :2]), (flat[:, :256], flat[:, 256:384]),
+                 (packed[..., 0:8:2, :], packed[..., 1:8:2, :]), (by_group[:, :, 0], by_group[:, :, 2]),
+                 (packed.transpose(0, 1)[:3, :3], packed.transpose(0, 1)[3:6, 3:6])):
+        ops.rotary_embedding(pos[:q.shape[0]], q, k, 64, tab)
+    ops.rotary_reshape_and_cache(pos, packed[:, :4], packed[:, 4:6], packed[:, 6:], tab, True,
+                                 *randn(g, 2, 4, 16, 2, 64, dtype=half).unbind(0), pos)
+    k, v = randn(g, 3, 2, 64, dtype=half), randn(g, 3, 2, 64, dtype=half)
+    for both in (randn(g, 2, 4, 16, 2, 64, dtype=half), randn(g, 4, 2, 16, 2, 64, dtype=half).transpose(0, 1),
+                 randn(g, 4, 16, 2, 2, 64, dtype=half).permute(2, 0, 1, 3, 4), randn(g, 4, 16, 2, 2, 64, dtype=half).permute(3, 0, 1, 2, 4),
+                 randn(g, 4, 16, 2, 128, dtype=half).view(4, 16, 2, 2, 64).permute(3, 0, 1, 2, 4),
+                 randn(g, 2, 4, 2, 16, 64, dtype=half).transpose(2, 3), randn(g, 4, 2, 2, 16, 64, dtype=half).permute(1, 0, 3, 2, 4)):
+        ops.reshape_and_cache(k, v, both[0], both[1], pos)
+        outs = randn(g, 2, 3, 2, 64, dtype=half)
+        ops.gather_cache(both[0], both[1], bt, cu, outs[0], outs[1])
+        assert torch.equal(outs[0], k) and torch.equal(outs[1], v)
+    kc8, vc8 = (torch.zeros(4, 16, 2, 64, dtype=torch.int8, device="cuda") for _ in range(2))
+    for s in (torch.zeros(4, 16, 2, 2, device="cuda").unbind(-1), torch.zeros(4, 2, 16, 2, device="cuda").unbind(1),
+              torch.zeros(2, 4, 16, 2, device="cuda").unbind(0)):
+        ops.reshape_and_cache(k, v, kc8, vc8, pos, *s)
+    shifted = randn(g, 4, 4, 64, dtype=half)
+    ops.rotary_embedding(pos, shifted[:3, :2], shifted[1:, 2:], 64, tab)  # a token further in the other heads
+    q = packed[:, 2:6]
+    want = ops.tree_attention(q, both[0], both[1], bt, cu[1:], cu, 3, 0.1)
+    assert torch.equal(ops.tree_attention(q, both[0], both[1], bt, cu[1:], cu, 3, 0.1, out=packed[:, 6:].repeat(1, 2, 1)), want)
+    assert torch.equal(ops.tree_attention(q, both[0], both[1], bt, cu[1:], cu, 3, 0.1, out=q), want)  # in place of the queries

@@ -219,7 +219,7 @@ def tree_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: to
     Returns the output (`out` where given), with return_lse also the float32
     [tokens, heads] logarithms of the softmax sums.  A token that sees nothing
     gives zeros and -inf; tokens outside every request are left as they are
-    (undefined in an output made by the call).  out overlaps no other tensor
-    of the call."""
+    (undefined in an output made by the call).  out may be query itself and
+    overlaps no other tensor of the call."""
     return (_ops or _native()).tree_attention(query, key_cache, value_cache, block_table, seq_lens, cu_query_lens,
                                               max_query_len, scale, tree_mask, k_scale, v_scale, out, return_lse)

@@ -98,6 +98,66 @@ void disjoint(std::array<std::pair<int64_t, int64_t>, N> dims, int64_t reach, co
   }
 }
 
+// Where a strided tensor lies, in bytes: its first address, what is contiguous, and (stride, count) of the dimensions outside
+// of that, largest stride first.
+struct Place {
+  intptr_t at = 0;
+  int64_t inner = 0;
+  std::array<std::pair<int64_t, int64_t>, 3> dims{};
+  int n = 0;
+  int64_t reach(int from) const {
+    int64_t r = inner;
+    for (int i = from; i < n; ++i) r += (dims[i].second - 1) * dims[i].first;
+    return r;
+  }
+};
+template <size_t N>
+Place place_of(const at::Tensor& t, const std::array<std::pair<int64_t, int64_t>, N>& dims, int64_t inner) {
+  const int64_t size = static_cast<int64_t>(t.element_size());
+  Place p;
+  p.at = reinterpret_cast<intptr_t>(t.const_data_ptr());
+  p.inner = inner * size;
+  for (const auto& d : dims) {
+    if (d.second == 0) p.inner = 0;
+    if (d.second > 1) p.dims[p.n++] = {d.first * size, d.second};
+  }
+  std::sort(p.dims.begin(), p.dims.begin() + p.n, [](const auto& a, const auto& b) { return a.first > b.first; });
+  while (p.n > 0 && p.dims[p.n - 1].first == p.inner) p.inner *= p.dims[--p.n].second;
+  return p;
+}
+inline int64_t down_div(int64_t a, int64_t b) { return a >= 0 ? a / b : -((-a + b - 1) / b); }
+// Whether the dimensions of a from i on and those of b from j on, b lying `off` bytes behind a, share a byte.  Dimensions of
+// one stride are taken together, so views of one tensor are decided in a few steps; others after `steps` count as apart.
+inline bool meet(const Place& a, int i, const Place& b, int j, int64_t off, int& steps) {
+  if (off >= a.reach(i) || -off >= b.reach(j)) return false;
+  if (i == a.n && j == b.n) return true;
+  if (--steps < 0) return false;
+  const int64_t sa = i < a.n ? a.dims[i].first : 0, sb = j < b.n ? b.dims[j].first : 0;
+  if (sa < sb) return meet(b, j, a, i, -off, steps);
+  const bool both = sa == sb;
+  const int64_t ra = a.reach(i + 1), rb = b.reach(both ? j + 1 : j);
+  // the k-th of a against b, or of one stride those that are k apart
+  const int64_t from = std::max(down_div(off - ra, sa) + 1, both ? 1 - b.dims[j].second : 0);
+  const int64_t to = std::min(down_div(off + rb - 1, sa), a.dims[i].second - 1);
+  for (int64_t k = from; k <= to; ++k)
+    if (meet(a, i + 1, b, both ? j + 1 : j, off - k * sa, steps)) return true;
+  return false;
+}
+inline bool overlap(const Place& a, const Place& b) {
+  if (a.inner == 0 || b.inner == 0) return false;
+  int steps = 4096;
+  return meet(a, 0, b, 0, b.at - a.at, steps);
+}
+using Dim = std::pair<int64_t, int64_t>;
+inline Place place_of(const at::Tensor& t, const Heads& h, int64_t inner) {
+  return place_of<2>(t, {Dim{h.token_stride, h.tokens}, Dim{h.head_stride, h.heads}}, inner);
+}
+inline Place place_of(const at::Tensor& t) {  // up to 3 dimensions and a contiguous one
+  std::array<Dim, 3> dims{};
+  for (int i = 0; i < 3; ++i) dims[i] = i < t.dim() ? Dim{t.stride(i), t.size(i)} : Dim{0, 1};
+  return place_of<3>(t, dims, t.dim() > 3 ? t.size(3) : 1);
+}
+
 inline int half_code(at::ScalarType t, const char* op) {
   TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf, op, ": bfloat16 or float16 tensors expected, got ", t);
   return t == at::kHalf ? MCPU_FLOAT16 : MCPU_BFLOAT16;
@@ -135,9 +195,7 @@ inline mcpuKvCache cache_of(const at::Tensor& key_cache, const at::Tensor& value
   TORCH_CHECK((ks[3] == 1 && vs[3] == 1) || sz[3] <= 1, op, ": cache rows must be contiguous");
   TORCH_CHECK(sz[1] < (1LL << 31) && sz[2] < (1LL << 31) && sz[3] < (1LL << 31), op, ": bad cache sizes");
   if (writes) {
-    TORCH_CHECK(key_cache.numel() == 0 || key_cache.data_ptr() != value_cache.data_ptr(), op,
-                ": key_cache and value_cache are written and must not overlap");
-    using Dim = std::pair<int64_t, int64_t>;
+    TORCH_CHECK(!overlap(place_of(key_cache), place_of(value_cache)), op, ": key_cache and value_cache are written and must not overlap");
     disjoint<3>({Dim{ks[0], sz[0]}, Dim{ks[1], sz[1]}, Dim{ks[2], sz[2]}}, sz[3], op, "key_cache");
     disjoint<3>({Dim{vs[0], sz[0]}, Dim{vs[1], sz[1]}, Dim{vs[2], sz[2]}}, sz[3], op, "value_cache");
   }
@@ -161,9 +219,7 @@ inline mcpuKvCache cache_of(const at::Tensor& key_cache, const at::Tensor& value
     c.scale_mode = MCPU_KV_SCALE_TOKEN;
     for (int i = 0; i < 3; ++i) c.k_scale_stride[i] = k_scale->stride(i), c.v_scale_stride[i] = v_scale->stride(i);
     if (writes) {
-      TORCH_CHECK(k_scale->numel() == 0 || k_scale->data_ptr() != v_scale->data_ptr(), op,
-                  ": k_scale and v_scale are written and must not overlap");
-      using Dim = std::pair<int64_t, int64_t>;
+      TORCH_CHECK(!overlap(place_of(*k_scale), place_of(*v_scale)), op, ": k_scale and v_scale are written and must not overlap");
       const int64_t *k3 = c.k_scale_stride, *v3 = c.v_scale_stride;
       disjoint<3>({Dim{k3[0], sz[0]}, Dim{k3[1], sz[1]}, Dim{k3[2], sz[2]}}, 1, op, "k_scale");
       disjoint<3>({Dim{v3[0], sz[0]}, Dim{v3[1], sz[1]}, Dim{v3[2], sz[2]}}, 1, op, "v_scale");
@@ -196,13 +252,12 @@ inline void rotary_embedding(const Api& api, const at::Tensor& positions, const 
   check_table(positions, q.tokens, table, op);
   const int64_t part = table.size(1);
   TORCH_CHECK(part <= head_size, op, ": rotary_dim ", part, " exceeds head_size ", head_size);
-  using Dim = std::pair<int64_t, int64_t>;
   disjoint<2>({Dim{q.token_stride, q.tokens}, Dim{q.head_stride, q.heads}}, part, op, "query");
   Heads k;
   if (key) {
     k = heads_of(*key, head_size, op, "key");
     TORCH_CHECK(k.tokens == q.tokens, op, ": key has ", k.tokens, " tokens, query ", q.tokens);
-    TORCH_CHECK(key->numel() == 0 || key->data_ptr() != query.data_ptr(), op, ": query and key are written and must not overlap");
+    TORCH_CHECK(!overlap(place_of(query, q, part), place_of(*key, k, part)), op, ": query and key are written and must not overlap");
     disjoint<2>({Dim{k.token_stride, k.tokens}, Dim{k.head_stride, k.heads}}, part, op, "key");
   }
   ok(api,
@@ -256,8 +311,10 @@ inline void write(const Api& api, const Opt& positions, const Opt& query, const 
     if (query) {
       q = heads_of(*query, c.head_size, op, "query");
       TORCH_CHECK(q.tokens == k.tokens, op, ": query has ", q.tokens, " tokens, key ", k.tokens);
-      using Dim = std::pair<int64_t, int64_t>;
       disjoint<2>({Dim{q.token_stride, q.tokens}, Dim{q.head_stride, q.heads}}, part, op, "query");
+      const Place place = place_of(*query, q, part);
+      TORCH_CHECK(!overlap(place, place_of(key, k, c.head_size)) && !overlap(place, place_of(value, v, c.head_size)), op,
+                  ": query is written and must not overlap key or value");
     }
   }
   ok(api,
@@ -298,7 +355,7 @@ inline void gather_cache(const Api& api, const at::Tensor& key_cache, const at::
   TORCH_CHECK(key_out.dim() == 3 && key_out.size(1) == c.kv_heads && key_out.size(2) == c.head_size &&
                   key_out.is_contiguous() && value_out.is_contiguous(),
               op, ": outputs must be contiguous [tokens, ", c.kv_heads, ", ", c.head_size, "] tensors");
-  TORCH_CHECK(key_out.numel() == 0 || key_out.data_ptr() != value_out.data_ptr(), op,
+  TORCH_CHECK(!overlap(place_of<0>(key_out, {}, key_out.numel()), place_of<0>(value_out, {}, value_out.numel())), op,
               ": key_out and value_out are written and must not overlap");
   check_block_table(block_table, op);
   const int64_t batch = block_table.size(0), width = block_table.size(1);
@@ -357,8 +414,10 @@ inline std::tuple<at::Tensor, at::Tensor> tree_attention(
     out = *out_given;
     TORCH_CHECK(out.sizes() == query.sizes() && out.scalar_type() == type && out.stride(2) == 1, op, ": out must be a ", type, " ",
                 query.sizes(), " tensor with contiguous heads");
-    using Dim = std::pair<int64_t, int64_t>;
     disjoint<2>({Dim{out.stride(0), tokens}, Dim{out.stride(1), heads}}, c.head_size, op, "out");
+    TORCH_CHECK((out.const_data_ptr() == query.const_data_ptr() && out.strides() == query.strides()) ||
+                    !overlap(place_of(out), place_of(query)),
+                op, ": out is written and must be query itself or not overlap it");
   } else {
     out = at::empty(query.sizes(), query.options());
   }
