@@ -168,3 +168,19 @@ def test_interleaved_tensors_are_taken():
     want = ops.tree_attention(q, both[0], both[1], bt, cu[1:], cu, 3, 0.1)
     assert torch.equal(ops.tree_attention(q, both[0], both[1], bt, cu[1:], cu, 3, 0.1, out=packed[:, 6:].repeat(1, 2, 1)), want)
     assert torch.equal(ops.tree_attention(q, both[0], both[1], bt, cu[1:], cu, 3, 0.1, out=q), want)  # in place of the queries
+
+
+def test_arguments_that_are_no_truth_values():
+    import numpy as np
+
+    neither = np.zeros(2)
+    q = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    kc, vc = (torch.zeros(4, 16, 2, 64, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    pos, tab = torch.arange(3, device="cuda"), table(8, 64)
+    bt = torch.arange(4, dtype=torch.int32, device="cuda")[None]
+    cu, sl = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0, 3], [3]))
+    for call, name in ((lambda: ops.rotary_embedding(pos, q, None, 64, tab, neither), "is_neox"),
+                       (lambda: ops.rotary_reshape_and_cache(pos, q, q.clone(), q.clone(), tab, neither, kc, vc, pos), "is_neox"),
+                       (lambda: ops.tree_attention(q, kc, vc, bt, sl, cu, 3, 0.1, return_lse=neither), "return_lse")):
+        with pytest.raises(RuntimeError, match=name + " must be a bool"):
+            call()

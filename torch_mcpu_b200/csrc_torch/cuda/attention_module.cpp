@@ -62,6 +62,14 @@ double number(PyObject* o, const char* op, const char* name) {
   }
   return v;
 }
+bool truth(PyObject* o, const char* op, const char* name) {
+  const int v = PyObject_IsTrue(o);
+  if (v < 0) {
+    PyErr_Clear();
+    TORCH_CHECK(false, op, ": ", name, " must be a bool");
+  }
+  return v == 1;
+}
 void arguments(Py_ssize_t n, Py_ssize_t want, const char* op) {
   TORCH_CHECK(n == want, op, ": ", want, " arguments expected, got ", n);
   TORCH_CHECK(g_api.rotary != nullptr, op, ": the device library is not loaded");
@@ -91,7 +99,7 @@ PyObject* py_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
   OnDevice on(q);
   mcpu_torch::attention::rotary_embedding(g_api, tensor(a[0], op, "positions"), q, optional(a[2], op, "key"),
                                           integer(a[3], op, "head_size"), tensor(a[4], op, "cos_sin_cache"),
-                                          PyObject_IsTrue(a[5]) == 1);
+                                          truth(a[5], op, "is_neox"));
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -103,7 +111,7 @@ PyObject* py_write(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const at::Tensor& key = tensor(a[2], op, "key");
   OnDevice on(key);
   mcpu_torch::attention::write(g_api, optional(a[0], op, "positions"), optional(a[1], op, "query"), key, tensor(a[3], op, "value"),
-                               optional(a[4], op, "cos_sin_cache"), PyObject_IsTrue(a[5]) == 1, tensor(a[6], op, "key_cache"),
+                               optional(a[4], op, "cos_sin_cache"), truth(a[5], op, "is_neox"), tensor(a[6], op, "key_cache"),
                                tensor(a[7], op, "value_cache"), tensor(a[8], op, "slot_mapping"), optional(a[9], op, "k_scale"),
                                optional(a[10], op, "v_scale"));
   Py_RETURN_NONE;
@@ -129,7 +137,7 @@ PyObject* py_attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   arguments(n, 13, op);
   const at::Tensor& q = tensor(a[0], op, "query");
   OnDevice on(q);
-  const bool lse = PyObject_IsTrue(a[12]) == 1;
+  const bool lse = truth(a[12], op, "return_lse");
   const auto r = mcpu_torch::attention::tree_attention(
       g_api, q, tensor(a[1], op, "key_cache"), tensor(a[2], op, "value_cache"), tensor(a[3], op, "block_table"),
       tensor(a[4], op, "seq_lens"), tensor(a[5], op, "cu_query_lens"), integer(a[6], op, "max_query_len"),
