@@ -286,7 +286,7 @@ __global__ void __maxnreg__(224) attend_kernel(const __grid_constant__ Params p)
   locate<kThreads>(
       p,
       [&](int tot) {
-        share = share_of(p, tot, gridDim.x);
+        share = share_of(tot, gridDim.x);
         return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
       },
       red, total, unit, b0, before);
@@ -707,7 +707,7 @@ __global__ void __launch_bounds__(kThreads, 3) attend8_kernel(const __grid_const
   locate<kThreads>(
       p,
       [&](int tot) {
-        share = share_of(p, tot, gridDim.x);
+        share = share_of(tot, gridDim.x);
         return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
       },
       red, total, unit, b0, before);
@@ -1207,7 +1207,6 @@ orError_t launch(Params& p, cudaStream_t st, int sms, int* grid) {
   p.rows_log2 = C::ROWS == 8 ? 3 : 4;
   p.keys_log2 = C::TN == 64 ? 6 : 7;
   p.item_cost = 2;  // measured: 0 293 us, 2 276 us, 5 275 us for a decoding batch of all lengths
-  p.min_share = 1;  // units a block takes at least; 2 and 4 cost a single request 0.6 and 1.9 us
   kernel<<<*grid, kThreads, C::kSmem, st>>>(p);
   return from_cuda(cudaGetLastError(), "tree_attention launch");
 }

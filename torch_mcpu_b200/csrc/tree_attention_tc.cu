@@ -822,7 +822,7 @@ __global__ void __launch_bounds__(C::kThreads, 1) attend_tc_kernel(const __grid_
   locate<C::kThreads>(
       p,
       [&](int tot) {
-        share = share_of(p, tot, gridDim.x);
+        share = share_of(tot, gridDim.x);
         return static_cast<int>(min(static_cast<long long>(blockIdx.x) * share, 2147483647ll));
       },
       red, total, unit, b0, before);
@@ -1208,7 +1208,6 @@ orError_t launch_tc(Params& p, int D, long long rows, cudaStream_t st, int sms, 
   p.rows_log2 = nq == 1 ? 7 : 8;
   p.keys_log2 = 7;
   p.item_cost = 4;  // measured: 0 340 us, 4 216 us, 10 228 us for full trees of all lengths
-  p.min_share = 1;
   *grid = sms;
   return D == 64 ? tc::pick<64>(p, nq, st, sms) : tc::pick<128>(p, nq, st, sms);
 }
