@@ -184,3 +184,26 @@ def test_arguments_that_are_no_truth_values():
                        (lambda: ops.tree_attention(q, kc, vc, bt, sl, cu, 3, 0.1, return_lse=neither), "return_lse")):
         with pytest.raises(RuntimeError, match=name + " must be a bool"):
             call()
+
+
+def test_expanded_tensors():
+    """Dimensions of stride 0: refused where they are written, taken where they are read."""
+    g = gen(6)
+    half = torch.bfloat16
+    pos, tab = torch.arange(3, device="cuda"), table(8, 64)
+    kc, vc = (randn(g, 4, 16, 2, 64, dtype=half) for _ in range(2))
+    one = randn(g, 1, 1, 64, dtype=half)
+    k = one.expand(3, 2, 64)  # the same row for all heads and tokens
+    ops.reshape_and_cache(k, k, kc, vc, pos)
+    assert torch.equal(kc[0, :3], k) and torch.equal(vc[0, :3], k)
+    q = randn(g, 3, 4, 64, dtype=half)
+    ops.rotary_reshape_and_cache(pos, q, k, k, tab, True, kc, vc, pos)
+    inside = q[:1, :1].expand(3, 2, 64)  # a row of the queries that are rotated
+    with pytest.raises(RuntimeError, match="query is written"):
+        ops.rotary_reshape_and_cache(pos, q, inside, k, tab, True, kc, vc, pos)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.reshape_and_cache(k, k, kc[:1].expand(4, 16, 2, 64), kc, pos)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.reshape_and_cache(k, k, kc[:, :, :1].expand(4, 16, 2, 64), kc[:, :, 1:].expand(4, 16, 2, 64), pos)
+    with pytest.raises(RuntimeError, match="overlap"):
+        ops.rotary_embedding(pos, q, inside, 64, tab)

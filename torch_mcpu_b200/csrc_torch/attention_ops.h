@@ -119,7 +119,7 @@ Place place_of(const at::Tensor& t, const std::array<std::pair<int64_t, int64_t>
   p.inner = inner * size;
   for (const auto& d : dims) {
     if (d.second == 0) p.inner = 0;
-    if (d.second > 1) p.dims[p.n++] = {d.first * size, d.second};
+    if (d.second > 1 && d.first != 0) p.dims[p.n++] = {d.first * size, d.second};  // an expanded dimension adds no place
   }
   std::sort(p.dims.begin(), p.dims.begin() + p.n, [](const auto& a, const auto& b) { return a.first > b.first; });
   while (p.n > 0 && p.dims[p.n - 1].first == p.inner) p.inner *= p.dims[--p.n].second;
@@ -134,12 +134,12 @@ inline bool meet(const Place& a, int i, const Place& b, int j, int64_t off, int&
   if (--steps < 0) return false;
   const int64_t sa = i < a.n ? a.dims[i].first : 0, sb = j < b.n ? b.dims[j].first : 0;
   if (sa < sb) return meet(b, j, a, i, -off, steps);
-  const bool both = sa == sb;
+  const bool both = sa == sb;  // not 0: one of the two has a dimension left
   const int64_t ra = a.reach(i + 1), rb = b.reach(both ? j + 1 : j);
   // the k-th of a against b, or of one stride those that are k apart
   const int64_t from = std::max(down_div(off - ra, sa) + 1, both ? 1 - b.dims[j].second : 0);
   const int64_t to = std::min(down_div(off + rb - 1, sa), a.dims[i].second - 1);
-  for (int64_t k = from; k <= to; ++k)
+  for (int64_t k = from; k <= to && steps >= 0; ++k)
     if (meet(a, i + 1, b, both ? j + 1 : j, off - k * sa, steps)) return true;
   return false;
 }
