@@ -1,12 +1,6 @@
-"""The attention path of a serving step: rotary positions, the paged key /
-value cache, quantised as it is written, its read-back, and attention over it
-for single tokens and drafted trees.
-
-Like vLLM's: rotary_embedding's arguments (the table is float32 here), the
-cache's layout [num_blocks, block_size, kv_heads, head_size], its slots and
-block tables.  Not like vLLM's: the cache write takes scales and no name of a
-cache type, gather_cache reads keys and values in one call, and scales may be
-held per token and head.
+"""The attention path of a serving step, with vLLM's signatures: rotary
+positions, the paged key / value cache, quantised as it is written, its
+read-back, and attention over it for single tokens and drafted trees.
 
 Like torch_mcpu_b200.ops (which re-exports every function here), each call
 checks its arguments, enqueues on torch's current stream of the tensors'
@@ -152,11 +146,11 @@ def rotary_cos_sin_cache(max_position: int, rotary_dim: int, base: float = 10000
 
 def rotary_embedding(positions: torch.Tensor, query: torch.Tensor, key: torch.Tensor | None, head_size: int,
                      cos_sin_cache: torch.Tensor, is_neox: bool = True) -> None:
-    """Rotary positions with vLLM's arguments, in place: the first rotary_dim =
-    cos_sin_cache.size(1) dimensions of every head of query and key ([tokens,
-    heads * head_size] or [tokens, heads, head_size], float32, bfloat16 or
-    float16; views of a larger tensor are fine) are rotated by their position's
-    angles.  is_neox: pairs (i, i + rotary_dim / 2), else (2i, 2i + 1).  bfloat16 and float16 results are
+    """Rotary positions with vLLM's argument order, in place: the first rotary_dim = cos_sin_cache.size(1) dimensions of every
+    head of query and key ([tokens, heads * head_size] or [tokens, heads,
+    head_size], float32, bfloat16 or float16; views of a larger tensor are
+    fine) are rotated by their position's angles.  is_neox: pairs (i, i +
+    rotary_dim / 2), else (2i, 2i + 1).  bfloat16 and float16 results are
     64-bit ones rounded once; float32 ones, a cos - b sin, are off by at most
     2^-24 (|b sin| + |result|)."""
     (_ops or _native()).rotary_embedding(positions, query, key, head_size, cos_sin_cache, is_neox)

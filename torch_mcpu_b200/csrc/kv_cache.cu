@@ -511,11 +511,8 @@ struct GatherParams {
 
 // q * s cut off to fp32, the last bit set where that lost something, so that
 // the rounding to T is that of the product (rounded to fp32 first, one in some
-// 10^5 lies on a border of T and goes the wrong way).  For plain scales: 0, or
-// in 2^-100 .. 2^100, where what was lost is an fp32 value.
-__device__ __forceinline__ bool plain_scale(float s) {
-  return (fabsf(s) >= 7.9e-31f && fabsf(s) <= 1.2e30f) || s == 0.0f;
-}
+// 10^5 lies on a border of T and goes the wrong way).  s in 2^-100 .. 2^100:
+// what was lost is an fp32 value.
 __device__ __forceinline__ float product_to_odd(float q, float s) {
   const float p = __fmul_rz(q, s);
   return __fmaf_rn(q, s, -p) != 0.0f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
@@ -569,9 +566,8 @@ __device__ __noinline__ void dequantise16_exact(const uint8_t* q, float s, T* ou
 // One warp per token: finds its sequence (32-way search of the offsets, one
 // step up to 32 sequences), looks its page up once, and moves all heads' key
 // and value, 16 values per lane and step.  Bound by HBM: 698 MB, mostly bf16
-// written, in 139 us (5.0 TB/s of 6.5 copied; 124 with products rounded twice);
-// 777 tokens in 3.8 us.  With the rare scales told apart inside the loop: 133 to
-// 160 us, and 4.2 us for the short one.
+// written, in 134 us (5.2 TB/s of 6.5 copied; 120 us with products rounded
+// twice, 160 with a branch each for keys and values).
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ GatherParams p) {
   const long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
@@ -616,7 +612,6 @@ __global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ Gat
   const float* vs = KIND == kSame ? nullptr : p.c.v_scale + id * p.c.v_scale_stride[0] + inside * p.c.v_scale_stride[1];
   T* kout = static_cast<T*>(p.key_out) + out_at;
   T* vout = static_cast<T*>(p.value_out) + out_at;
-  bool far = false;
 #pragma unroll 2
   for (int c = lane; c < chunks; c += 32) {
     const int h = c / per_row, d = (c - h * per_row) * 16;
@@ -630,18 +625,13 @@ __global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ Gat
     } else {
       const uint4 a = *ksrc, e = *vsrc;
       const float sk = ks[h * p.c.k_scale_stride[2]], sv = vs[h * p.c.v_scale_stride[2]];
-      dequantise16<T, KIND>(a, sk, kd);
-      dequantise16<T, KIND>(e, sv, vd);
-      far |= !plain_scale(sk) || !plain_scale(sv);
-    }
-  }
-  if constexpr (KIND != kSame) {
-    if (!far) return;
-    for (int c = lane; c < chunks; c += 32) {  // scales of other sizes: again, behind the loop that all others take
-      const int h = c / per_row, d = (c - h * per_row) * 16;
-      const float sk = ks[h * p.c.k_scale_stride[2]], sv = vs[h * p.c.v_scale_stride[2]];
-      if (!plain_scale(sk)) dequantise16_exact<T, KIND>(kin + h * p.c.key_stride[2] + d, sk, kout + 16ll * c);
-      if (!plain_scale(sv)) dequantise16_exact<T, KIND>(vin + h * p.c.value_stride[2] + d, sv, vout + 16ll * c);
+      if (fminf(sk, sv) >= 7.9e-31f && fmaxf(sk, sv) <= 1.2e30f) {
+        dequantise16<T, KIND>(a, sk, kd);
+        dequantise16<T, KIND>(e, sv, vd);
+      } else {
+        dequantise16_exact<T, KIND>(reinterpret_cast<const uint8_t*>(ksrc), sk, reinterpret_cast<T*>(kd));
+        dequantise16_exact<T, KIND>(reinterpret_cast<const uint8_t*>(vsrc), sv, reinterpret_cast<T*>(vd));
+      }
     }
   }
 }

@@ -1,5 +1,5 @@
-// The attention path on the mcpu device: the arguments of the Python functions
-// (torch_mcpu_b200/attention.py), bodies in attention_ops.h.
+// The attention path on the mcpu device: schemas with vLLM's argument order,
+// bodies in attention_ops.h.
 #include <torch/library.h>
 
 #include "attention_ops.h"
