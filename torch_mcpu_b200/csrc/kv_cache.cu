@@ -511,11 +511,20 @@ struct GatherParams {
 
 // q * s cut off to fp32, the last bit set where that lost something, so that
 // the rounding to T is that of the product (rounded to fp32 first, one in some
-// 10^5 lies on a border of T and goes the wrong way).  s in 2^-100 .. 2^100:
-// what was lost is an fp32 value.
-__device__ __forceinline__ float product_to_odd(float q, float s) {
-  const float p = __fmul_rz(q, s);
-  return __fmaf_rn(q, s, -p) != 0.0f ? __uint_as_float(__float_as_uint(p) | 1u) : p;
+// 10^5 lies on a border of T and goes the wrong way); two at a time.  s in
+// 2^-100 .. 2^100: what was lost is an fp32 value.
+__device__ __forceinline__ void products_to_odd(float& lo, float& hi, float s) {
+  unsigned long long q, p, r, s2, n2;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(q) : "f"(lo), "f"(hi));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(s2) : "f"(s));
+  asm("mov.b64 %0, {%1, %1};" : "=l"(n2) : "f"(-s));
+  asm("mul.rz.f32x2 %0, %1, %2;" : "=l"(p) : "l"(q), "l"(s2));
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(q), "l"(n2), "l"(p));
+  float r0, r1;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p));
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r0), "=f"(r1) : "l"(r));
+  if (r0 != 0.0f) lo = __uint_as_float(__float_as_uint(lo) | 1u);
+  if (r1 != 0.0f) hi = __uint_as_float(__float_as_uint(hi) | 1u);
 }
 
 // Dequantises 16 values held in 16 bytes to two 16-byte vectors of T.
@@ -538,7 +547,7 @@ __device__ __forceinline__ void dequantise16(const uint4& q, float s, uint4* out
       lo = __uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7650)) - 8388736.0f;
       hi = __uint_as_float(__byte_perm(biased, 0x4B000000u, 0x7651)) - 8388736.0f;
     }
-    lo = product_to_odd(lo, s), hi = product_to_odd(hi, s);
+    products_to_odd(lo, hi, s);
     if constexpr (std::is_same<T, __nv_bfloat16>::value) {
       o[i] = pack_bf16x2(lo, hi);
     } else {
@@ -566,8 +575,8 @@ __device__ __noinline__ void dequantise16_exact(const uint8_t* q, float s, T* ou
 // One warp per token: finds its sequence (32-way search of the offsets, one
 // step up to 32 sequences), looks its page up once, and moves all heads' key
 // and value, 16 values per lane and step.  Bound by HBM: 698 MB, mostly bf16
-// written, in 134 us (5.2 TB/s of 6.5 copied; 120 us with products rounded
-// twice, 160 with a branch each for keys and values).
+// written, in 130 us (5.4 TB/s of 6.5 copied; 124 with products rounded twice;
+// 133 with products one at a time, 160 with a branch each for keys and values).
 template <typename T, int KIND>
 __global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ GatherParams p) {
   const long long t = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5);
