@@ -58,7 +58,9 @@ def _use_shared_libstdcxx_compiler() -> None:
 
 def build(verbose: bool = False) -> str:
     _cabi.build()
-    if up_to_date():
+    # a process that runs on the extension cannot load another build of it: its
+    # registrations are there already, and torch ends the process
+    if up_to_date() or (f"{__package__}.device" in sys.modules and os.path.exists(SO)):
         return SO
     _use_shared_libstdcxx_compiler()
     from torch.utils import cpp_extension
