@@ -430,8 +430,8 @@ OPENREG_EXPORT orError_t mcpu_vllm_bad_words(void* logits, int dtype, int64_t nu
  * cache that is quantised as it is written, its read-back, and attention over
  * it for single tokens, chains and trees of drafted tokens.  No counterpart
  * in the reference, whose mcpu device leaves attention to vLLM's CPU backend;
- * the Python signatures follow vLLM's (rotary_embedding, reshape_and_cache,
- * gather_cache).
+ * the Python rotary_embedding takes vLLM's arguments, and the cache has its
+ * layout; the other calls are of their own.
  *
  * mcpuKvCache: key and value are [num_blocks, block_size, kv_heads,
  *   head_size] with strides (in elements) for block, slot in the block and

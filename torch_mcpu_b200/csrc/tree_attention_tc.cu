@@ -27,7 +27,9 @@
 // which fp16 and bf16 hold and fp32 sums take without loss.
 //
 // Measured: 16 requests of up to 8192 tokens with trees of 61, 64 / 8 heads of
-// 128, bf16 (133 GFLOP) 212 us, 630 TFLOP/s; 6 requests of up to 32768 with
+// 128, bf16 (133 GFLOP) 211 us, 632 TFLOP/s, in a burst, and 245 us, 545
+// TFLOP/s, in seconds of calls, when the power cap holds the SM clock at 1.7 GHz
+// instead of 1.96; 6 requests of up to 32768 with
 // trees of 13, 32 / 8 heads, fp16 over int8 (279 MB) 137 us, 2.0 TB/s.  The
 // tensor pipe is 36 % and the exponentials' 31 % busy: each stream's chain
 // (scores, softmax, product) is what a pair of tiles waits for, about 3500
