@@ -250,7 +250,7 @@ __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2^-22 rela
 // instead of 137 for the small trees of tree_attention_tc.cu.)  A reference
 // taken from the scales alone, the largest of a step, lost whole outputs beside
 // one key of a large scale and no probability.  Lifts, and the maxima they go
-// with, are whole numbers: the scaling is exact.
+// with, are whole numbers, so that sums are scaled by powers of two.
 constexpr float kLift = 100.0f;    // the highest; where no product above 0 has been seen
 constexpr float kRoom = 32768.0f;  // of 65504
 __device__ __forceinline__ float exp2_whole(float e) {  // -126 .. 127
